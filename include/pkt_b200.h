@@ -139,6 +139,8 @@ typedef struct pkt_dp_bias_args {
 #define PKT_DTYPE_BF16 1
 #define PKT_DTYPE_TF32 2 /* fp32 storage, TF32 tensor-core inputs */
 #define PKT_DTYPE_F32 3  /* fp32 output storage */
+#define PKT_DTYPE_E4M3 4 /* 8-bit float: 4 exponent bits, largest value 448, no infinity */
+#define PKT_DTYPE_E5M2 5 /* 8-bit float: 5 exponent bits, largest finite value 57344 */
 
 #define PKT_MAJOR_K 0  /* operand stored [rows][K] (K contiguous) */
 #define PKT_MAJOR_MN 1 /* operand stored [K][rows] (rows contiguous) */
@@ -274,6 +276,164 @@ int pkt_axpy_noalloc(const float* x, float* y, float a, long long n, void* strea
  * PKT_DEV_TIMEOUT_PIPE or PKT_DEV_TIMEOUT_DEPS here. The next pkt_axpy_noalloc
  * call clears the words. */
 int pkt_axpy_noalloc_status(int* code, int* task_index, int* detail);
+
+/* ---- stand-alone operators ---------------------------------------------- */
+/* These run on the current device and in the order of `stream`; every pointer is
+ * memory of that device (checked: a host pointer or another device's memory is
+ * PKT_ERR_ARGS). They allocate nothing and may be captured into a CUDA graph.
+ * A descriptor is read during the call only. Outputs must not overlap inputs
+ * unless an operator says so. No counterpart in pkt. */
+
+/* Layer norm over the last dimension of [rows, cols]. Statistics and sums are
+ * fp32; each result is rounded to its type once.
+ *   forward   mean = sum x / C, rstd = 1/sqrt(sum (x-mean)^2 / C + eps),
+ *             y = (x - mean) rstd gamma + beta
+ *   backward  dx, and the sums over all rows dgamma = sum dy (x-mean) rstd,
+ *             dbeta = sum dy, from x, dy and the forward pass's mean and rstd
+ * Any cols >= 1 and row strides >= cols (16-byte aligned rows are fastest).
+ * y may be x, dx may be dy or x, with the same row stride. The columns of a
+ * padded row past cols are neither read nor written. rows = 0 is allowed (dgamma
+ * and dbeta are then zero). */
+typedef struct pkt_layernorm_desc {
+  long long rows;
+  int cols;
+  int dtype;         /* of x, y, dy, dx: PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
+  int param_dtype;   /* of gamma, beta: PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
+  float eps;         /* forward */
+  const void* x;     /* row stride ldx, in elements (so the other ld*) */
+  long long ldx;
+  const void* gamma; /* [cols], null: ones */
+  const void* beta;  /* forward: [cols], null: zeros */
+  void* y;           /* forward */
+  long long ldy;
+  float* mean;       /* [rows]: forward writes it (may be null), backward reads it */
+  float* rstd;
+  const void* dy;    /* backward */
+  long long lddy;
+  void* dx;          /* backward, may be null */
+  long long lddx;
+  float* dgamma;     /* backward: [cols], overwritten; may be null */
+  float* dbeta;
+  void* workspace;   /* backward: pkt_layernorm_backward_workspace bytes, used during the
+                        call alone; calls that overlap on the GPU (two graphs, two
+                        streams) need one each */
+  size_t workspace_bytes;
+} pkt_layernorm_desc;
+int pkt_layernorm_forward(const pkt_layernorm_desc* d, void* stream);
+/* Workspace of a backward call with these rows and cols on the current device. */
+int pkt_layernorm_backward_workspace(const pkt_layernorm_desc* d, size_t* bytes);
+int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream);
+
+/* Block-scaled 8-bit floats: a block of values with the largest magnitude `amax`
+ * is held as q = round(x * (most / amax)) and scale = amax / most, where `most` is
+ * the type's largest value (448 or 57344); x is about q * scale. Rounding is to
+ * nearest, ties to even. A block with amax < 2^-100 is zeros with scale 0; a block
+ * that holds an infinity or NaN has a non-finite scale. */
+
+/* Quantises x [rows, cols]:
+ *   q  [rows, cols]: blocks of 128 columns x block_rows rows,
+ *      scale [ceil(cols/128), ceil(rows/block_rows)]: one row of scales per 128 columns
+ *   qt [cols, rows]: the transposed matrix quantised the same way (blocks of 128 rows
+ *      of x x block_rows columns), scale_t [ceil(rows/128), ceil(cols/block_rows)]
+ * Either may be left out (null); both together read x once. These are operands of
+ * pkt_fp8_gemm whose summed dimension is the contiguous one. Bytes of padded rows
+ * past the matrix are not written. */
+typedef struct pkt_fp8_quantize_desc {
+  int rows, cols;
+  int dtype;        /* of x: PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
+  int q_dtype;      /* PKT_DTYPE_E4M3 or PKT_DTYPE_E5M2 */
+  int block_rows;   /* 1 (activations, gradients) or 128 (weights) */
+  const void* x;
+  long long ldx;
+  void* q;          /* 16-byte aligned, ldq a multiple of 16 */
+  long long ldq;
+  float* scale;
+  long long ld_scale;
+  void* qt;         /* 16-byte aligned, ldqt a multiple of 16 */
+  long long ldqt;
+  float* scale_t;
+  long long ld_scale_t;
+} pkt_fp8_quantize_desc;
+int pkt_fp8_quantize(const pkt_fp8_quantize_desc* d, void* stream);
+
+/* out[m, n] = sum over blocks kb of 128 along K of
+ *             scale_a[kb, m / a_block_rows] * scale_b[kb, n / b_block_rows]
+ *             * sum over k in kb of a[m, k] * b[n, k]
+ * on the tensor cores (tcgen05, fp32 accumulators); the scales are applied to each
+ * block's fp32 sum and the blocks are added in fp32. Any M, N, K >= 0 (K = 0:
+ * zeros); a and b are 16-byte aligned with row strides that are multiples of 16.
+ * The result of a call does not depend on timing. */
+typedef struct pkt_fp8_gemm_desc {
+  int M, N, K;
+  int a_dtype, b_dtype; /* PKT_DTYPE_E4M3 or PKT_DTYPE_E5M2, each on its own */
+  const void* a;        /* [M, K], row stride lda */
+  long long lda;
+  const float* scale_a; /* [ceil(K/128), ceil(M/a_block_rows)], row stride ld_scale_a */
+  long long ld_scale_a;
+  int a_block_rows;     /* 1 or 128 */
+  const void* b;        /* [N, K], row stride ldb */
+  long long ldb;
+  const float* scale_b; /* [ceil(K/128), ceil(N/b_block_rows)], row stride ld_scale_b */
+  long long ld_scale_b;
+  int b_block_rows;     /* 1 or 128 */
+  void* out;            /* [M, N], row stride ldo */
+  long long ldo;
+  int out_dtype;        /* PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
+} pkt_fp8_gemm_desc;
+int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream);
+/* Whether a wait inside a pkt_fp8_gemm launch on the current device ran out of time
+ * since the last call (PKT_DEV_OK or PKT_DEV_TIMEOUT_PIPE; its output is then not
+ * valid). Synchronises the device and clears the word. */
+int pkt_fp8_gemm_status(int* code);
+
+/* AdamW over many tensors in one launch. For step t of a tensor, with g = grad *
+ * gradient scale:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay)
+ *           - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32. state_dtype PKT_DTYPE_F32 keeps m and v as fp32. PKT_DTYPE_E4M3 keeps m
+ * and sqrt(v) as block-scaled 8-bit floats (blocks of 128 consecutive values from
+ * the tensor's start, scales m_scale / v_scale): 2 1/16 bytes per parameter instead
+ * of 8; a positive sqrt(v) is held as at least the smallest 8-bit value, so that it
+ * never divides by eps alone. States start as zeros (scales too).
+ * The plan keeps the pointers and, on the device, the step count: replaying a
+ * captured step advances it. Steps of a plan are ordered by the caller (one
+ * stream, or events). */
+typedef struct pkt_adamw pkt_adamw;
+typedef struct pkt_adamw_tensor {
+  void* param;           /* [n], param_dtype, updated in place */
+  const void* grad;      /* [n], grad_dtype; null: the tensor is left alone */
+  void* m;               /* [n], state_dtype */
+  void* v;               /* [n], state_dtype */
+  float* m_scale;        /* 8-bit states: [ceil(n/128)] */
+  float* v_scale;
+  void* copy_bf16;       /* optional [n]: the new parameters rounded to bf16 */
+  long long n;
+  float weight_decay;
+  int pad;
+} pkt_adamw_tensor;
+typedef struct pkt_adamw_config {
+  int num_tensors;
+  const pkt_adamw_tensor* tensors; /* read by pkt_adamw_create only */
+  int param_dtype;                 /* PKT_DTYPE_F32 or PKT_DTYPE_BF16 */
+  int grad_dtype;                  /* PKT_DTYPE_F32 or PKT_DTYPE_BF16 */
+  int state_dtype;                 /* PKT_DTYPE_F32 or PKT_DTYPE_E4M3 */
+  double beta1, beta2, eps;
+  long long step;                  /* steps taken before the first call */
+} pkt_adamw_config;
+int pkt_adamw_create(int device, const pkt_adamw_config* cfg, pkt_adamw** out);
+int pkt_adamw_destroy(pkt_adamw* h);
+/* One step. `scales` (device memory, may be null): lr is multiplied by scales[0] and
+ * the gradients by scales[1], read when the step runs (a schedule or a clipping
+ * factor computed on the device, also under graph replay). grad_scale multiplies
+ * the gradients too. */
+int pkt_adamw_step(pkt_adamw* h, float lr, float grad_scale, const float* scales, void* stream);
+/* New gradient pointers (num_tensors of them), for steps enqueued from now on. Not
+ * inside a stream capture: steps captured before then read the new pointers too. */
+int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream);
+/* Steps taken: set (stream-ordered), and read (synchronises the stream). */
+int pkt_adamw_set_step(pkt_adamw* h, long long step, void* stream);
+int pkt_adamw_get_step(pkt_adamw* h, long long* step, void* stream);
 
 /* ---- MLP training engine (the hot path) -------------------------------- */
 typedef struct pkt_mlp pkt_mlp;

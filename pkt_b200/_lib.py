@@ -14,6 +14,7 @@ c_u16, c_u32, c_u64 = ctypes.c_uint16, ctypes.c_uint32, ctypes.c_uint64
 
 PKT_OK, PKT_ERR_ARGS, PKT_ERR_CUDA, PKT_ERR_TIMEOUT, PKT_ERR_OPCODE = 0, -1, -2, -3, -4
 PKT_DTYPE_BF16, PKT_DTYPE_TF32, PKT_DTYPE_F32 = 1, 2, 3
+PKT_DTYPE_E4M3, PKT_DTYPE_E5M2 = 4, 5
 PKT_MAJOR_K, PKT_MAJOR_MN = 0, 1
 EPI_STORE, EPI_BIAS_ACT, EPI_MSE, EPI_DGRAD_RELU, EPI_WGRAD_SGD, EPI_WGRAD_STORE = range(6)
 DEV_OK, DEV_TIMEOUT_DEPS, DEV_TIMEOUT_PIPE, DEV_BAD_OPCODE, DEV_BAD_ARGS = range(5)
@@ -59,6 +60,40 @@ class MlpConfig(ctypes.Structure):
                 ("grad_mode", c_int), ("max_bn", c_int), ("cta_pair", c_int)]
 
 
+class LayerNormDesc(ctypes.Structure):
+    _fields_ = [("rows", c_longlong), ("cols", c_int), ("dtype", c_int), ("param_dtype", c_int), ("eps", c_float),
+                ("x", c_void_p), ("ldx", c_longlong), ("gamma", c_void_p), ("beta", c_void_p),
+                ("y", c_void_p), ("ldy", c_longlong), ("mean", c_void_p), ("rstd", c_void_p),
+                ("dy", c_void_p), ("lddy", c_longlong), ("dx", c_void_p), ("lddx", c_longlong),
+                ("dgamma", c_void_p), ("dbeta", c_void_p), ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class Fp8QuantizeDesc(ctypes.Structure):
+    _fields_ = [("rows", c_int), ("cols", c_int), ("dtype", c_int), ("q_dtype", c_int), ("block_rows", c_int),
+                ("x", c_void_p), ("ldx", c_longlong),
+                ("q", c_void_p), ("ldq", c_longlong), ("scale", c_void_p), ("ld_scale", c_longlong),
+                ("qt", c_void_p), ("ldqt", c_longlong), ("scale_t", c_void_p), ("ld_scale_t", c_longlong)]
+
+
+class Fp8GemmDesc(ctypes.Structure):
+    _fields_ = [("M", c_int), ("N", c_int), ("K", c_int), ("a_dtype", c_int), ("b_dtype", c_int),
+                ("a", c_void_p), ("lda", c_longlong), ("scale_a", c_void_p), ("ld_scale_a", c_longlong), ("a_block_rows", c_int),
+                ("b", c_void_p), ("ldb", c_longlong), ("scale_b", c_void_p), ("ld_scale_b", c_longlong), ("b_block_rows", c_int),
+                ("out", c_void_p), ("ldo", c_longlong), ("out_dtype", c_int)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("m", c_void_p), ("v", c_void_p),
+                ("m_scale", c_void_p), ("v_scale", c_void_p), ("copy_bf16", c_void_p), ("n", c_longlong),
+                ("weight_decay", c_float), ("pad", c_int)]
+
+
+class AdamWConfig(ctypes.Structure):
+    _fields_ = [("num_tensors", c_int), ("tensors", ctypes.POINTER(AdamWTensor)), ("param_dtype", c_int),
+                ("grad_dtype", c_int), ("state_dtype", c_int), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("step", c_longlong)]
+
+
 _P = c_void_p
 _SIGS = {
     "pkt_last_error": ([], ctypes.c_char_p),
@@ -90,6 +125,18 @@ _SIGS = {
     "pkt_axpy": ([_P, _P, c_float, c_longlong, _P], c_int),
     "pkt_axpy_noalloc": ([_P, _P, c_float, c_longlong, _P], c_int),
     "pkt_axpy_noalloc_status": ([_P, _P, _P], c_int),
+    "pkt_layernorm_forward": ([ctypes.POINTER(LayerNormDesc), _P], c_int),
+    "pkt_layernorm_backward_workspace": ([ctypes.POINTER(LayerNormDesc), ctypes.POINTER(ctypes.c_size_t)], c_int),
+    "pkt_layernorm_backward": ([ctypes.POINTER(LayerNormDesc), _P], c_int),
+    "pkt_fp8_quantize": ([ctypes.POINTER(Fp8QuantizeDesc), _P], c_int),
+    "pkt_fp8_gemm": ([ctypes.POINTER(Fp8GemmDesc), _P], c_int),
+    "pkt_fp8_gemm_status": ([ctypes.POINTER(c_int)], c_int),
+    "pkt_adamw_create": ([c_int, ctypes.POINTER(AdamWConfig), ctypes.POINTER(_P)], c_int),
+    "pkt_adamw_destroy": ([_P], c_int),
+    "pkt_adamw_step": ([_P, c_float, c_float, _P, _P], c_int),
+    "pkt_adamw_set_grads": ([_P, _P, _P], c_int),
+    "pkt_adamw_set_step": ([_P, c_longlong, _P], c_int),
+    "pkt_adamw_get_step": ([_P, ctypes.POINTER(c_longlong), _P], c_int),
     "pkt_mlp_create": ([c_int, _P, ctypes.POINTER(_P)], c_int),
     "pkt_mlp_destroy": ([_P], c_int),
     "pkt_mlp_set_params": ([_P, _P, _P], c_int),

@@ -1,0 +1,424 @@
+// pkt_adamw_*: one AdamW step over many tensors in one launch.
+//
+// Bound by memory: 28 bytes per parameter with fp32 states (parameter, m and v read
+// and written, gradient read), 16 1/8 with 8-bit states, 2 more for a bf16 copy.
+// The tensors are cut into chunks of 4096 values, listed once in device memory; a
+// block takes every gridDim-th chunk, and within it a warp owns blocks of 128 values,
+// 4 per lane, so that a block of 8-bit states is quantised with one warp reduction.
+// All loads of a warp's share are issued before the first is used.
+//
+// 8-bit states hold m and r = sqrt(v) as e4m3 with an fp32 scale per 128 values. The
+// root, because its range is half of v's in octaves (e4m3 spans 18 octaves below the
+// block's maximum, v would need 36) and because r is what the update divides by.
+// The arithmetic of a step is fp32 with each operation rounded on its own where the
+// result is quantised, so the stored 8-bit values do not depend on how a compiler
+// contracts the expressions.
+//
+// The step count and the bias corrections live on the device: every block reads the
+// corrections, and the last block to finish (an atomic ticket) advances them, in
+// 64 bits, so a captured step can be replayed.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "ops_common.h"
+#include "ops_device.cuh"
+
+namespace pkb {
+namespace {
+
+constexpr int kChunk = 4096;
+constexpr int kAdamThreads = 256;
+constexpr int kBlocksPerWarp = kChunk / kScaleBlock / (kAdamThreads / 32);
+
+struct AdamTensor {
+  void* param;
+  const void* grad;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  uint16_t* copy;
+  long long n;
+  float decay;
+  int wide;  // every array starts on a boundary of 4 of its values
+};
+
+struct AdamState {
+  double pow1, pow2;  // beta1^t, beta2^t of the steps taken
+  long long step;
+  float inv_bc1, inv_root_bc2;  // of the next step
+  unsigned ticket;
+};
+
+struct AdamArgs {
+  const AdamTensor* tensors;
+  const int2* chunks;  // tensor, chunk within it
+  int num_chunks;
+  AdamState* state;
+  const float* scales;
+  float lr, grad_scale, b1, c1, b2, c2, eps;
+  double beta1, beta2;
+};
+
+__device__ __forceinline__ void adam_advance(AdamState* s, double beta1, double beta2) {
+  s->step += 1;
+  s->pow1 *= beta1;
+  s->pow2 *= beta2;
+  s->inv_bc1 = float(1.0 / (1.0 - s->pow1 * beta1));
+  s->inv_root_bc2 = float(1.0 / sqrt(1.0 - s->pow2 * beta2));
+}
+
+__global__ void adam_set_state(AdamState* s, double pow1, double pow2, long long step, double beta1, double beta2) {
+  s->pow1 = pow1;
+  s->pow2 = pow2;
+  s->step = step;
+  s->inv_bc1 = float(1.0 / (1.0 - pow1 * beta1));
+  s->inv_root_bc2 = float(1.0 / sqrt(1.0 - pow2 * beta2));
+}
+
+// A lane's 4 values of one block: consecutive (one access) in whole blocks of
+// aligned tensors, 32 apart otherwise.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, bool wide, int lane, int left, float (&v)[4]) {
+  if (wide) {
+    Raw<T, 4> r;
+    r.load(p + 4 * lane, 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r.get(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lane + 32 * i < left ? to_f32(p[lane + 32 * i]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool wide, int lane, int left, const float (&v)[4]) {
+  if (wide) {
+    store_vec<T, 4>(p + 4 * lane, v, 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < left) from_f32(v[i], p + lane + 32 * i);
+  }
+}
+__device__ __forceinline__ uint32_t load_bytes4(const uint8_t* p, bool wide, int lane, int left) {
+  if (wide) return *reinterpret_cast<const uint32_t*>(p + 4 * lane);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < left) w |= uint32_t(p[lane + 32 * i]) << (8 * i);
+  return w;
+}
+__device__ __forceinline__ void store_bytes4(uint8_t* p, bool wide, int lane, int left, uint32_t w) {
+  if (wide) {
+    *reinterpret_cast<uint32_t*>(p + 4 * lane) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < left) p[lane + 32 * i] = uint8_t(w >> (8 * i));
+  }
+}
+__device__ __forceinline__ void unpack4(uint32_t w, float scale, float (&v)[4]) {
+  const float2 lo = unpack_e4m3x2(uint16_t(w)), hi = unpack_e4m3x2(uint16_t(w >> 16));
+  v[0] = lo.x * scale, v[1] = lo.y * scale, v[2] = hi.x * scale, v[3] = hi.y * scale;
+}
+
+template <typename P, typename G, bool EIGHT>
+__global__ void __launch_bounds__(kAdamThreads) adam_step(const AdamArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float lr = a.scales ? a.lr * a.scales[0] : a.lr;
+  const float gs = a.scales ? a.grad_scale * a.scales[1] : a.grad_scale;
+  const float step_size = lr * a.state->inv_bc1, inv_root = a.state->inv_root_bc2;
+  for (int c = blockIdx.x; c < a.num_chunks; c += gridDim.x) {
+    const int2 where = a.chunks[c];
+    const AdamTensor t = a.tensors[where.x];
+    if (t.grad == nullptr) continue;
+    const float keep = 1.f - lr * t.decay;
+    const long long base = (long long)where.y * kChunk + warp * kBlocksPerWarp * kScaleBlock;
+    float p[kBlocksPerWarp][4], g[kBlocksPerWarp][4], m[EIGHT ? 1 : kBlocksPerWarp][4], v[EIGHT ? 1 : kBlocksPerWarp][4];
+    uint32_t mq[EIGHT ? kBlocksPerWarp : 1], vq[EIGHT ? kBlocksPerWarp : 1];
+    float ms[EIGHT ? kBlocksPerWarp : 1], vs[EIGHT ? kBlocksPerWarp : 1];
+#pragma unroll
+    for (int b = 0; b < kBlocksPerWarp; ++b) {
+      const long long at = base + b * kScaleBlock;
+      const int left = int(min(t.n - at, (long long)kScaleBlock));
+      if (left <= 0) continue;
+      const bool wide = t.wide && left == kScaleBlock;
+      load4(static_cast<const P*>(t.param) + at, wide, lane, left, p[b]);
+      load4(static_cast<const G*>(t.grad) + at, wide, lane, left, g[b]);
+      if constexpr (EIGHT) {
+        mq[b] = load_bytes4(static_cast<const uint8_t*>(t.m) + at, wide, lane, left);
+        vq[b] = load_bytes4(static_cast<const uint8_t*>(t.v) + at, wide, lane, left);
+        ms[b] = t.m_scale[at / kScaleBlock];
+        vs[b] = t.v_scale[at / kScaleBlock];
+      } else {
+        load4(static_cast<const float*>(t.m) + at, wide, lane, left, m[b]);
+        load4(static_cast<const float*>(t.v) + at, wide, lane, left, v[b]);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBlocksPerWarp; ++b) {
+      const long long at = base + b * kScaleBlock;
+      const int left = int(min(t.n - at, (long long)kScaleBlock));
+      if (left <= 0) continue;
+      const bool wide = t.wide && left == kScaleBlock;
+      float mm[4], vv[4], root[4];
+      if constexpr (EIGHT) {
+        unpack4(mq[b], ms[b], mm);
+        unpack4(vq[b], vs[b], vv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vv[i] = __fmul_rn(vv[i], vv[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mm[i] = m[b][i], vv[i] = v[b][i];
+      }
+      uint32_t mbig = 0, vbig = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float gr = g[b][i] * gs;
+        mm[i] = __fadd_rn(__fmul_rn(mm[i], a.b1), __fmul_rn(gr, a.c1));
+        vv[i] = __fadd_rn(__fmul_rn(vv[i], a.b2), __fmul_rn(__fmul_rn(gr, gr), a.c2));
+        root[i] = __fsqrt_rn(vv[i]);
+        p[b][i] = p[b][i] * keep - step_size * mm[i] / fmaf(root[i], inv_root, a.eps);
+        mbig = max(mbig, abs_bits(mm[i]));
+        vbig = max(vbig, abs_bits(root[i]));
+      }
+      store4(static_cast<P*>(t.param) + at, wide, lane, left, p[b]);
+      if (t.copy) store4(reinterpret_cast<bf16_t*>(t.copy) + at, wide, lane, left, p[b]);
+      if constexpr (EIGHT) {
+        mbig = __reduce_max_sync(0xffffffffu, mbig);
+        vbig = __reduce_max_sync(0xffffffffu, vbig);
+        float mf, mscale, vf, vscale;
+        block_scale(mbig, 448.f, &mf, &mscale);
+        block_scale(vbig, 448.f, &vf, &vscale);
+        store_bytes4(static_cast<uint8_t*>(t.m) + at, wide, lane, left,
+                     pack_fp8x4<false>(__fmul_rn(mm[0], mf), __fmul_rn(mm[1], mf), __fmul_rn(mm[2], mf), __fmul_rn(mm[3], mf)));
+        uint32_t q = pack_fp8x4<false>(__fmul_rn(root[0], vf), __fmul_rn(root[1], vf), __fmul_rn(root[2], vf), __fmul_rn(root[3], vf));
+        // a root above zero stays above zero: the smallest 8-bit value is code 1
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (root[i] > 0.f && vf > 0.f && ((q >> (8 * i)) & 0xffu) == 0) q |= 1u << (8 * i);
+        store_bytes4(static_cast<uint8_t*>(t.v) + at, wide, lane, left, q);
+        if (lane == 0) t.m_scale[at / kScaleBlock] = mscale, t.v_scale[at / kScaleBlock] = vscale;
+      } else {
+        store4(static_cast<float*>(t.m) + at, wide, lane, left, mm);
+        store4(static_cast<float*>(t.v) + at, wide, lane, left, vv);
+      }
+    }
+  }
+  __syncthreads();  // every thread of the block has read the state
+  if (threadIdx.x == 0 && atomicAdd(&a.state->ticket, 1u) == gridDim.x - 1) {
+    a.state->ticket = 0;
+    adam_advance(a.state, a.beta1, a.beta2);
+  }
+}
+
+struct AdamW {
+  int device = 0, sms = 0;
+  std::vector<AdamTensor> tensors;
+  int num_chunks = 0;
+  int param_dtype = 0, grad_dtype = 0, state_dtype = 0;
+  double beta1 = 0, beta2 = 0, eps = 0;
+  AdamTensor* d_tensors = nullptr;
+  int2* d_chunks = nullptr;
+  AdamState* d_state = nullptr;
+
+  ~AdamW() {
+    int before = 0;
+    const bool back = cudaGetDevice(&before) == cudaSuccess && before != device;
+    cudaSetDevice(device);
+    cudaFree(d_tensors);
+    cudaFree(d_chunks);
+    cudaFree(d_state);
+    if (back) cudaSetDevice(before);
+  }
+  void set_wide(AdamTensor* t) const {
+    const size_t p = param_dtype == PKT_DTYPE_F32 ? 16 : 8, g = grad_dtype == PKT_DTYPE_F32 ? 16 : 8,
+                 s = state_dtype == PKT_DTYPE_F32 ? 16 : 4;
+    t->wide = aligned_to(t->param, p) && aligned_to(t->grad, g) && aligned_to(t->m, s) && aligned_to(t->v, s) && aligned_to(t->copy, 8);
+  }
+  int check_grad(const void* g, size_t i) const {
+    if (!aligned_to(g, grad_dtype == PKT_DTYPE_F32 ? 4 : 2)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
+    return op_check_memory(g, "grad", device);
+  }
+  int set_step(long long step, cudaStream_t st) {
+    const cudaError_t e = op_launch(adam_set_state, dim3(1), dim3(1), 0, st, false, d_state, std::pow(beta1, double(step)),
+                                    std::pow(beta2, double(step)), step, beta1, beta2);
+    return e == cudaSuccess ? PKT_OK : cuda_fail(e, "set the AdamW step");
+  }
+  int setup(const pkt_adamw_config& c);
+  int run(float lr, float grad_scale, const float* scales, cudaStream_t st);
+};
+
+int AdamW::setup(const pkt_adamw_config& c) {
+  if (c.num_tensors < 0 || (c.num_tensors > 0 && !c.tensors)) return fail(PKT_ERR_ARGS, "bad AdamW tensor list");
+  if (c.param_dtype != PKT_DTYPE_F32 && c.param_dtype != PKT_DTYPE_BF16) return fail(PKT_ERR_ARGS, "AdamW param_dtype must be f32 or bf16");
+  if (c.grad_dtype != PKT_DTYPE_F32 && c.grad_dtype != PKT_DTYPE_BF16) return fail(PKT_ERR_ARGS, "AdamW grad_dtype must be f32 or bf16");
+  if (c.state_dtype != PKT_DTYPE_F32 && c.state_dtype != PKT_DTYPE_E4M3) return fail(PKT_ERR_ARGS, "AdamW state_dtype must be f32 or e4m3");
+  if (!(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1)) return fail(PKT_ERR_ARGS, "AdamW betas must be in [0, 1)");
+  if (!(c.eps >= 0) || !std::isfinite(c.eps)) return fail(PKT_ERR_ARGS, "AdamW eps must be >= 0");
+  if (c.step < 0) return fail(PKT_ERR_ARGS, "AdamW step must be >= 0");
+  param_dtype = c.param_dtype, grad_dtype = c.grad_dtype, state_dtype = c.state_dtype;
+  beta1 = c.beta1, beta2 = c.beta2, eps = c.eps;
+  const bool eight = state_dtype == PKT_DTYPE_E4M3;
+  const size_t ps = param_dtype == PKT_DTYPE_F32 ? 4 : 2, ss = eight ? 1 : 4;
+  std::vector<int2> chunks;
+  int rc;
+  for (int i = 0; i < c.num_tensors; ++i) {
+    const pkt_adamw_tensor& s = c.tensors[i];
+    if (s.n < 0) return fail(PKT_ERR_ARGS, "tensor %d has %lld values", i, s.n);
+    if (s.n > 0 && (!s.param || !s.m || !s.v)) return fail(PKT_ERR_ARGS, "tensor %d needs param, m and v", i);
+    if (s.n > 0 && eight && (!s.m_scale || !s.v_scale)) return fail(PKT_ERR_ARGS, "tensor %d needs m_scale and v_scale (8-bit states)", i);
+    if (!aligned_to(s.param, ps) || !aligned_to(s.m, ss) || !aligned_to(s.v, ss) || !aligned_to(s.m_scale, 4) || !aligned_to(s.v_scale, 4) ||
+        !aligned_to(s.copy_bf16, 2))
+      return fail(PKT_ERR_ARGS, "an array of tensor %d is not aligned to its type", i);
+    if ((rc = op_check_memory(s.param, "param", device)) || (rc = op_check_memory(s.m, "m", device)) || (rc = op_check_memory(s.v, "v", device)) ||
+        (rc = op_check_memory(s.copy_bf16, "copy_bf16", device)) || (rc = check_grad(s.grad, size_t(i))))
+      return rc;
+    if (eight && ((rc = op_check_memory(s.m_scale, "m_scale", device)) || (rc = op_check_memory(s.v_scale, "v_scale", device)))) return rc;
+    AdamTensor t{s.param, s.grad, s.m, s.v, s.m_scale, s.v_scale, static_cast<uint16_t*>(s.copy_bf16), s.n, s.weight_decay, 0};
+    set_wide(&t);
+    tensors.push_back(t);
+    const long long count = (s.n + kChunk - 1) / kChunk;
+    if (count + (long long)chunks.size() > 0x7fffffffLL) return fail(PKT_ERR_ARGS, "too many parameters for one AdamW plan");
+    for (long long k = 0; k < count; ++k) chunks.push_back(make_int2(i, int(k)));
+  }
+  num_chunks = int(chunks.size());
+  cudaError_t e = cudaMalloc(&d_tensors, sizeof(AdamTensor) * std::max<size_t>(1, tensors.size()));
+  if (e == cudaSuccess) e = cudaMalloc(&d_chunks, sizeof(int2) * std::max<size_t>(1, chunks.size()));
+  if (e == cudaSuccess) e = cudaMalloc(&d_state, sizeof(AdamState));
+  if (e == cudaSuccess) e = cudaMemset(d_state, 0, sizeof(AdamState));
+  if (e == cudaSuccess && !tensors.empty())
+    e = cudaMemcpy(d_tensors, tensors.data(), sizeof(AdamTensor) * tensors.size(), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess && num_chunks) e = cudaMemcpy(d_chunks, chunks.data(), sizeof(int2) * chunks.size(), cudaMemcpyHostToDevice);
+  if (e != cudaSuccess) return cuda_fail(e, "AdamW tables");
+  if ((rc = set_step(c.step, nullptr))) return rc;
+  e = cudaDeviceSynchronize();  // the state is set before a step on any stream
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "AdamW set-up");
+}
+
+template <typename P, typename G>
+cudaError_t adam_launch(const AdamArgs& a, bool eight, int blocks, cudaStream_t st) {
+  return eight ? op_launch(adam_step<P, G, true>, dim3(blocks), dim3(kAdamThreads), 0, st, false, a)
+               : op_launch(adam_step<P, G, false>, dim3(blocks), dim3(kAdamThreads), 0, st, false, a);
+}
+
+int AdamW::run(float lr, float grad_scale, const float* scales, cudaStream_t st) {
+  if (!aligned_to(scales, 4)) return fail(PKT_ERR_ARGS, "scales is not aligned to its type");
+  int rc = op_check_memory(scales, "scales", device);
+  if (rc) return rc;
+  AdamArgs a{};
+  a.tensors = d_tensors, a.chunks = d_chunks, a.num_chunks = num_chunks, a.state = d_state, a.scales = scales;
+  a.lr = lr, a.grad_scale = grad_scale;
+  a.b1 = float(beta1), a.c1 = float(1.0 - beta1), a.b2 = float(beta2), a.c2 = float(1.0 - beta2), a.eps = float(eps);
+  a.beta1 = beta1, a.beta2 = beta2;
+  // one block per chunk up to what the SMs hold; a plan without values still counts the step
+  const int blocks = std::max(1, std::min(num_chunks, sms * 8));
+  const bool eight = state_dtype == PKT_DTYPE_E4M3, pf = param_dtype == PKT_DTYPE_F32, gf = grad_dtype == PKT_DTYPE_F32;
+  const cudaError_t e = pf ? (gf ? adam_launch<float, float>(a, eight, blocks, st) : adam_launch<float, bf16_t>(a, eight, blocks, st))
+                           : (gf ? adam_launch<bf16_t, float>(a, eight, blocks, st) : adam_launch<bf16_t, bf16_t>(a, eight, blocks, st));
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch AdamW");
+}
+
+// The plan's device is current inside a call, the caller's afterwards.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(int device) {
+    int cur = 0;
+    if (cudaGetDevice(&cur) == cudaSuccess && cur != device) {
+      before = cur;
+      cudaSetDevice(device);
+    }
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+}  // namespace
+}  // namespace pkb
+
+struct pkt_adamw {
+  pkb::AdamW plan;
+};
+
+extern "C" {
+
+int pkt_adamw_create(int device, const pkt_adamw_config* cfg, pkt_adamw** out) {
+  using namespace pkb;
+  if (!cfg || !out) return fail(PKT_ERR_ARGS, "null argument");
+  int count = 0;
+  const cudaError_t e = cudaGetDeviceCount(&count);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDeviceCount");
+  if (device < 0 || device >= count) return fail(PKT_ERR_ARGS, "device %d out of range (%d devices)", device, count);
+  OnDevice on(device);
+  int dev = 0, sms = 0, rc;
+  if ((rc = op_device(&dev, &sms))) return rc;
+  pkt_adamw* h = nullptr;
+  try {
+    h = new pkt_adamw();
+    h->plan.device = dev, h->plan.sms = sms;
+    rc = h->plan.setup(*cfg);
+  } catch (const std::bad_alloc&) {
+    rc = fail(PKT_ERR_ARGS, "out of host memory");
+  }
+  if (rc) {
+    delete h;
+    return rc;
+  }
+  *out = h;
+  return PKT_OK;
+}
+
+int pkt_adamw_destroy(pkt_adamw* h) {
+  delete h;
+  return PKT_OK;
+}
+
+int pkt_adamw_step(pkt_adamw* h, float lr, float grad_scale, const float* scales, void* stream) {
+  if (!h) return pkb::fail(PKT_ERR_ARGS, "null AdamW plan");
+  pkb::OnDevice on(h->plan.device);
+  return h->plan.run(lr, grad_scale, scales, static_cast<cudaStream_t>(stream));
+}
+
+int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream) {
+  using namespace pkb;
+  if (!h || (!grads && !h->plan.tensors.empty())) return fail(PKT_ERR_ARGS, "null argument");
+  AdamW& p = h->plan;
+  OnDevice on(p.device);
+  int rc;
+  for (size_t i = 0; i < p.tensors.size(); ++i)
+    if ((rc = p.check_grad(grads[i], i))) return rc;
+  for (size_t i = 0; i < p.tensors.size(); ++i) {
+    p.tensors[i].grad = grads[i];
+    p.set_wide(&p.tensors[i]);
+  }
+  if (p.tensors.empty()) return PKT_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus capturing;
+  cudaError_t e = cudaStreamIsCapturing(st, &capturing);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  if (capturing != cudaStreamCaptureStatusNone) return fail(PKT_ERR_ARGS, "AdamW gradients cannot be set inside a stream capture");
+  e = cudaMemcpyAsync(p.d_tensors, p.tensors.data(), sizeof(AdamTensor) * p.tensors.size(), cudaMemcpyHostToDevice, st);
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "copy AdamW gradients");
+}
+
+int pkt_adamw_set_step(pkt_adamw* h, long long step, void* stream) {
+  if (!h || step < 0) return pkb::fail(PKT_ERR_ARGS, "bad AdamW step");
+  pkb::OnDevice on(h->plan.device);
+  return h->plan.set_step(step, static_cast<cudaStream_t>(stream));
+}
+
+int pkt_adamw_get_step(pkt_adamw* h, long long* step, void* stream) {
+  using namespace pkb;
+  if (!h || !step) return fail(PKT_ERR_ARGS, "null argument");
+  OnDevice on(h->plan.device);
+  AdamState s;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(&s, h->plan.d_state, sizeof(s), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return cuda_fail(e, "read the AdamW step");
+  *step = s.step;
+  return PKT_OK;
+}
+
+}  // extern "C"

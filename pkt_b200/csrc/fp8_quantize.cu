@@ -1,0 +1,256 @@
+// pkt_fp8_quantize: block-scaled 8-bit operands, plain and transposed, from one read.
+//
+// Bound by memory: a value is read once (2 or 4 bytes) and written once or twice as
+// one byte, with one fp32 scale per 128 or 128 x 128 values.
+//
+// A warp holds 128 columns of a row, 4 consecutive ones per lane. Rows alone
+// (block_rows 1, no transposed result) need nothing beyond a warp: the largest
+// magnitude is one warp reduction, and every warp takes several rows so that their
+// loads overlap. Otherwise a block of 8 warps takes a 128 x 128 tile into registers
+// (a lane has 4 columns x 16 rows, so a column's 16 values of a warp are 16
+// consecutive bytes of the transposed result); column maxima meet in shared memory,
+// and the transposed bytes pass through it to leave as whole 128-byte rows.
+#include <algorithm>
+
+#include "ops_common.h"
+#include "ops_device.cuh"
+
+namespace pkb {
+namespace {
+
+struct QuantArgs {
+  int rows, cols, block_rows;
+  const void* x;
+  long long ldx;
+  uint8_t* q;
+  long long ldq;
+  float* scale;
+  long long ld_scale;
+  uint8_t* qt;
+  long long ldqt;
+  float* scale_t;
+  long long ld_scale_t;
+  float most;
+};
+
+constexpr int kRowsPerWarp = 4;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_cols4(const T* row, int col, int cols, float (&v)[4]) {
+  Raw<T, WIDE ? 4 : 1> r[WIDE ? 1 : 4];
+  if (WIDE) {
+    r[0].load(row + col, cols - col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[0].get(WIDE ? i : 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = col + i < cols ? to_f32(row[col + i]) : 0.f;
+  }
+}
+
+// 4 bytes of a row that starts on a 16-byte boundary, only those inside the matrix
+__device__ __forceinline__ void store_cols4(uint8_t* row, int col, int cols, uint32_t q) {
+  if (col + 4 <= cols) {
+    *reinterpret_cast<uint32_t*>(row + col) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < cols) row[col + i] = uint8_t(q >> (8 * i));
+  }
+}
+
+template <bool E5M2>
+__device__ __forceinline__ uint32_t quantize4(const float (&v)[4], float f) {
+  return pack_fp8x4<E5M2>(__fmul_rn(v[0], f), __fmul_rn(v[1], f), __fmul_rn(v[2], f), __fmul_rn(v[3], f));
+}
+
+template <typename T, bool WIDE, bool E5M2>
+__global__ void __launch_bounds__(128) quantize_rows(const QuantArgs a) {
+  const int lane = threadIdx.x & 31, kb = blockIdx.x, col = kb * kScaleBlock + 4 * lane;
+  const long long groups = ((long long)a.rows + kRowsPerWarp - 1) / kRowsPerWarp;
+  for (long long g = (long long)blockIdx.y * 4 + (threadIdx.x >> 5); g < groups; g += (long long)gridDim.y * 4) {
+    const long long row0 = g * kRowsPerWarp;
+    float v[kRowsPerWarp][4];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[r][i] = 0.f;
+      if (row0 + r < a.rows) load_cols4<T, WIDE>(static_cast<const T*>(a.x) + (row0 + r) * a.ldx, col, a.cols, v[r]);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+      uint32_t big = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) big = max(big, abs_bits(v[r][i]));
+      float f, s;
+      block_scale(__reduce_max_sync(0xffffffffu, big), a.most, &f, &s);
+      if (lane == r) mine = s;
+      if (row0 + r < a.rows) store_cols4(a.q + (row0 + r) * a.ldq, col, a.cols, quantize4<E5M2>(v[r], f));
+    }
+    if (lane < kRowsPerWarp && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = mine;
+  }
+}
+
+template <typename T, bool WIDE, bool E5M2>
+__global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
+  __shared__ uint32_t col_big[8][128];
+  __shared__ float col_factor[128];
+  __shared__ uint32_t tile_big[8];
+  __shared__ __align__(16) uint8_t bytes[128 * 128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kb = blockIdx.x, col = kb * 128 + 4 * lane;
+  const bool square = a.block_rows == 128;
+  const int row_tiles = (a.rows + 127) / 128;
+  for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
+    const int row0 = rt * 128 + warp * 16;
+    float v[16][4];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[r][i] = 0.f;
+      if (row0 + r < a.rows) load_cols4<T, WIDE>(static_cast<const T*>(a.x) + (long long)(row0 + r) * a.ldx, col, a.cols, v[r]);
+    }
+    uint32_t cbig[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cbig[i] = max(cbig[i], abs_bits(v[r][i]));
+    float f = 0.f, s = 0.f;
+    if (square) {
+      const uint32_t big = __reduce_max_sync(0xffffffffu, max(max(cbig[0], cbig[1]), max(cbig[2], cbig[3])));
+      if (lane == 0) tile_big[warp] = big;
+      __syncthreads();
+      uint32_t all = tile_big[0];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) all = max(all, tile_big[w]);
+      block_scale(all, a.most, &f, &s);
+      if (threadIdx.x == 0) {
+        if (a.q) a.scale[kb * a.ld_scale + rt] = s;
+        if (a.qt) a.scale_t[rt * a.ld_scale_t + kb] = s;
+      }
+    } else if (a.qt) {
+      *reinterpret_cast<uint4*>(&col_big[warp][4 * lane]) = make_uint4(cbig[0], cbig[1], cbig[2], cbig[3]);
+      __syncthreads();
+      if (threadIdx.x < 128) {
+        uint32_t all = col_big[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) all = max(all, col_big[w][threadIdx.x]);
+        float cf, cs;
+        block_scale(all, a.most, &cf, &cs);
+        col_factor[threadIdx.x] = cf;
+        if (kb * 128 + threadIdx.x < a.cols) a.scale_t[rt * a.ld_scale_t + kb * 128 + threadIdx.x] = cs;
+      }
+    }
+    if (a.q) {
+      float mine = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float rf = f;
+        if (!square) {
+          uint32_t big = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big = max(big, abs_bits(v[r][i]));
+          block_scale(__reduce_max_sync(0xffffffffu, big), a.most, &rf, &s);
+          if (lane == r) mine = s;
+        }
+        if (row0 + r < a.rows) store_cols4(a.q + (long long)(row0 + r) * a.ldq, col, a.cols, quantize4<E5M2>(v[r], rf));
+      }
+      if (!square && lane < 16 && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = mine;
+    }
+    if (a.qt) {
+      __syncthreads();  // col_factor is written; the tile before has left `bytes`
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 4 * lane + i;
+        const float cf = square ? f : col_factor[c];
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float u[4] = {v[4 * k][i], v[4 * k + 1][i], v[4 * k + 2][i], v[4 * k + 3][i]};
+          w[k] = quantize4<E5M2>(u, cf);
+        }
+        // 16-byte pieces of a row are permuted by its column group: 8 lanes, 8 banks
+        *reinterpret_cast<uint4*>(bytes + c * 128 + ((warp ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncthreads();
+      const int piece = threadIdx.x & 7, left = a.rows - rt * 128 - piece * 16;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = k * 32 + (threadIdx.x >> 3), out = kb * 128 + c;
+        if (out >= a.cols || left <= 0) continue;
+        const uint4 w = *reinterpret_cast<const uint4*>(bytes + c * 128 + ((piece ^ ((c >> 2) & 7)) * 16));
+        uint8_t* to = a.qt + out * a.ldqt + (long long)rt * 128 + piece * 16;
+        if (left >= 16) {
+          *reinterpret_cast<uint4*>(to) = w;
+        } else {
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < left) to[i] = uint8_t(ws[i >> 2] >> (8 * (i & 3)));
+        }
+      }
+    }
+    __syncthreads();  // the maxima and bytes are free for the next tile
+  }
+}
+
+template <typename T, bool WIDE, bool E5M2>
+cudaError_t quantize_run(const QuantArgs& a, cudaStream_t st) {
+  const unsigned kbs = unsigned((a.cols - 1) / kScaleBlock + 1);
+  if (a.block_rows == 1 && !a.qt) {
+    const long long blocks = ((long long)a.rows + 4 * kRowsPerWarp - 1) / (4 * kRowsPerWarp);
+    return op_launch(quantize_rows<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(blocks, 65535LL))), dim3(128), 0, st, false, a);
+  }
+  const int tiles = (a.rows - 1) / 128 + 1;
+  return op_launch(quantize_tile<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(tiles, 65535))), dim3(256), 0, st, false, a);
+}
+
+template <typename T>
+cudaError_t quantize_dispatch(const QuantArgs& a, bool wide, bool e5m2, cudaStream_t st) {
+  if (wide) return e5m2 ? quantize_run<T, true, true>(a, st) : quantize_run<T, true, false>(a, st);
+  return e5m2 ? quantize_run<T, false, true>(a, st) : quantize_run<T, false, false>(a, st);
+}
+
+int check_result(const char* name, const void* q, long long ld, const float* scale, long long ld_scale, int cols, long long scales) {
+  if (!aligned_to(q, 16) || ld % 16 != 0) return fail(PKT_ERR_ARGS, "%s must be 16-byte aligned with a row stride that is a multiple of 16", name);
+  if (ld < cols) return fail(PKT_ERR_ARGS, "row stride %lld of %s is below its %d columns", ld, name, cols);
+  if (!scale || !aligned_to(scale, 4)) return fail(PKT_ERR_ARGS, "%s needs its scales, aligned to 4 bytes", name);
+  if (ld_scale < scales) return fail(PKT_ERR_ARGS, "row stride %lld of %s's scales is below their %lld columns", ld_scale, name, scales);
+  return PKT_OK;
+}
+
+}  // namespace
+}  // namespace pkb
+
+extern "C" int pkt_fp8_quantize(const pkt_fp8_quantize_desc* d, void* stream) {
+  using namespace pkb;
+  if (!d) return fail(PKT_ERR_ARGS, "null quantize descriptor");
+  if (d->rows < 0 || d->cols < 0) return fail(PKT_ERR_ARGS, "quantize of %d x %d values", d->rows, d->cols);
+  if (d->dtype != PKT_DTYPE_BF16 && d->dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "quantize dtype must be bf16 or f32");
+  if (d->q_dtype != PKT_DTYPE_E4M3 && d->q_dtype != PKT_DTYPE_E5M2) return fail(PKT_ERR_ARGS, "quantize q_dtype must be e4m3 or e5m2");
+  if (d->block_rows != 1 && d->block_rows != 128) return fail(PKT_ERR_ARGS, "block_rows must be 1 or 128");
+  if (!d->q && !d->qt) return fail(PKT_ERR_ARGS, "quantize needs q or qt");
+  if (d->rows == 0 || d->cols == 0) return PKT_OK;
+  int dev = 0, sms = 0, rc;
+  const int es = d->dtype == PKT_DTYPE_BF16 ? 2 : 4;
+  if (!d->x || !aligned_to(d->x, es)) return fail(PKT_ERR_ARGS, "quantize needs x, aligned to its type");
+  if (d->ldx < d->cols) return fail(PKT_ERR_ARGS, "row stride %lld of x is below the %d columns", d->ldx, d->cols);
+  if (d->q && (rc = check_result("q", d->q, d->ldq, d->scale, d->ld_scale, d->cols, (d->rows - 1) / d->block_rows + 1))) return rc;
+  if (d->qt && (rc = check_result("qt", d->qt, d->ldqt, d->scale_t, d->ld_scale_t, d->rows, (d->cols - 1) / d->block_rows + 1))) return rc;
+  if ((rc = op_device(&dev, &sms)) || (rc = op_check_memory(d->x, "x", dev)) || (rc = op_check_memory(d->q, "q", dev)) ||
+      (d->q && (rc = op_check_memory(d->scale, "scale", dev))) || (rc = op_check_memory(d->qt, "qt", dev)) ||
+      (d->qt && (rc = op_check_memory(d->scale_t, "scale_t", dev))))
+    return rc;
+  QuantArgs a{};
+  a.rows = d->rows, a.cols = d->cols, a.block_rows = d->block_rows, a.x = d->x, a.ldx = d->ldx;
+  a.q = static_cast<uint8_t*>(d->q), a.ldq = d->ldq, a.scale = d->scale, a.ld_scale = d->ld_scale;
+  a.qt = static_cast<uint8_t*>(d->qt), a.ldqt = d->ldqt, a.scale_t = d->scale_t, a.ld_scale_t = d->ld_scale_t;
+  const bool e5m2 = d->q_dtype == PKT_DTYPE_E5M2;
+  a.most = e5m2 ? 57344.f : 448.f;
+  // 4 values in one access: every row of x starts on a boundary of 4 values
+  const bool wide = aligned_to(d->x, 4 * es) && d->ldx % 4 == 0;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = d->dtype == PKT_DTYPE_BF16 ? quantize_dispatch<bf16_t>(a, wide, e5m2, st) : quantize_dispatch<float>(a, wide, e5m2, st);
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch quantize");
+}

@@ -1,0 +1,50 @@
+// What the stand-alone operators (layer norm, AdamW, 8-bit quantising and product)
+// share on the host side: the device they run on, argument checks, launches.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "runtime_impl.h"
+
+namespace pkb {
+
+constexpr int kScaleBlock = 128;  // values of one 8-bit block along the contiguous dimension
+// A block whose largest magnitude is below 2^-100 is held as zeros with scale 0:
+// from there on, largest value / magnitude stays far from fp32 overflow.
+constexpr float kScaleTiny = 7.888609052210118e-31f;
+
+// The current device, checked once to be one this build runs on, and its SM count.
+int op_device(int* dev, int* sms);
+// `p` is memory of device `dev` (or managed memory), so that a host pointer or
+// another GPU's buffer is an error here and not a fault in the kernel. Null passes.
+int op_check_memory(const void* p, const char* what, int dev);
+// cuTensorMapEncodeTiled, looked up once; null when the driver has none.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled op_encode_tiled();
+
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// One launch; `dependent`: programmatic dependent launch (the kernel starts its
+// preamble early and waits for the grid before it itself, griddepcontrol.wait).
+template <typename... KArgs, typename... Args>
+cudaError_t op_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool dependent,
+                      Args... args) {
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  if (dependent) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+}  // namespace pkb

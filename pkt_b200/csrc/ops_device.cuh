@@ -1,0 +1,130 @@
+// Device helpers of the stand-alone operators: typed vector loads and stores,
+// warp reductions, block-scaled 8-bit floats.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "../../include/pk/detail/ptx.cuh"
+
+namespace pkb {
+
+struct bf16_t {
+  uint16_t bits;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float(uint32_t(v.bits) << 16); }
+__device__ __forceinline__ void from_f32(float v, float* out) { *out = v; }
+// results are rounded to the tensor's type once, at the store
+__device__ __forceinline__ void from_f32(float v, bf16_t* out) { out->bits = f32_to_bf16_rn(v); }
+
+// VEC consecutive elements as raw words: one load of up to 16 bytes each.
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int kBytes = VEC * int(sizeof(T));
+  static constexpr int kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+
+  // Elements [0, valid) of p; the rest are zero. A whole vector is one aligned
+  // access when VEC > 1 (the callers' rule), a partial one element by element.
+  __device__ __forceinline__ void load(const T* p, int valid) {
+    if (VEC > 1 && valid >= VEC) {
+      if (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+          const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+      } else if (kBytes == 8) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[kWords - 1] = v.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < valid) set(i, p[i]);
+    }
+  }
+  __device__ __forceinline__ void set(int i, float v) { w[i * int(sizeof(T)) / 4] = __float_as_uint(v); }
+  __device__ __forceinline__ void set(int i, bf16_t v) { w[i >> 1] |= uint32_t(v.bits) << (16 * (i & 1)); }
+  __device__ __forceinline__ float get(int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[i]);
+    return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
+  }
+};
+
+// Stores v[0..valid) to p, as one aligned access per 16 bytes where whole.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC], int valid) {
+  constexpr int kBytes = VEC * int(sizeof(T));
+  if (VEC > 1 && valid >= VEC) {
+    uint32_t w[(kBytes + 3) / 4];
+#pragma unroll
+    for (int i = 0; i < (kBytes + 3) / 4; ++i)
+      w[i] = sizeof(T) == 4 ? __float_as_uint(v[i < VEC ? i : 0]) : pack_bf16x2(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
+    if (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[kBytes / 4 - 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < valid) from_f32(v[i], p + i);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---------------------------------------------------------------- block-scaled 8-bit floats
+// Magnitudes are compared as unsigned bits of |x|: the order of finite values,
+// infinities above them and NaN above those, so a block that holds one says so
+// in its scale.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Factor and scale of a block from its largest magnitude: q = rn(x * factor), x ~ q * scale.
+__device__ __forceinline__ void block_scale(uint32_t amax_bits, float most, float* factor, float* scale) {
+  const float big = __uint_as_float(amax_bits);
+  const bool none = big < 7.888609052210118e-31f;  // kScaleTiny
+  *factor = none ? 0.f : __fdiv_rn(most, big);
+  *scale = none ? 0.f : __fdiv_rn(big, most);
+}
+
+// Two values to e4m3 / e5m2 (round to nearest even, out of range to the largest
+// finite value, NaN stays NaN); the first in the low byte.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t pack_fp8x2(float lo, float hi) {
+  uint16_t r;
+  if (E5M2)
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool E5M2>
+__device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
+  return pack_fp8x2<E5M2>(a, b) | (pack_fp8x2<E5M2>(c, d) << 16);
+}
+// Two e4m3 values to fp32 (exact).
+__device__ __forceinline__ float2 unpack_e4m3x2(uint16_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(v));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+}  // namespace pkb
