@@ -9,8 +9,10 @@
 // the MMAs of the next blocks run. One fp32 FMA per output value and block of 128.
 //
 // Roles of a CTA: warps 0..3 (0..7) epilogue, one per 32 TMEM lanes (and half of the
-// columns); then one TMA producer warp and one MMA issuer warp. Operand tiles are
-// 128-byte rows (128 values of K) in 128B-swizzled shared memory, in a ring of stages.
+// columns); then one TMA producer warp, one MMA issuer warp and one that copies the
+// scales of the coming blocks into shared memory (a load from L2 takes longer than a
+// block). Operand tiles are 128-byte rows (128 values of K) in 128B-swizzled shared
+// memory, in a ring of stages.
 //
 // "Rows" below are the operand whose 128 rows lie along the TMEM lanes, "cols" the one
 // along the columns of a tile. For few output rows (M) the operands change places, so
@@ -31,12 +33,11 @@ namespace {
 
 constexpr int kRows = 128;    // TMEM lanes
 constexpr int kKBytes = 128;  // one block of K: a 128-byte row of an operand tile
-constexpr unsigned long long kWaitNs = 2000000000ull;
 
 __device__ int g_fp8_status;
 
 struct alignas(64) Fp8Args {
-  CUtensorMap map_r, map_c;
+  CUtensorMap map_r, map_c, map_out;
   int rows, cols, num_kb;
   int tiles_r, tiles_c;
   const float *scale_r, *scale_c;
@@ -44,7 +45,8 @@ struct alignas(64) Fp8Args {
   int r_shift, c_shift;  // log2 of the rows that share a scale (0 or 7)
   void* out;
   long long ldo;
-  int out_bf16, swap, wide;  // swap: out[col * ldo + row]; wide: 16-byte stores along out's rows
+  int out_bf16, swap;  // swap: out[col * ldo + row]
+  int wide, tma_out;   // 4 values of out in one store; map_out is valid
   uint32_t idesc;
 };
 
@@ -53,51 +55,98 @@ struct Shape {
   static constexpr int kHalves = BN > 128 ? 2 : 1;   // epilogue warps per 32 lanes
   static constexpr int kCols = BN / kHalves;         // columns of an epilogue warp
   static constexpr int kEpiWarps = 4 * kHalves;
-  static constexpr int kThreads = 32 * (kEpiWarps + (kHalves == 2 ? 4 : 2));
+  static constexpr int kThreads = 32 * (kEpiWarps + 4);
   static constexpr int kRowBytes = kRows * kKBytes;
   static constexpr int kColBytes = BN / PAIR * kKBytes;
   static constexpr int kStageBytes = kRowBytes + kColBytes;
-  static constexpr int kStages = kStageBytes >= 32768 ? 6 : 8;
-  static constexpr int kBufs = BN > 128 ? 2 : 4;     // TMEM accumulators
+  static constexpr int kStages = kStageBytes >= 32768 ? 5 : 8;
+  static constexpr int kBufs = BN > 128 ? 2 : 4;     // TMEM accumulators of each half
   static constexpr int kTmemCols = kBufs * BN < 32 ? 32 : kBufs * BN;
-  static constexpr int kChunk = kCols < 32 ? kCols : 32;  // columns per TMEM load
+  static constexpr int kChunk = kCols < 32 ? kCols : 32;  // columns per TMEM load, two in flight
+  static constexpr bool kStore = BN >= 128;          // the result leaves by TMA stores
+  static constexpr int kGroup = 4;                   // blocks of K whose scales are handed over together
+  static constexpr int kScales = 2;                  // such groups held
 };
 
 template <int BN, int PAIR>
 struct Smem {
   using S = Shape<BN, PAIR>;
   uint8_t stages[S::kStages][S::kStageBytes];
-  float col_scale[S::kEpiWarps][S::kCols];
+  uint8_t staging[S::kStore ? S::kEpiWarps : 1][S::kStore ? 4096 : 16];  // 32 rows x 128 bytes of the result
+  float row_scale[S::kScales][S::kGroup][kRows];
+  float col_scale[S::kScales][S::kGroup][BN];  // of every column, or one for each half's columns
+  uint64_t sfull[S::kScales], sempty[S::kScales];
   uint64_t full[S::kStages], empty[S::kStages];
-  uint64_t tfull[S::kBufs], tempty[S::kBufs];
-  uint64_t drain;
+  uint64_t tfull[S::kHalves][S::kBufs], tempty[S::kHalves][S::kBufs];
+  uint64_t drain[S::kHalves];
   uint32_t tmem;
   int abort;
 };
 
-template <bool CL>
-__device__ __forceinline__ bool wait_once(uint64_t* bar, uint32_t parity) {
-  return CL ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+// Waits until the phase of `parity` has completed; false when it has not after 2^21
+// tries of up to a microsecond each (about 2 s). The loop is one block of assembly:
+// the compiler's own form of it kept the lanes apart and cost the hot loops a third of
+// their instructions.
+__device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "AGAIN:\n"
+      " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, 1000;\n"
+      " @p bra DONE;\n"
+      " add.u32 n, n, 1;\n"
+      " setp.lt.u32 q, n, 0x200000;\n"
+      " @q bra AGAIN;\n"
+      "DONE:\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// One look without waiting. While MMAs run, a shared-memory access of any kind takes
+// 150 to 250 cycles, so the loops ask for the next block's barrier early and use the
+// answer late.
+__device__ __forceinline__ uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
+}
+// The same for a converged warp (one answer for all lanes); a timeout is recorded.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* abort) {
+  if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
+  *reinterpret_cast<volatile int*>(abort) = 1;
+  *reinterpret_cast<volatile int*>(&g_fp8_status) = PKT_DEV_TIMEOUT_PIPE;
+  return false;
 }
 
-// Waits until the phase of `parity` has completed; false when the time ran out here
-// or somewhere else in the CTA.
-template <bool CL>
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* abort) {
-  if (wait_once<CL>(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t it = 0;
-  while (!wait_once<CL>(bar, parity)) {
-    if ((++it & 31u) == 0) {
-      if (*reinterpret_cast<volatile int*>(abort)) return false;
-      if (globaltimer_ns() - t0 > kWaitNs) {
-        *reinterpret_cast<volatile int*>(abort) = 1;
-        atomicExch(&g_fp8_status, PKT_DEV_TIMEOUT_PIPE);
-        return false;
-      }
-    }
-  }
-  return true;
+// One lane of a converged warp; known to the compiler as one, which lets the
+// descriptors of tcgen05 instructions stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred P;\n elect.sync _|P, 0xffffffff;\n selp.u32 %0, 1, 0, P;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// One word global -> shared without waiting for it; zero where !in.
+__device__ __forceinline__ void copy_word_async(float* to, const float* from, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(in ? 4 : 0) : "memory");
+}
+// Arrives on `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Arrives on a barrier of another CTA of the cluster. Only the order of TMEM reads
+// matters here (tcgen05.wait::ld and the fence come before it), no memory is handed
+// over: a release at cluster scope would wait for this thread's global stores, which
+// measured 2000 cycles per block of K.
+__device__ __forceinline__ void arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 template <int PAIR>
@@ -114,10 +163,9 @@ __device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t ad, uint64_t bd, ui
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
-  tmem_ld32(taddr, r);
-  tmem_ld_wait_regs(r);
-}
+// Columns of this warp's 32 lanes to registers; they hold the values after tmem_wait.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) { tmem_ld_wait_regs(r); }
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -125,6 +173,8 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
                  "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
@@ -132,31 +182,9 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
                : "memory");
 }
 
-// Two fp32 lanes in one 64-bit register.
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
@@ -178,30 +206,29 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int row, int col, fl
     static_cast<float*>(a.out)[at] = v;
 }
 
-// Columns [col, col + 8) of one row per lane.
-__device__ __forceinline__ void store_row8(const Fp8Args& a, int row, int col, const float (&v)[8]) {
-  if (row >= a.rows) return;
-  if (a.wide && col + 8 <= a.cols) {
-    if (a.out_bf16) {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)row * a.ldo + col) =
-          make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-    } else {
-      float4* to = reinterpret_cast<float4*>(static_cast<float*>(a.out) + (long long)row * a.ldo + col);
-      to[0] = make_float4(v[0], v[1], v[2], v[3]);
-      to[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
+// 4 consecutive values along out's rows: of one row, or (swap) of one column.
+__device__ __forceinline__ void store_four(const Fp8Args& a, int row, int col, float4 v) {
+  const int at = a.swap ? row : col, end = a.swap ? a.rows : a.cols;
+  if (a.swap ? col >= a.cols : row >= a.rows) return;
+  const long long off = (long long)(a.swap ? col : row) * a.ldo + at;
+  if (a.wide && at + 4 <= end) {
+    if (a.out_bf16)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + off) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    else
+      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + off) = v;
     return;
   }
+  const float u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < a.cols) store_one(a, row, col + i, v[i]);
+  for (int i = 0; i < 4; ++i)
+    if (at + i < end) store_one(a, a.swap ? row + i : row, a.swap ? col : col + i, u[i]);
 }
 
 template <int BN, int PAIR, bool COLV>
 __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(const __grid_constant__ Fp8Args a) {
   using S = Shape<BN, PAIR>;
-  extern __shared__ uint8_t smem_raw[];
-  Smem<BN, PAIR>& s = *reinterpret_cast<Smem<BN, PAIR>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];  // the swizzle pattern's alignment
+  Smem<BN, PAIR>& s = *reinterpret_cast<Smem<BN, PAIR>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t cluster_size;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cluster_size));
@@ -210,9 +237,11 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   const uint32_t half = PAIR == 2 ? rank : 0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
-    for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[i], 1), mbar_init(&s.tempty[i], S::kEpiWarps * PAIR);
-    mbar_init(&s.drain, 1);
+    for (int i = 0; i < S::kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], S::kHalves);
+    for (int i = 0; i < S::kScales; ++i) mbar_init(&s.sfull[i], 32), mbar_init(&s.sempty[i], S::kEpiWarps);
+    for (int h = 0; h < S::kHalves; ++h)
+      for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[h][i], 1), mbar_init(&s.tempty[h][i], 4 * PAIR);
+    for (int h = 0; h < S::kHalves; ++h) mbar_init(&s.drain[h], 1);
     s.abort = 0;
     fence_mbar_init();
   }
@@ -238,81 +267,86 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   if (warp == S::kEpiWarps) {
     // ---- producer: one lane
     if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, issued = 0;
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step) {
-        int tr, tc;
-        tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
-        const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (BN / PAIR);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = wait_phase<false>(&s.empty[stage], phase ^ 1, &s.abort))) break;
+    uint32_t stage = 0, phase = 0, issued = 0;
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step) {
+      int tr, tc;
+      tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
+      const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (S::kCols / PAIR);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = wait_phase(&s.empty[stage], phase ^ 1, &s.abort))) break;
+        if (elect_one()) {
           if (half == 0) mbar_arrive_expect_tx(&s.full[stage], PAIR * S::kStageBytes);
           uint8_t* to = s.stages[stage];
           if (PAIR == 2) {
             const uint32_t bar = mapa_shared(smem_u32(&s.full[stage]), 0);  // both CTAs' bytes count on the leader's barrier
             tma_load_2d_pair(to, &a.map_r, bar, kb * kKBytes, r0);
-            tma_load_2d_pair(to + S::kRowBytes, &a.map_c, bar, kb * kKBytes, c0);
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)  // each half's columns come from both CTAs
+              tma_load_2d_pair(to + S::kRowBytes + h * (S::kColBytes / S::kHalves), &a.map_c, bar, kb * kKBytes, c0 + h * S::kCols);
           } else {
             tma_load_2d(to, &a.map_r, &s.full[stage], kb * kKBytes, r0);
             tma_load_2d(to + S::kRowBytes, &a.map_c, &s.full[stage], kb * kKBytes, c0);
           }
-          ++issued;
-          if (++stage == S::kStages) stage = 0, phase ^= 1;
         }
-      }
-      // every issued copy lands before the CTA may exit (the leader's barriers count
-      // the other CTA's bytes too, which the final cluster barrier waits for)
-      const uint32_t last = half != 0 ? 0 : min(issued, uint32_t(S::kStages));
-      for (uint32_t i = 0; i < last; ++i) {
-        const uint32_t fill = issued - 1 - i;
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&s.full[fill % S::kStages], (fill / S::kStages) & 1))
-          if (globaltimer_ns() - t0 > kWaitNs) break;
+        __syncwarp();
+        ++issued;
+        if (++stage == S::kStages) stage = 0, phase ^= 1;
       }
     }
+    // every issued copy lands before the CTA may exit (the leader's barriers count
+    // the other CTA's bytes too, which the final cluster barrier waits for)
+    const uint32_t last = half != 0 ? 0 : min(issued, uint32_t(S::kStages));
+    for (uint32_t i = 0; i < last; ++i) {
+      const uint32_t fill = issued - 1 - i;
+      try_phase(&s.full[fill % S::kStages], (fill / S::kStages) & 1);
+    }
     __syncwarp();
-  } else if (warp == S::kEpiWarps + 1) {
-    // ---- MMA issuer: the leader's warp, one lane issues
+  } else if (warp == S::kEpiWarps + 1 || (S::kHalves == 2 && warp == S::kEpiWarps + 3)) {
+    // ---- MMA issuers, in the leader CTA: a warp per half, as issuing a block's MMAs
+    // and commits takes about as long as running them; one lane issues
     if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    const int h = warp == S::kEpiWarps + 1 ? 0 : 1;
     if (half == 0) {
       uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
+      uint32_t loaded = 0, drained = 0;  // the next block's barriers were found complete
       bool ok = true, any = false;
       const uint64_t hi = smem_desc(0, 16, 1024, 2);
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = kb0; kb < kb1; ++kb) {
-          ok = wait_phase<(PAIR == 2)>(&s.tempty[buf], bphase ^ 1, &s.abort);
-          ok = ok && wait_phase<false>(&s.full[stage], phase, &s.abort);
-          ok = __all_sync(0xffffffffu, ok);
+          if (!__all_sync(0xffffffffu, loaded)) ok = wait_phase(&s.full[stage], phase, &s.abort);
+          if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[h][buf], bphase ^ 1, &s.abort);
           if (!ok) break;
+          const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes + h * (S::kColBytes / S::kHalves);
+          const uint32_t to = tmem + (buf * S::kHalves + h) * S::kCols;
+          const uint32_t now = stage, nbuf = buf;
+          if (++stage == S::kStages) stage = 0, phase ^= 1;
+          if (++buf == S::kBufs) buf = 0, bphase ^= 1;
+          loaded = peek_phase(&s.full[stage], phase);
+          drained = peek_phase(&s.tempty[h][buf], bphase ^ 1);
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes;
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_fp8<PAIR>(tmem + buf * BN, hi | uint64_t((sr + 32 * k) >> 4), hi | uint64_t((sc + 32 * k) >> 4), a.idesc, k > 0);
+              mma_fp8<PAIR>(to, hi | uint64_t((sr + 32 * k) >> 4), hi | uint64_t((sc + 32 * k) >> 4), a.idesc, k > 0);
             if (PAIR == 2)
-              mma_commit_pair_both(&s.empty[stage]), mma_commit_pair_both(&s.tfull[buf]);
+              mma_commit_pair_both(&s.tfull[h][nbuf]), mma_commit_pair_both(&s.empty[now]);
             else
-              mma_commit(&s.empty[stage]), mma_commit(&s.tfull[buf]);
+              mma_commit(&s.tfull[h][nbuf]), mma_commit(&s.empty[now]);
           }
           __syncwarp();
           any = true;
-          if (++stage == S::kStages) stage = 0, phase ^= 1;
-          if (++buf == S::kBufs) buf = 0, bphase ^= 1;
         }
       }
       if (any) {  // no MMA is in flight when TMEM is released
-        if (lane == 0) {
+        if (elect_one()) {
           if (PAIR == 2)
-            mma_commit_pair_local(&s.drain);
+            mma_commit_pair_local(&s.drain[h]);
           else
-            mma_commit(&s.drain);
+            mma_commit(&s.drain[h]);
         }
         __syncwarp();
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&s.drain, 0))
-          if (globaltimer_ns() - t0 > kWaitNs) break;
+        try_phase(&s.drain[h], 0);
       }
     }
     __syncwarp();
@@ -320,121 +354,204 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
     // ---- epilogue
     if (S::kHalves == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quad = warp & 3, side = warp >> 2;
-    uint32_t buf = 0, bphase = 0;
+    uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
     bool ok = true;
     for (int t = first; ok && t < tiles; t += step) {
       int tr, tc;
       tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
       const int row = (tr * PAIR + int(half)) * kRows + quad * 32 + lane, col0 = tc * BN + side * S::kCols;
-      const float* pr = a.scale_r + (min(row, a.rows - 1) >> a.r_shift);
-      // the scale of a column (COLV: 4 columns per lane) or of all columns of the warp
-      const float* pc = a.scale_c + (min(col0, a.cols - 1) >> a.c_shift);
-      uint64_t acc[S::kCols / 2];
+      float acc[S::kCols];
 #pragma unroll
-      for (int i = 0; i < S::kCols / 2; ++i) acc[i] = 0;
-      constexpr int kPer = (S::kCols + 31) / 32;
-      float rs = 0.f, cs[kPer];
-      auto fetch = [&](int kb) {
-        rs = pr[kb * a.ld_r];
-        if (COLV) {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int c = col0 + lane + 32 * i;
-            cs[i] = c < a.cols && lane + 32 * i < S::kCols ? a.scale_c[kb * a.ld_c + c] : 0.f;
-          }
-        } else {
-          cs[0] = pc[kb * a.ld_c];
-        }
+      for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
+      // the scales of a block are fetched while the block before it is added, and its
+      // barrier is asked for
+      float next_r = 0.f, next_c = 1.f;
+      auto fetch = [&](int kb, uint32_t at, uint32_t ph) {
+        const int in = (kb - kb0) % S::kGroup;
+        if (in == 0 && !wait_phase(&s.sfull[at], ph, &s.abort)) return false;
+        next_r = s.row_scale[at][in][quad * 32 + lane];
+        if (!COLV) next_c = s.col_scale[at][in][side];
+        return true;
       };
-      if (kb0 < kb1) fetch(kb0);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const float r = rs, c = cs[0];
-        if (COLV) {
-          __syncwarp();  // the last block's scales have been read
-#pragma unroll
-          for (int i = 0; i < kPer; ++i)
-            if (lane + 32 * i < S::kCols) s.col_scale[warp][lane + 32 * i] = cs[i];
-          __syncwarp();
-        }
-        if (kb + 1 < kb1) fetch(kb + 1);
-        ok = __all_sync(0xffffffffu, wait_phase<(PAIR == 2)>(&s.tfull[buf], bphase, &s.abort));
+      uint32_t ready = 0;
+      if (kb0 < kb1) ok = fetch(kb0, slot, sphase);
+      for (int kb = kb0; ok && kb < kb1; ++kb) {
+        const int in = (kb - kb0) % S::kGroup;
+        const bool last = in == S::kGroup - 1 || kb == kb1 - 1;
+        const float scale = next_r * next_c;
+        const float* cs = &s.col_scale[slot][in][side * S::kCols];
+        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[side][buf], bphase, &s.abort);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t both = COLV ? pair_of(r, r) : pair_of(r * c, r * c);
-        const uint32_t from = tmem + buf * BN + side * S::kCols + (uint32_t(quad * 32) << 16);
+        const uint32_t from = tmem + (buf * S::kHalves + side) * S::kCols + (uint32_t(quad * 32) << 16);
+        constexpr int kLoads = S::kCols / S::kChunk;
+        // the next load is in flight while one is added; with a scale per column the
+        // registers hold the chunk's scales instead, loaded under the TMEM load
+        uint32_t v[COLV ? 1 : 2][S::kChunk];
+        tmem_load(from, v[0]);
+        if (kb + 1 < kb1) {
+          const bool wrap = slot + 1 == S::kScales;
+          ok = fetch(kb + 1, last ? (wrap ? 0 : slot + 1) : slot, last && wrap ? sphase ^ 1 : sphase);
+        }
 #pragma unroll
-        for (int j = 0; j < S::kCols / S::kChunk; ++j) {
-          uint32_t v[S::kChunk];
-          tmem_load(from + j * S::kChunk, v);
-          if (j == S::kCols / S::kChunk - 1) {  // all of the buffer is in registers
+        for (int j = 0; j < kLoads; ++j) {
+          float4 c[COLV ? S::kChunk / 4 : 1];
+          if (COLV) {
+#pragma unroll
+            for (int i = 0; i < S::kChunk / 4; ++i) c[i] = *reinterpret_cast<const float4*>(cs + j * S::kChunk + 4 * i);
+          }
+          uint32_t(&u)[S::kChunk] = v[COLV ? 0 : j & 1];
+          tmem_wait(u);
+          if (j + 1 == kLoads) {  // all of the buffer is in registers
+            ready = peek_phase(&s.tfull[side][buf + 1 == S::kBufs ? 0 : buf + 1], buf + 1 == S::kBufs ? bphase ^ 1 : bphase);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
               if (PAIR == 2 && half != 0)
-                mbar_arrive_remote(mapa_shared(smem_u32(&s.tempty[buf]), 0));
+                arrive_peer(mapa_shared(smem_u32(&s.tempty[side][buf]), 0));
               else
-                mbar_arrive(&s.tempty[buf]);
+                mbar_arrive(&s.tempty[side][buf]);
             }
+          } else if (!COLV) {
+            tmem_load(from + (j + 1) * S::kChunk, v[(j + 1) & 1]);
           }
 #pragma unroll
-          for (int i = 0; i < S::kChunk; i += 2) {
-            const int at = (j * S::kChunk + i) / 2;
-            const uint64_t p = pair_of(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          for (int i = 0; i < S::kChunk; ++i) {
+            const float p = __uint_as_float(u[i]);
+            float& to = acc[j * S::kChunk + i];
             if (COLV) {
-              const float2 c2 = *reinterpret_cast<const float2*>(&s.col_scale[warp][j * S::kChunk + i]);
-              acc[at] = fma2(p, mul2(pair_of(c2.x, c2.y), both), acc[at]);
+              const float4& q = c[i / 4];
+              to = fmaf(p * (i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w), scale, to);
             } else {
-              acc[at] = fma2(p, both, acc[at]);
+              to = fmaf(p, scale, to);
             }
           }
+          if (COLV && j + 1 < kLoads) tmem_load(from + (j + 1) * S::kChunk, v[0]);
+        }
+        if (last) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.sempty[slot]);
+          if (++slot == S::kScales) slot = 0, sphase ^= 1;
         }
         if (++buf == S::kBufs) buf = 0, bphase ^= 1;
       }
       if (!ok) break;
       if (PAIR == 1 && split > 1) {
-        // this CTA's sums over its part of K, column by column (the operand stages
-        // have all been consumed: the last block's product has been read)
+        // this CTA's sums over its part of K, 4 consecutive values of the result to 16
+        // bytes (the operand stages have all been consumed: the last block's product
+        // has been read)
         float* sums = reinterpret_cast<float*>(s.stages);
+        const int at = quad * 32 + lane;
+        if (a.swap) {
 #pragma unroll
-        for (int i = 0; i < S::kCols / 2; ++i) {
-          const float2 v = unpair(acc[i]);
-          sums[(side * S::kCols + 2 * i) * kRows + quad * 32 + lane] = v.x;
-          sums[(side * S::kCols + 2 * i + 1) * kRows + quad * 32 + lane] = v.y;
+          for (int i = 0; i < S::kCols; ++i) sums[(side * S::kCols + i) * kRows + at] = acc[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::kCols; i += 4)
+            *reinterpret_cast<float4*>(sums + at * (BN + 4) + side * S::kCols + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         }
-      } else if (a.swap) {
+      } else if (S::kStore && a.tma_out) {
+        // 32 rows x 128 bytes at a time through swizzled shared memory
+        uint8_t* to = s.staging[S::kStore ? warp : 0];
+        const int row0 = row - lane, per = a.out_bf16 ? 64 : 32;
 #pragma unroll
-        for (int i = 0; i < S::kCols / 2; ++i) {
-          const float2 v = unpair(acc[i]);
-          if (row < a.rows && col0 + 2 * i < a.cols) store_one(a, row, col0 + 2 * i, v.x);
-          if (row < a.rows && col0 + 2 * i + 1 < a.cols) store_one(a, row, col0 + 2 * i + 1, v.y);
+        for (int j = 0; j < S::kCols / 32; ++j) {
+          if (!a.out_bf16 || (j & 1) == 0) {
+            if (lane == 0) bulk_wait_read_all();  // the last store has left the staging
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            const float* v = acc + j * 32 + i;
+            if (a.out_bf16) {
+              *reinterpret_cast<uint4*>(to + lane * 128 + ((((j & 1) * 4 + i / 8) ^ (lane & 7)) << 4)) =
+                  make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            } else {
+              *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4) ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4 + 1) ^ (lane & 7)) << 4)) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+          }
+          if (!a.out_bf16 || (j & 1) == 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            const int col = col0 + j * 32 + 32 - per;
+            if (lane == 0 && row0 < a.rows && col < a.cols) {
+              tma_store_2d(&a.map_out, to, col, row0);
+              bulk_commit();
+            }
+          }
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < S::kCols / 2; i += 4) {
-          const float2 v0 = unpair(acc[i]), v1 = unpair(acc[i + 1]), v2 = unpair(acc[i + 2]), v3 = unpair(acc[i + 3]);
-          const float v[8] = {v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
-          store_row8(a, row, col0 + 2 * i, v);
-        }
+        for (int i = 0; i < S::kCols; ++i)
+          if (row < a.rows && col0 + i < a.cols) store_one(a, row, col0 + i, acc[i]);
       }
     }
-  } else if constexpr (S::kHalves == 2) {  // two warps that only complete the register exchange
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (S::kStore && a.tma_out && lane == 0) bulk_wait_all();
+  } else {
+    // ---- scales: a warp copies those of the tile's rows and columns, blocks ahead
+    if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == S::kEpiWarps + 2) {
+      uint32_t slot = 0, phase = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int tr, tc;
+        tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
+        const int row0 = (tr * PAIR + int(half)) * kRows, col0 = tc * BN;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if ((kb - kb0) % S::kGroup == 0) {
+            ok = (wait_phase(&s.sempty[slot], phase ^ 1, &s.abort));
+            if (!ok) break;
+          }
+          const int in = (kb - kb0) % S::kGroup;
+          const float *pr = a.scale_r + kb * a.ld_r, *pc = a.scale_c + kb * a.ld_c;
+#pragma unroll
+          for (int i = 0; i < kRows; i += 32) {
+            const int row = row0 + lane + i;
+            copy_word_async(&s.row_scale[slot][in][lane + i], pr + (min(row, a.rows - 1) >> a.r_shift), row < a.rows);
+          }
+          if (COLV) {
+#pragma unroll
+            for (int i = 0; i < BN; i += 32) {
+              const int col = col0 + lane + i;
+              if (BN >= 32 || lane < BN) copy_word_async(&s.col_scale[slot][in][lane + i], pc + min(col, a.cols - 1), col < a.cols);
+            }
+          } else if (lane < S::kHalves) {
+            const int col = col0 + lane * S::kCols;
+            copy_word_async(&s.col_scale[slot][in][lane], pc + (min(col, a.cols - 1) >> 7), col < a.cols);
+          }
+          if (in == S::kGroup - 1 || kb == kb1 - 1) {
+            copy_arrive(&s.sfull[slot]);
+            if (++slot == S::kScales) slot = 0, phase ^= 1;
+          }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    __syncwarp();
   }
 
   __syncthreads();
   if (PAIR == 1 && split > 1) {
     cluster_sync();  // the sums of every CTA of the cluster are in its shared memory
-    if (warp < 4 && first < tiles && !*reinterpret_cast<volatile int*>(&s.abort)) {
+    if (first < tiles && !*reinterpret_cast<volatile int*>(&s.abort)) {
       int tr, tc;
       tile_at(first, a.tiles_r, a.tiles_c, &tr, &tc);
-      const int per = BN / split, at = warp * 32 + lane, row = tr * kRows + at;
-      for (int c = part * per; c < (part + 1) * per; ++c) {
-        const int col = tc * BN + c;
-        if (row >= a.rows || col >= a.cols) continue;
-        const uint32_t from = smem_u32(reinterpret_cast<float*>(s.stages) + c * kRows + at);
-        float v = 0.f;
-        for (int q = 0; q < split; ++q) v += ld_cluster(mapa_shared(from, q));
-        store_one(a, row, col, v);
+      const uint32_t sums = smem_u32(s.stages);
+      uint32_t peer[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) peer[q] = mapa_shared(sums, min(q, split - 1));
+      // a part of the tile's groups of 4 values for each CTA, added in rank order
+      constexpr int kItems = kRows * BN / 4;
+      for (int i = part * kItems / split + int(threadIdx.x); i < (part + 1) * kItems / split; i += S::kThreads) {
+        const int r = a.swap ? i % (kRows / 4) * 4 : i / (BN / 4), c = a.swap ? i / (kRows / 4) : i % (BN / 4) * 4;
+        const uint32_t at = 4 * (a.swap ? c * kRows + r : r * (BN + 4) + c);
+        float4 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < split ? ld_cluster(peer[q] + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 1; q < 8; ++q) v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+        store_four(a, tr * kRows + r, tc * BN + c, v[0]);
       }
     }
   }
@@ -463,10 +580,24 @@ int operand_map(CUtensorMap* map, const void* base, int k, int rows, long long l
   return r == CUDA_SUCCESS ? PKT_OK : fail(PKT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
 }
 
+// The result in boxes of 32 rows x 128 bytes (one epilogue warp's staging).
+int result_map(CUtensorMap* map, void* base, int dtype, int cols, int rows, long long ld) {
+  const EncodeTiled enc = op_encode_tiled();
+  if (!enc) return fail(PKT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const bool bf = dtype == PKT_DTYPE_BF16;
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * (bf ? 2 : 4)};
+  cuuint32_t box[2] = {bf ? 64u : 32u, 32};
+  cuuint32_t ones[2] = {1, 1};
+  const CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, dims, strides, box, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? PKT_OK : fail(PKT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+}
+
 template <int BN, int PAIR, bool COLV>
 cudaError_t fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaStream_t st) {
   using S = Shape<BN, PAIR>;
-  constexpr int smem = int(sizeof(Smem<BN, PAIR>)) + 1024;
+  constexpr int smem = int(sizeof(Smem<BN, PAIR>));
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   static std::atomic<bool> ready[64];
   if (!ready[dev].load(std::memory_order_acquire)) {
@@ -550,16 +681,21 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
     while (split < 8 && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
   const void *pr = swap ? d->b : d->a, *pc = swap ? d->a : d->b;
   if ((rc = operand_map(&a.map_r, pr, d->K, a.rows, swap ? d->ldb : d->lda, kRows)) ||
-      (rc = operand_map(&a.map_c, pc, d->K, a.cols, swap ? d->lda : d->ldb, bn / pair)))
+      (rc = operand_map(&a.map_c, pc, d->K, a.cols, swap ? d->lda : d->ldb, (bn > 128 ? 128 : bn) / pair)))
     return rc;
   a.scale_r = swap ? d->scale_b : d->scale_a, a.ld_r = swap ? d->ld_scale_b : d->ld_scale_a;
   a.scale_c = swap ? d->scale_a : d->scale_b, a.ld_c = swap ? d->ld_scale_a : d->ld_scale_b;
   a.r_shift = (swap ? d->b_block_rows : d->a_block_rows) == 1 ? 0 : 7;
   a.c_shift = (swap ? d->a_block_rows : d->b_block_rows) == 1 ? 0 : 7;
   a.out = d->out, a.ldo = d->ldo, a.out_bf16 = es == 2, a.swap = swap;
-  a.wide = !swap && aligned_to(d->out, 16) && d->ldo * es % 16 == 0;
+  a.wide = aligned_to(d->out, 4 * es) && d->ldo % 4 == 0;
+  // TMA stores need 16-byte aligned rows; else value by value
+  if (!swap && aligned_to(d->out, 16) && d->ldo * es % 16 == 0) {
+    if ((rc = result_map(&a.map_out, d->out, d->out_dtype, d->N, d->M, d->ldo))) return rc;
+    a.tma_out = 1;
+  }
   const uint32_t fr = (swap ? d->b_dtype : d->a_dtype) == PKT_DTYPE_E5M2, fc = (swap ? d->a_dtype : d->b_dtype) == PKT_DTYPE_E5M2;
-  a.idesc = (1u << 4) | (fr << 7) | (fc << 10) | (uint32_t(bn >> 3) << 17) | (uint32_t((kRows * pair) >> 4) << 24);
+  a.idesc = (1u << 4) | (fr << 7) | (fc << 10) | (uint32_t((bn > 128 ? 128 : bn) >> 3) << 17) | (uint32_t((kRows * pair) >> 4) << 24);
   // a cluster per tile when K is split, else a persistent grid
   const int clusters = split > 1 ? int(tiles) : int(std::min<long long>(tiles, sms / pair));
   const int cs = pair == 2 ? 2 : split;
