@@ -284,6 +284,11 @@ int pkt_axpy_noalloc_status(int* code, int* task_index, int* detail);
  * A descriptor is read during the call only. Outputs must not overlap inputs
  * unless an operator says so. No counterpart in pkt. */
 
+/* Every wait inside their kernels is bounded (about 2 s). code: PKT_DEV_TIMEOUT_PIPE
+ * when one has run out on the current device since the last call (results since then
+ * are not valid), else PKT_DEV_OK. Synchronises the device and clears the word. */
+int pkt_ops_status(int* code);
+
 /* Layer norm over the last dimension of [rows, cols]. Statistics and sums are
  * fp32; each result is rounded to its type once.
  *   forward   mean = sum x / C, rstd = 1/sqrt(sum (x-mean)^2 / C + eps),
@@ -381,11 +386,6 @@ typedef struct pkt_fp8_gemm_desc {
   int out_dtype;        /* PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
 } pkt_fp8_gemm_desc;
 int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream);
-/* Whether a wait inside a pkt_fp8_gemm launch on the current device ran out of time
- * since the last call (PKT_DEV_OK or PKT_DEV_TIMEOUT_PIPE; its output is then not
- * valid). Synchronises the device and clears the word. */
-int pkt_fp8_gemm_status(int* code);
-
 /* AdamW over many tensors in one launch. For step t of a tensor, with g = grad *
  * gradient scale:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2

@@ -130,7 +130,7 @@ _SIGS = {
     "pkt_layernorm_backward": ([ctypes.POINTER(LayerNormDesc), _P], c_int),
     "pkt_fp8_quantize": ([ctypes.POINTER(Fp8QuantizeDesc), _P], c_int),
     "pkt_fp8_gemm": ([ctypes.POINTER(Fp8GemmDesc), _P], c_int),
-    "pkt_fp8_gemm_status": ([ctypes.POINTER(c_int)], c_int),
+    "pkt_ops_status": ([ctypes.POINTER(c_int)], c_int),
     "pkt_adamw_create": ([c_int, ctypes.POINTER(AdamWConfig), ctypes.POINTER(_P)], c_int),
     "pkt_adamw_destroy": ([_P], c_int),
     "pkt_adamw_step": ([_P, c_float, c_float, _P, _P], c_int),

@@ -5,7 +5,8 @@
 // The tensors are cut into chunks of 4096 values, listed once in device memory; a
 // block takes every gridDim-th chunk, and within it a warp owns blocks of 128 values,
 // 4 per lane, so that a block of 8-bit states is quantised with one warp reduction.
-// All loads of a warp's share are issued before the first is used.
+// All loads of a warp's share are issued before the first is used, and the scales of
+// its 8 state blocks are computed at once, one per lane.
 //
 // 8-bit states hold m and r = sqrt(v) as e4m3 with an fp32 scale per 128 values. The
 // root, because its range is half of v's in octaves (e4m3 spans 18 octaves below the
@@ -76,40 +77,42 @@ __global__ void adam_set_state(AdamState* s, double pow1, double pow2, long long
   s->inv_root_bc2 = float(1.0 / sqrt(1.0 - pow2 * beta2));
 }
 
-// A lane's 4 values of one block: consecutive (one access) in whole blocks of
-// aligned tensors, 32 apart otherwise.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool wide, int lane, int left, float (&v)[4]) {
-  if (wide) {
-    Raw<T, 4> r;
-    r.load(p + 4 * lane, 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = r.get(i);
+// A lane's 4 values of a block of 128: consecutive, one access (FULL), or 32 apart and
+// one by one, only those inside the tensor.
+template <bool FULL, typename T>
+__device__ __forceinline__ void load4(const T* p, int lane, int left, Raw<T, 4>* r) {
+  if constexpr (FULL) {
+    r->load(p + 4 * lane, true);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = lane + 32 * i < left ? to_f32(p[lane + 32 * i]) : 0.f;
+    for (int i = 0; i < Raw<T, 4>::kWords; ++i) r->w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < left) r->set(i, p[lane + 32 * i]);
   }
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, bool wide, int lane, int left, const float (&v)[4]) {
-  if (wide) {
-    store_vec<T, 4>(p + 4 * lane, v, 4);
+template <bool FULL, typename T>
+__device__ __forceinline__ void store4(T* p, int lane, int left, const float (&v)[4]) {
+  if constexpr (FULL) {
+    store_vec<T, 4>(p + 4 * lane, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (lane + 32 * i < left) from_f32(v[i], p + lane + 32 * i);
   }
 }
-__device__ __forceinline__ uint32_t load_bytes4(const uint8_t* p, bool wide, int lane, int left) {
-  if (wide) return *reinterpret_cast<const uint32_t*>(p + 4 * lane);
+template <bool FULL>
+__device__ __forceinline__ uint32_t load_bytes4(const uint8_t* p, int lane, int left) {
+  if constexpr (FULL) return *reinterpret_cast<const uint32_t*>(p + 4 * lane);
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (lane + 32 * i < left) w |= uint32_t(p[lane + 32 * i]) << (8 * i);
   return w;
 }
-__device__ __forceinline__ void store_bytes4(uint8_t* p, bool wide, int lane, int left, uint32_t w) {
-  if (wide) {
+template <bool FULL>
+__device__ __forceinline__ void store_bytes4(uint8_t* p, int lane, int left, uint32_t w) {
+  if constexpr (FULL) {
     *reinterpret_cast<uint32_t*>(p + 4 * lane) = w;
   } else {
 #pragma unroll
@@ -119,91 +122,118 @@ __device__ __forceinline__ void store_bytes4(uint8_t* p, bool wide, int lane, in
 }
 __device__ __forceinline__ void unpack4(uint32_t w, float scale, float (&v)[4]) {
   const float2 lo = unpack_e4m3x2(uint16_t(w)), hi = unpack_e4m3x2(uint16_t(w >> 16));
-  v[0] = lo.x * scale, v[1] = lo.y * scale, v[2] = hi.x * scale, v[3] = hi.y * scale;
+  v[0] = __fmul_rn(lo.x, scale), v[1] = __fmul_rn(lo.y, scale), v[2] = __fmul_rn(hi.x, scale), v[3] = __fmul_rn(hi.y, scale);
+}
+
+// The factors of a step that all values share.
+struct AdamStep {
+  float gs, keep, step_size, inv_root;
+};
+
+// A warp's 4 blocks of 128 values from `base` on. FULL: all of them inside the tensor
+// and every array aligned.
+template <typename P, typename G, bool EIGHT, bool FULL>
+__device__ __forceinline__ void adam_blocks(const AdamArgs& a, const AdamTensor& t, const AdamStep& u, long long base, int lane) {
+  constexpr int B = kBlocksPerWarp;
+  P* param = static_cast<P*>(t.param) + base;
+  Raw<P, 4> rp[B];
+  Raw<G, 4> rg[B];
+  Raw<float, 4> rm[EIGHT ? 1 : B], rv[EIGHT ? 1 : B];
+  uint32_t mq[EIGHT ? B : 1], vq[EIGHT ? B : 1];
+  float ms[EIGHT ? B : 1], vs[EIGHT ? B : 1];
+  const long long sb = base / kScaleBlock;
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const int left = FULL ? kScaleBlock : int(min(t.n - base - b * kScaleBlock, (long long)kScaleBlock));
+    load4<FULL>(param + b * kScaleBlock, lane, left, &rp[b]);
+    load4<FULL>(static_cast<const G*>(t.grad) + base + b * kScaleBlock, lane, left, &rg[b]);
+    if constexpr (EIGHT) {
+      mq[b] = load_bytes4<FULL>(static_cast<const uint8_t*>(t.m) + base + b * kScaleBlock, lane, left);
+      vq[b] = load_bytes4<FULL>(static_cast<const uint8_t*>(t.v) + base + b * kScaleBlock, lane, left);
+      ms[b] = FULL || left > 0 ? t.m_scale[sb + b] : 0.f;
+      vs[b] = FULL || left > 0 ? t.v_scale[sb + b] : 0.f;
+    } else {
+      load4<FULL>(static_cast<const float*>(t.m) + base + b * kScaleBlock, lane, left, &rm[b]);
+      load4<FULL>(static_cast<const float*>(t.v) + base + b * kScaleBlock, lane, left, &rv[b]);
+    }
+  }
+  float m[B][4], r[B][4];  // new m, new sqrt(v)
+  uint32_t big = 0;        // lane b: the largest |m| of block b, lane B + b: of sqrt(v)
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    const int left = FULL ? kScaleBlock : int(min(t.n - base - b * kScaleBlock, (long long)kScaleBlock));
+    float v[4], p[4];
+    if constexpr (EIGHT) {
+      unpack4(mq[b], ms[b], m[b]);
+      unpack4(vq[b], vs[b], v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[b][i] = rm[b].get(i), v[i] = rv[b].get(i);
+    }
+    uint32_t mbig = 0, rbig = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float g = rg[b].get(i) * u.gs;
+      m[b][i] = __fadd_rn(__fmul_rn(m[b][i], a.b1), __fmul_rn(g, a.c1));
+      v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g, g), a.c2));
+      r[b][i] = __fsqrt_rn(v[i]);
+      // the quotient's own error (2 ulp of the step) is far below p's last bit
+      p[i] = rp[b].get(i) * u.keep - __fdividef(u.step_size * m[b][i], fmaf(r[b][i], u.inv_root, a.eps));
+      mbig = max(mbig, abs_bits(m[b][i]));
+      rbig = max(rbig, abs_bits(r[b][i]));
+    }
+    store4<FULL>(param + b * kScaleBlock, lane, left, p);
+    if (t.copy) store4<FULL>(reinterpret_cast<bf16_t*>(t.copy) + base + b * kScaleBlock, lane, left, p);
+    if constexpr (EIGHT) {
+      mbig = __reduce_max_sync(0xffffffffu, mbig);
+      rbig = __reduce_max_sync(0xffffffffu, rbig);
+      if (lane == b) big = mbig;
+      if (lane == B + b) big = rbig;
+    } else {
+      store4<FULL>(static_cast<float*>(t.m) + base + b * kScaleBlock, lane, left, m[b]);
+      store4<FULL>(static_cast<float*>(t.v) + base + b * kScaleBlock, lane, left, v);
+    }
+  }
+  if constexpr (EIGHT) {
+    float factor, scale;  // of 8 blocks at once, one per lane
+    block_scale(big, 448.f, &factor, &scale);
+    if (lane < 2 * B && (FULL || base + (lane & (B - 1)) * kScaleBlock < t.n)) (lane < B ? t.m_scale : t.v_scale)[sb + (lane & (B - 1))] = scale;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int left = FULL ? kScaleBlock : int(min(t.n - base - b * kScaleBlock, (long long)kScaleBlock));
+      const float mf = __shfl_sync(0xffffffffu, factor, b), rf = __shfl_sync(0xffffffffu, factor, B + b);
+      store_bytes4<FULL>(static_cast<uint8_t*>(t.m) + base + b * kScaleBlock, lane, left,
+                         pack_fp8x4<false>(__fmul_rn(m[b][0], mf), __fmul_rn(m[b][1], mf), __fmul_rn(m[b][2], mf), __fmul_rn(m[b][3], mf)));
+      uint32_t q = pack_fp8x4<false>(__fmul_rn(r[b][0], rf), __fmul_rn(r[b][1], rf), __fmul_rn(r[b][2], rf), __fmul_rn(r[b][3], rf));
+      // a root above zero stays above zero: the smallest 8-bit value is code 1
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r[b][i] > 0.f && rf > 0.f && ((q >> (8 * i)) & 0xffu) == 0) q |= 1u << (8 * i);
+      store_bytes4<FULL>(static_cast<uint8_t*>(t.v) + base + b * kScaleBlock, lane, left, q);
+    }
+  }
 }
 
 template <typename P, typename G, bool EIGHT>
 __global__ void __launch_bounds__(kAdamThreads) adam_step(const AdamArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float lr = a.scales ? a.lr * a.scales[0] : a.lr;
-  const float gs = a.scales ? a.grad_scale * a.scales[1] : a.grad_scale;
-  const float step_size = lr * a.state->inv_bc1, inv_root = a.state->inv_root_bc2;
+  AdamStep u;
+  u.gs = a.scales ? a.grad_scale * a.scales[1] : a.grad_scale;
+  u.step_size = lr * a.state->inv_bc1;
+  u.inv_root = a.state->inv_root_bc2;
   for (int c = blockIdx.x; c < a.num_chunks; c += gridDim.x) {
     const int2 where = a.chunks[c];
     const AdamTensor t = a.tensors[where.x];
     if (t.grad == nullptr) continue;
-    const float keep = 1.f - lr * t.decay;
-    const long long base = (long long)where.y * kChunk + warp * kBlocksPerWarp * kScaleBlock;
-    float p[kBlocksPerWarp][4], g[kBlocksPerWarp][4], m[EIGHT ? 1 : kBlocksPerWarp][4], v[EIGHT ? 1 : kBlocksPerWarp][4];
-    uint32_t mq[EIGHT ? kBlocksPerWarp : 1], vq[EIGHT ? kBlocksPerWarp : 1];
-    float ms[EIGHT ? kBlocksPerWarp : 1], vs[EIGHT ? kBlocksPerWarp : 1];
-#pragma unroll
-    for (int b = 0; b < kBlocksPerWarp; ++b) {
-      const long long at = base + b * kScaleBlock;
-      const int left = int(min(t.n - at, (long long)kScaleBlock));
-      if (left <= 0) continue;
-      const bool wide = t.wide && left == kScaleBlock;
-      load4(static_cast<const P*>(t.param) + at, wide, lane, left, p[b]);
-      load4(static_cast<const G*>(t.grad) + at, wide, lane, left, g[b]);
-      if constexpr (EIGHT) {
-        mq[b] = load_bytes4(static_cast<const uint8_t*>(t.m) + at, wide, lane, left);
-        vq[b] = load_bytes4(static_cast<const uint8_t*>(t.v) + at, wide, lane, left);
-        ms[b] = t.m_scale[at / kScaleBlock];
-        vs[b] = t.v_scale[at / kScaleBlock];
-      } else {
-        load4(static_cast<const float*>(t.m) + at, wide, lane, left, m[b]);
-        load4(static_cast<const float*>(t.v) + at, wide, lane, left, v[b]);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < kBlocksPerWarp; ++b) {
-      const long long at = base + b * kScaleBlock;
-      const int left = int(min(t.n - at, (long long)kScaleBlock));
-      if (left <= 0) continue;
-      const bool wide = t.wide && left == kScaleBlock;
-      float mm[4], vv[4], root[4];
-      if constexpr (EIGHT) {
-        unpack4(mq[b], ms[b], mm);
-        unpack4(vq[b], vs[b], vv);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vv[i] = __fmul_rn(vv[i], vv[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mm[i] = m[b][i], vv[i] = v[b][i];
-      }
-      uint32_t mbig = 0, vbig = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float gr = g[b][i] * gs;
-        mm[i] = __fadd_rn(__fmul_rn(mm[i], a.b1), __fmul_rn(gr, a.c1));
-        vv[i] = __fadd_rn(__fmul_rn(vv[i], a.b2), __fmul_rn(__fmul_rn(gr, gr), a.c2));
-        root[i] = __fsqrt_rn(vv[i]);
-        p[b][i] = p[b][i] * keep - step_size * mm[i] / fmaf(root[i], inv_root, a.eps);
-        mbig = max(mbig, abs_bits(mm[i]));
-        vbig = max(vbig, abs_bits(root[i]));
-      }
-      store4(static_cast<P*>(t.param) + at, wide, lane, left, p[b]);
-      if (t.copy) store4(reinterpret_cast<bf16_t*>(t.copy) + at, wide, lane, left, p[b]);
-      if constexpr (EIGHT) {
-        mbig = __reduce_max_sync(0xffffffffu, mbig);
-        vbig = __reduce_max_sync(0xffffffffu, vbig);
-        float mf, mscale, vf, vscale;
-        block_scale(mbig, 448.f, &mf, &mscale);
-        block_scale(vbig, 448.f, &vf, &vscale);
-        store_bytes4(static_cast<uint8_t*>(t.m) + at, wide, lane, left,
-                     pack_fp8x4<false>(__fmul_rn(mm[0], mf), __fmul_rn(mm[1], mf), __fmul_rn(mm[2], mf), __fmul_rn(mm[3], mf)));
-        uint32_t q = pack_fp8x4<false>(__fmul_rn(root[0], vf), __fmul_rn(root[1], vf), __fmul_rn(root[2], vf), __fmul_rn(root[3], vf));
-        // a root above zero stays above zero: the smallest 8-bit value is code 1
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (root[i] > 0.f && vf > 0.f && ((q >> (8 * i)) & 0xffu) == 0) q |= 1u << (8 * i);
-        store_bytes4(static_cast<uint8_t*>(t.v) + at, wide, lane, left, q);
-        if (lane == 0) t.m_scale[at / kScaleBlock] = mscale, t.v_scale[at / kScaleBlock] = vscale;
-      } else {
-        store4(static_cast<float*>(t.m) + at, wide, lane, left, mm);
-        store4(static_cast<float*>(t.v) + at, wide, lane, left, vv);
-      }
-    }
+    u.keep = 1.f - lr * t.decay;
+    const long long base = (long long)where.y * kChunk + warp * (kBlocksPerWarp * kScaleBlock);
+    if (t.wide && base + kBlocksPerWarp * kScaleBlock <= t.n)
+      adam_blocks<P, G, EIGHT, true>(a, t, u, base, lane);
+    else if (base < t.n)
+      adam_blocks<P, G, EIGHT, false>(a, t, u, base, lane);
   }
   __syncthreads();  // every thread of the block has read the state
   if (threadIdx.x == 0 && atomicAdd(&a.state->ticket, 1u) == gridDim.x - 1) {

@@ -21,7 +21,7 @@
 // accumulators through distributed shared memory in rank order.
 //
 // Every wait is bounded (2 s); one that runs out sets a status word that
-// pkt_fp8_gemm_status reads, and the kernel drains its copies and returns.
+// pkt_ops_status reads, and the kernel drains its copies and returns.
 #include <algorithm>
 #include <atomic>
 
@@ -33,8 +33,6 @@ namespace {
 
 constexpr int kRows = 128;    // TMEM lanes
 constexpr int kKBytes = 128;  // one block of K: a 128-byte row of an operand tile
-
-__device__ int g_fp8_status;
 
 struct alignas(64) Fp8Args {
   CUtensorMap map_r, map_c, map_out;
@@ -48,6 +46,7 @@ struct alignas(64) Fp8Args {
   int out_bf16, swap;  // swap: out[col * ldo + row]
   int wide, tma_out;   // 4 values of out in one store; map_out is valid
   uint32_t idesc;
+  int* status;
 };
 
 template <int BN, int PAIR>
@@ -83,27 +82,6 @@ struct Smem {
   int abort;
 };
 
-// Waits until the phase of `parity` has completed; false when it has not after 2^21
-// tries of up to a microsecond each (about 2 s). The loop is one block of assembly:
-// the compiler's own form of it kept the lanes apart and cost the hot loops a third of
-// their instructions.
-__device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
-      "AGAIN:\n"
-      " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, 1000;\n"
-      " @p bra DONE;\n"
-      " add.u32 n, n, 1;\n"
-      " setp.lt.u32 q, n, 0x200000;\n"
-      " @q bra AGAIN;\n"
-      "DONE:\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // One look without waiting. While MMAs run, a shared-memory access of any kind takes
 // 150 to 250 cycles, so the loops ask for the next block's barrier early and use the
 // answer late.
@@ -116,11 +94,10 @@ __device__ __forceinline__ uint32_t peek_phase(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok;
 }
-// The same for a converged warp (one answer for all lanes); a timeout is recorded.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* abort) {
-  if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
+// A warp's bounded wait; a timeout is recorded for the CTA too.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* status, int* abort) {
+  if (pkb::wait_phase(bar, parity, status)) return true;
   *reinterpret_cast<volatile int*>(abort) = 1;
-  *reinterpret_cast<volatile int*>(&g_fp8_status) = PKT_DEV_TIMEOUT_PIPE;
   return false;
 }
 
@@ -274,7 +251,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
       const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (S::kCols / PAIR);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = wait_phase(&s.empty[stage], phase ^ 1, &s.abort))) break;
+        if (!(ok = wait_phase(&s.empty[stage], phase ^ 1, a.status, &s.abort))) break;
         if (elect_one()) {
           if (half == 0) mbar_arrive_expect_tx(&s.full[stage], PAIR * S::kStageBytes);
           uint8_t* to = s.stages[stage];
@@ -314,8 +291,8 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       const uint64_t hi = smem_desc(0, 16, 1024, 2);
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!__all_sync(0xffffffffu, loaded)) ok = wait_phase(&s.full[stage], phase, &s.abort);
-          if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[h][buf], bphase ^ 1, &s.abort);
+          if (!__all_sync(0xffffffffu, loaded)) ok = wait_phase(&s.full[stage], phase, a.status, &s.abort);
+          if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[h][buf], bphase ^ 1, a.status, &s.abort);
           if (!ok) break;
           const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes + h * (S::kColBytes / S::kHalves);
           const uint32_t to = tmem + (buf * S::kHalves + h) * S::kCols;
@@ -368,7 +345,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       float next_r = 0.f, next_c = 1.f;
       auto fetch = [&](int kb, uint32_t at, uint32_t ph) {
         const int in = (kb - kb0) % S::kGroup;
-        if (in == 0 && !wait_phase(&s.sfull[at], ph, &s.abort)) return false;
+        if (in == 0 && !wait_phase(&s.sfull[at], ph, a.status, &s.abort)) return false;
         next_r = s.row_scale[at][in][quad * 32 + lane];
         if (!COLV) next_c = s.col_scale[at][in][side];
         return true;
@@ -380,7 +357,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
         const bool last = in == S::kGroup - 1 || kb == kb1 - 1;
         const float scale = next_r * next_c;
         const float* cs = &s.col_scale[slot][in][side * S::kCols];
-        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[side][buf], bphase, &s.abort);
+        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[side][buf], bphase, a.status, &s.abort);
         if (!ok) break;
         tc_fence_after();
         const uint32_t from = tmem + (buf * S::kHalves + side) * S::kCols + (uint32_t(quad * 32) << 16);
@@ -500,7 +477,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
         const int row0 = (tr * PAIR + int(half)) * kRows, col0 = tc * BN;
         for (int kb = kb0; kb < kb1; ++kb) {
           if ((kb - kb0) % S::kGroup == 0) {
-            ok = (wait_phase(&s.sempty[slot], phase ^ 1, &s.abort));
+            ok = (wait_phase(&s.sempty[slot], phase ^ 1, a.status, &s.abort));
             if (!ok) break;
           }
           const int in = (kb - kb0) % S::kGroup;
@@ -595,16 +572,13 @@ int result_map(CUtensorMap* map, void* base, int dtype, int cols, int rows, long
 }
 
 template <int BN, int PAIR, bool COLV>
-cudaError_t fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaStream_t st) {
+int fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaStream_t st) {
   using S = Shape<BN, PAIR>;
   constexpr int smem = int(sizeof(Smem<BN, PAIR>));
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
-  static std::atomic<bool> ready[64];
-  if (!ready[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<BN, PAIR, COLV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    ready[dev].store(true, std::memory_order_release);
-  }
+  static std::atomic<uint64_t> done;
+  const int rc = op_shared_memory(reinterpret_cast<const void*>(fp8_gemm_kernel<BN, PAIR, COLV>), &done, dev, smem);
+  if (rc) return rc;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(cluster_size);
@@ -616,11 +590,12 @@ cudaError_t fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, PAIR, COLV>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, PAIR, COLV>, a);
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch fp8 gemm");
 }
 
 template <int BN, int PAIR>
-cudaError_t fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaStream_t st) {
+int fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaStream_t st) {
   return a.c_shift == 0 ? fp8_launch<BN, PAIR, true>(a, dev, clusters, cluster_size, st)
                         : fp8_launch<BN, PAIR, false>(a, dev, clusters, cluster_size, st);
 }
@@ -654,7 +629,8 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
   if (d->K > 0 && ((rc = check_operand("a", d->a, d->lda, d->scale_a, d->ld_scale_a, d->M, d->K, d->a_block_rows, d->a_dtype)) ||
                    (rc = check_operand("b", d->b, d->ldb, d->scale_b, d->ld_scale_b, d->N, d->K, d->b_block_rows, d->b_dtype))))
     return rc;
-  if ((rc = op_device(&dev, &sms)) || (rc = op_check_memory(d->out, "out", dev))) return rc;
+  int* status = nullptr;
+  if ((rc = op_device(&dev, &sms, &status)) || (rc = op_check_memory(d->out, "out", dev))) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->K == 0) {
     const cudaError_t e = cudaMemset2DAsync(d->out, size_t(d->ldo) * es, 0, size_t(d->N) * es, size_t(d->M), st);
@@ -673,6 +649,7 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
     bn = 256, pair = 2;
   }
   Fp8Args a{};
+  a.status = status;
   a.rows = swap ? d->N : d->M, a.cols = swap ? d->M : d->N, a.num_kb = num_kb;
   a.tiles_r = (a.rows - 1) / (kRows * pair) + 1, a.tiles_c = (a.cols - 1) / bn + 1;
   const long long tiles = (long long)a.tiles_r * a.tiles_c;
@@ -699,24 +676,11 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
   // a cluster per tile when K is split, else a persistent grid
   const int clusters = split > 1 ? int(tiles) : int(std::min<long long>(tiles, sms / pair));
   const int cs = pair == 2 ? 2 : split;
-  const cudaError_t e = pair == 2 ? fp8_launch<256, 2>(a, dev, clusters, cs, st)
-                        : bn == 128 ? fp8_launch<128, 1>(a, dev, clusters, cs, st)
-                        : bn == 64 ? fp8_launch<64, 1>(a, dev, clusters, cs, st)
-                        : bn == 32 ? fp8_launch<32, 1>(a, dev, clusters, cs, st)
-                                   : fp8_launch<16, 1>(a, dev, clusters, cs, st);
-  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch fp8 gemm");
-}
-
-int pkt_fp8_gemm_status(int* code) {
-  using namespace pkb;
-  if (!code) return fail(PKT_ERR_ARGS, "null argument");
-  int dev = 0, sms = 0, rc;
-  if ((rc = op_device(&dev, &sms))) return rc;
-  cudaError_t e = cudaDeviceSynchronize();
-  const int zero = 0;
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(code, g_fp8_status, sizeof(int));
-  if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(g_fp8_status, &zero, sizeof(int));
-  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "read the fp8 gemm status");
+  return pair == 2 ? fp8_launch<256, 2>(a, dev, clusters, cs, st)
+         : bn == 128 ? fp8_launch<128, 1>(a, dev, clusters, cs, st)
+         : bn == 64 ? fp8_launch<64, 1>(a, dev, clusters, cs, st)
+         : bn == 32 ? fp8_launch<32, 1>(a, dev, clusters, cs, st)
+                    : fp8_launch<16, 1>(a, dev, clusters, cs, st);
 }
 
 }  // extern "C"

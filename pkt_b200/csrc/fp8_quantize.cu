@@ -5,8 +5,8 @@
 //
 // A warp holds 128 columns of a row, 4 consecutive ones per lane. Rows alone
 // (block_rows 1, no transposed result) need nothing beyond a warp: the largest
-// magnitude is one warp reduction, and every warp takes several rows so that their
-// loads overlap. Otherwise a block of 8 warps takes a 128 x 128 tile into registers
+// magnitude is one warp reduction, and every warp takes 8 rows: their loads overlap and
+// their scales are computed at once, one per lane. Otherwise a block of 8 warps takes a 128 x 128 tile into registers
 // (a lane has 4 columns x 16 rows, so a column's 16 values of a warp are 16
 // consecutive bytes of the transposed result); column maxima meet in shared memory,
 // and the transposed bytes pass through it to leave as whole 128-byte rows.
@@ -33,18 +33,60 @@ struct QuantArgs {
   float most;
 };
 
-constexpr int kRowsPerWarp = 4;
+constexpr int kRowsPerWarp = 8;
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_cols4(const T* row, int col, int cols, float (&v)[4]) {
-  Raw<T, WIDE ? 4 : 1> r[WIDE ? 1 : 4];
-  if (WIDE) {
-    r[0].load(row + col, cols - col);
+// A lane's 4 consecutive values of a row as raw words.
+template <typename T>
+using Row4 = Raw<T, 4>;
+
+// The largest magnitude of 4 values, as bits of |x| in fp32: packed pairs for bf16.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t row_big(const Row4<bf16_t>& r) {
+  const uint32_t m = max_u16x2(r.w[0] & 0x7fff7fffu, r.w[1] & 0x7fff7fffu);
+  return max(m << 16, m & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t row_big(const Row4<float>& r) {
+  return max(max(r.w[0] & 0x7fffffffu, r.w[1] & 0x7fffffffu), max(r.w[2] & 0x7fffffffu, r.w[3] & 0x7fffffffu));
+}
+// The largest magnitude of each of 4 columns over N rows.
+template <int N>
+__device__ __forceinline__ void cols_big(const Row4<bf16_t> (&r)[N], uint32_t (&big)[4]) {
+  uint32_t a = 0, b = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = r[0].get(WIDE ? i : 0);
-  } else {
+  for (int i = 0; i < N; ++i) a = max_u16x2(a, r[i].w[0] & 0x7fff7fffu), b = max_u16x2(b, r[i].w[1] & 0x7fff7fffu);
+  big[0] = a << 16, big[1] = a & 0xffff0000u, big[2] = b << 16, big[3] = b & 0xffff0000u;
+}
+template <int N>
+__device__ __forceinline__ void cols_big(const Row4<float> (&r)[N], uint32_t (&big)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = col + i < cols ? to_f32(row[col + i]) : 0.f;
+  for (int c = 0; c < 4; ++c) {
+    big[c] = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) big[c] = max(big[c], r[i].w[c] & 0x7fffffffu);
+  }
+}
+
+// N rows of 4 columns: all loads before the first use. `whole`: every value is inside
+// the matrix and the accesses are aligned.
+template <typename T, bool WIDE, int N>
+__device__ __forceinline__ void load_rows(const QuantArgs& a, long long row0, int col, bool whole, Row4<T> (&r)[N]) {
+  const T* p = static_cast<const T*>(a.x) + row0 * a.ldx + col;
+  if (WIDE && whole) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i].load(p + i * a.ldx, true);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int k = 0; k < Row4<T>::kWords; ++k) r[i].w[k] = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (row0 + i < a.rows && col + k < a.cols) r[i].set(k, p[i * a.ldx + k]);
   }
 }
 
@@ -60,8 +102,32 @@ __device__ __forceinline__ void store_cols4(uint8_t* row, int col, int cols, uin
 }
 
 template <bool E5M2>
-__device__ __forceinline__ uint32_t quantize4(const float (&v)[4], float f) {
-  return pack_fp8x4<E5M2>(__fmul_rn(v[0], f), __fmul_rn(v[1], f), __fmul_rn(v[2], f), __fmul_rn(v[3], f));
+__device__ __forceinline__ uint32_t quantize4(float v0, float v1, float v2, float v3, float f) {
+  return pack_fp8x4<E5M2>(__fmul_rn(v0, f), __fmul_rn(v1, f), __fmul_rn(v2, f), __fmul_rn(v3, f));
+}
+
+// Quantises N rows of a warp, each with its own scale: one reduction per row, then the
+// N scales at once, one per lane.
+template <typename T, bool E5M2, int N>
+__device__ __forceinline__ void quantize_each_row(const QuantArgs& a, long long row0, int col, int kb, bool whole, const Row4<T> (&r)[N], int lane) {
+  uint32_t big = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, row_big(r[i]));
+    if (lane == i) big = m;
+  }
+  float f, s;
+  block_scale(big, a.most, &f, &s);
+  if (lane < N && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = s;
+  uint8_t* q = a.q + row0 * a.ldq;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w = quantize4<E5M2>(r[i].get(0), r[i].get(1), r[i].get(2), r[i].get(3), __shfl_sync(0xffffffffu, f, i));
+    if (whole)
+      *reinterpret_cast<uint32_t*>(q + i * a.ldq + col) = w;
+    else if (row0 + i < a.rows)
+      store_cols4(q + i * a.ldq, col, a.cols, w);
+  }
 }
 
 template <typename T, bool WIDE, bool E5M2>
@@ -70,53 +136,31 @@ __global__ void __launch_bounds__(128) quantize_rows(const QuantArgs a) {
   const long long groups = ((long long)a.rows + kRowsPerWarp - 1) / kRowsPerWarp;
   for (long long g = (long long)blockIdx.y * 4 + (threadIdx.x >> 5); g < groups; g += (long long)gridDim.y * 4) {
     const long long row0 = g * kRowsPerWarp;
-    float v[kRowsPerWarp][4];
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[r][i] = 0.f;
-      if (row0 + r < a.rows) load_cols4<T, WIDE>(static_cast<const T*>(a.x) + (row0 + r) * a.ldx, col, a.cols, v[r]);
-    }
-    float mine = 0.f;
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-      uint32_t big = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) big = max(big, abs_bits(v[r][i]));
-      float f, s;
-      block_scale(__reduce_max_sync(0xffffffffu, big), a.most, &f, &s);
-      if (lane == r) mine = s;
-      if (row0 + r < a.rows) store_cols4(a.q + (row0 + r) * a.ldq, col, a.cols, quantize4<E5M2>(v[r], f));
-    }
-    if (lane < kRowsPerWarp && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = mine;
+    const bool whole = row0 + kRowsPerWarp <= a.rows && (kb + 1) * kScaleBlock <= a.cols;
+    Row4<T> r[kRowsPerWarp];
+    load_rows<T, WIDE>(a, row0, col, whole, r);
+    quantize_each_row<T, E5M2>(a, row0, col, kb, whole, r, lane);
   }
 }
 
 template <typename T, bool WIDE, bool E5M2>
 __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
-  __shared__ uint32_t col_big[8][128];
-  __shared__ float col_factor[128];
+  __shared__ __align__(16) uint32_t col_big[8][128];
+  __shared__ __align__(16) float col_factor[128];
   __shared__ uint32_t tile_big[8];
   __shared__ __align__(16) uint8_t bytes[128 * 128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kb = blockIdx.x, col = kb * 128 + 4 * lane;
   const bool square = a.block_rows == 128;
-  const int row_tiles = (a.rows + 127) / 128;
+  const int row_tiles = (a.rows - 1) / 128 + 1;
   for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
-    const int row0 = rt * 128 + warp * 16;
-    float v[16][4];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[r][i] = 0.f;
-      if (row0 + r < a.rows) load_cols4<T, WIDE>(static_cast<const T*>(a.x) + (long long)(row0 + r) * a.ldx, col, a.cols, v[r]);
-    }
-    uint32_t cbig[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cbig[i] = max(cbig[i], abs_bits(v[r][i]));
+    const long long row0 = (long long)rt * 128 + warp * 16;
+    const bool whole = (rt + 1LL) * 128 <= a.rows && (kb + 1LL) * 128 <= a.cols;
+    Row4<T> r[16];
+    load_rows<T, WIDE>(a, row0, col, whole, r);
+    uint32_t cbig[4];
     float f = 0.f, s = 0.f;
+    if (square || a.qt) cols_big(r, cbig);
     if (square) {
       const uint32_t big = __reduce_max_sync(0xffffffffu, max(max(cbig[0], cbig[1]), max(cbig[2], cbig[3])));
       if (lane == 0) tile_big[warp] = big;
@@ -129,7 +173,18 @@ __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
         if (a.q) a.scale[kb * a.ld_scale + rt] = s;
         if (a.qt) a.scale_t[rt * a.ld_scale_t + kb] = s;
       }
-    } else if (a.qt) {
+      if (a.q) {
+        uint8_t* q = a.q + row0 * a.ldq;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t w = quantize4<E5M2>(r[i].get(0), r[i].get(1), r[i].get(2), r[i].get(3), f);
+          if (whole)
+            *reinterpret_cast<uint32_t*>(q + i * a.ldq + col) = w;
+          else if (row0 + i < a.rows)
+            store_cols4(q + i * a.ldq, col, a.cols, w);
+        }
+      }
+    } else {
       *reinterpret_cast<uint4*>(&col_big[warp][4 * lane]) = make_uint4(cbig[0], cbig[1], cbig[2], cbig[3]);
       __syncthreads();
       if (threadIdx.x < 128) {
@@ -141,40 +196,24 @@ __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
         col_factor[threadIdx.x] = cf;
         if (kb * 128 + threadIdx.x < a.cols) a.scale_t[rt * a.ld_scale_t + kb * 128 + threadIdx.x] = cs;
       }
-    }
-    if (a.q) {
-      float mine = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float rf = f;
-        if (!square) {
-          uint32_t big = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) big = max(big, abs_bits(v[r][i]));
-          block_scale(__reduce_max_sync(0xffffffffu, big), a.most, &rf, &s);
-          if (lane == r) mine = s;
-        }
-        if (row0 + r < a.rows) store_cols4(a.q + (long long)(row0 + r) * a.ldq, col, a.cols, quantize4<E5M2>(v[r], rf));
-      }
-      if (!square && lane < 16 && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = mine;
+      if (a.q) quantize_each_row<T, E5M2>(a, row0, col, kb, whole, r, lane);
     }
     if (a.qt) {
       __syncthreads();  // col_factor is written; the tile before has left `bytes`
+      const float4 cf = square ? make_float4(f, f, f, f) : *reinterpret_cast<const float4*>(&col_factor[4 * lane]);
+      const float cfs[4] = {cf.x, cf.y, cf.z, cf.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = 4 * lane + i;
-        const float cf = square ? f : col_factor[c];
         uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float u[4] = {v[4 * k][i], v[4 * k + 1][i], v[4 * k + 2][i], v[4 * k + 3][i]};
-          w[k] = quantize4<E5M2>(u, cf);
-        }
+        for (int k = 0; k < 4; ++k)
+          w[k] = quantize4<E5M2>(r[4 * k].get(i), r[4 * k + 1].get(i), r[4 * k + 2].get(i), r[4 * k + 3].get(i), cfs[i]);
         // 16-byte pieces of a row are permuted by its column group: 8 lanes, 8 banks
-        *reinterpret_cast<uint4*>(bytes + c * 128 + ((warp ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(bytes + (4 * lane + i) * 128 + ((warp ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       __syncthreads();
-      const int piece = threadIdx.x & 7, left = a.rows - rt * 128 - piece * 16;
+      const int piece = threadIdx.x & 7;
+      const long long left = a.rows - (long long)rt * 128 - piece * 16;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int c = k * 32 + (threadIdx.x >> 3), out = kb * 128 + c;

@@ -6,17 +6,21 @@
 //             dx = rstd (w - mean(w) - h mean(w h)),
 //             dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
 //
-// Both are bound by memory. A row is read once and stays in registers between the
-// statistics and the result (the variance is the mean square of the centred
-// values, not E x^2 - mean^2, which cancels); short rows belong to one warp
-// (shuffles only), longer ones to more threads, and rows beyond what 1024 threads
-// hold are read again from L2. All sums are fp32.
+// Both are bound by memory: 2 and 3 passes over the rows. A row is read once and stays
+// in registers between the statistics and the result (the variance is the mean square
+// of the centred values, not E x^2 - mean^2, which cancels). Rows belong to groups of
+// 32..512 threads, several groups to a block where rows are short.
 //
-// The column sums dgamma / dbeta of the backward pass are kept in the registers of
-// the threads that own the columns, across the rows of a block; every block writes
-// one partial row to the workspace and a second kernel (launched with programmatic
-// dependency) adds the partial rows in a fixed order, so results do not depend on
-// timing.
+// Where there are many 16-byte aligned rows, each group runs its own ring of row
+// buffers in shared memory, filled by bulk copies several rows ahead: the bytes in
+// flight do not depend on the registers left over. Few rows, or unaligned ones, are
+// loaded directly. Rows of more than 8192 values take two passes in the backward
+// direction: the row sums first, then slabs of columns that need no reduction.
+//
+// The column sums dgamma / dbeta are kept in the registers of the threads that own the
+// columns, across the rows of a block; every block writes one partial row to the
+// workspace and a second kernel (launched with programmatic dependency) adds the
+// partial rows in a fixed order, so results do not depend on timing. All sums are fp32.
 #include <algorithm>
 
 #include "ops_common.h"
@@ -34,94 +38,189 @@ struct LnArgs {
   long long ldx, ldy, lddy, lddx;
   float *mean, *rstd;
   float *dgamma, *dbeta;
-  float* part;  // backward: [parts][2][cols]
-  int parts;
+  float* part;    // backward: [parts][2][cols]
+  float4* stats;  // backward, long rows: [rows] mean, rstd and the two row sums
+  int parts, size, slots;
+  int* status;
 };
 
-constexpr int kWarpsPerBlock = 4;  // rows per block where a warp has a row
+constexpr int kWarpsPerBlock = 4;   // rows per block where a warp has a row (direct loads)
+constexpr int kRingThreads = 512;
+constexpr int kMaxSlots = 8;
 
-// The sum of `v` over the threads of a row: a warp, or the block with one barrier.
-// `red` holds one word per warp; the callers alternate between two buffers, so the
-// barrier of one reduction protects the other's words.
-template <bool WARP>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+// The sums of `v` over the threads of a row group; `red` holds one word per warp of
+// the block. One barrier: callers alternate between two arrays, so that the barrier
+// of one reduction protects the other's words.
+__device__ __forceinline__ float group_sum(float v, float* red, int size, int group) {
   v = warp_sum(v);
-  if (WARP) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
-  return warp_sum(lane < nw ? red[lane] : 0.f);
+  if (size == 32) return v;
+  const int lane = threadIdx.x & 31, nw = size >> 5;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  named_barrier_sync(1 + group, size);
+  return warp_sum(lane < nw ? red[group * nw + lane] : 0.f);
 }
-__device__ __forceinline__ float2 row_sum2(float2 v, float2* red) {
+__device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int size, int group) {
   v.x = warp_sum(v.x), v.y = warp_sum(v.y);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
-  const float2 r = lane < nw ? red[lane] : make_float2(0.f, 0.f);
+  if (size == 32) return v;
+  const int lane = threadIdx.x & 31, nw = size >> 5;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  named_barrier_sync(1 + group, size);
+  const float2 r = lane < nw ? red[group * nw + lane] : make_float2(0.f, 0.f);
   return make_float2(warp_sum(r.x), warp_sum(r.y));
 }
 
+// VEC parameters at col (whole vectors: a row's columns are a multiple of VEC).
 template <typename P, int VEC>
-__device__ __forceinline__ void load_param(const void* base, int col, int valid, float other, float (&v)[VEC]) {
-  if (base == nullptr) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = i < valid ? other : 0.f;
-    return;
-  }
+__device__ __forceinline__ void load_param(const void* base, int col, bool in, float other, float (&v)[VEC]) {
   Raw<P, VEC> r;
-  r.load(static_cast<const P*>(base) + col, valid);
+  r.load(static_cast<const P*>(base) + col, in && base != nullptr);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = r.get(i);
+  for (int i = 0; i < VEC; ++i) v[i] = base != nullptr ? r.get(i) : in ? other : 0.f;
 }
 
-template <typename T, typename P, int VEC, int K, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) ln_forward(const LnArgs a) {
+// ---------------------------------------------------------------- forward
+// Statistics of a row that a group holds as K vectors per thread.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ float2 row_stats(const Raw<T, VEC> (&raw)[K], const LnArgs& a, int tid, int size, int group, float (*red)[32]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum += raw[k].get(i);
+  const float mean = group_sum(sum, red[0], size, group) * a.inv_cols;
+  float sq = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if ((k * size + tid) * VEC < a.cols) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float d = raw[k].get(i) - mean;
+        sq = fmaf(d, d, sq);
+      }
+    }
+  }
+  return make_float2(mean, 1.f / sqrtf(group_sum(sq, red[1], size, group) * a.inv_cols + a.eps));
+}
+
+__device__ __forceinline__ void put_stats(const LnArgs& a, long long row, float2 st) {
+  if (a.mean) a.mean[row] = st.x;
+  if (a.rstd) a.rstd[row] = st.y;
+}
+
+template <typename T, typename P, int VEC, int K>
+__global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
   __shared__ float red[2][32];
-  const int size = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
-  const long long first = WARP ? (long long)blockIdx.x * kWarpsPerBlock + (threadIdx.x >> 5) : blockIdx.x;
-  const long long step = WARP ? (long long)gridDim.x * kWarpsPerBlock : gridDim.x;
-  for (long long row = first; row < a.rows; row += step) {
+  const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     Raw<T, VEC> raw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int col = (k * size + tid) * VEC;
-      raw[k].load(x + col, a.cols - col);
+      raw[k].load(x + col, col < a.cols);
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += raw[k].get(i);
-    const float mean = row_sum<WARP>(sum, red[0]) * a.inv_cols;
-    float sq = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int valid = a.cols - (k * size + tid) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = i < valid ? raw[k].get(i) - mean : 0.f;
-        sq = fmaf(d, d, sq);
-      }
-    }
-    const float rstd = 1.f / sqrtf(row_sum<WARP>(sq, red[1]) * a.inv_cols + a.eps);
-    if (tid == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
-    }
+    const float2 st = row_stats<T, VEC, K>(raw, a, tid, size, group, red);
+    if (tid == 0) put_stats(a, row, st);
     T* y = static_cast<T*>(a.y) + row * a.ldy;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC, valid = a.cols - col;
-      if (valid <= 0) continue;
+      const int col = (k * size + tid) * VEC;
+      if (col >= a.cols) continue;
       float g[VEC], b[VEC], out[VEC];
-      load_param<P, VEC>(a.gamma, col, valid, 1.f, g);
-      load_param<P, VEC>(a.beta, col, valid, 0.f, b);
+      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
+      load_param<P, VEC>(a.beta, col, true, 0.f, b);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = fmaf((raw[k].get(i) - mean) * rstd, g[i], b[i]);
-      store_vec<T, VEC>(y + col, out, valid);
+      for (int i = 0; i < VEC; ++i) out[i] = fmaf((raw[k].get(i) - st.x) * st.y, g[i], b[i]);
+      store_vec<T, VEC>(y + col, out);
     }
   }
+}
+
+// One ring of row buffers per group.
+struct Ring {
+  uint8_t* buf;     // [slots][bytes]
+  uint64_t* full;   // [slots]
+  uint32_t bytes;
+  int slots, slot;
+  uint32_t phase;
+  bool dead;        // a wait ran out: go on without waiting (the results are not valid)
+
+  __device__ __forceinline__ void wait(int* status) {
+    if (!dead) dead = !wait_phase(&full[slot], phase, status);
+  }
+  __device__ __forceinline__ const uint8_t* at() const { return buf + slot * bytes; }
+  __device__ __forceinline__ void next() {
+    if (++slot == slots) slot = 0, phase ^= 1;
+  }
+  // no copy is in flight when the block exits, not even after a timeout
+  __device__ __forceinline__ void drain(long long filled) {
+    if (!dead) return;
+    for (long long f = filled > slots ? filled - slots : 0; f < filled; ++f) try_phase(&full[f % slots], (f / slots) & 1);
+  }
+};
+
+__device__ __forceinline__ Ring make_ring(uint8_t* smem, uint64_t (*full)[kMaxSlots], const LnArgs& a, int groups, int group, uint32_t bytes) {
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < groups; ++g)
+      for (int i = 0; i < a.slots; ++i) mbar_init(&full[g][i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  return Ring{smem + (size_t)group * a.slots * bytes, full[group], bytes, a.slots, 0, 0, false};
+}
+
+template <typename T, typename P, int VEC, int K>
+__global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_forward_ring(const LnArgs a) {
+  extern __shared__ __align__(128) uint8_t ring_smem[];
+  __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
+  __shared__ float red[2][32];
+  const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
+  const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
+  Ring ring = make_ring(ring_smem, full, a, groups, group, bytes);
+  const T* x = static_cast<const T*>(a.x);
+  long long fill = first;  // the next row to copy
+  auto copy = [&](int slot) {
+    mbar_arrive_expect_tx(&ring.full[slot], bytes);
+    bulk_load(ring.buf + slot * bytes, x + fill * a.ldx, bytes, &ring.full[slot]);
+  };
+  for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
+    if (tid == 0) copy(i);
+  float g[K][VEC], b[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int col = (k * size + tid) * VEC;
+    load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, g[k]);
+    load_param<P, VEC>(a.beta, col, col < a.cols, 0.f, b[k]);
+  }
+  for (long long row = first; row < a.rows; row += step) {
+    ring.wait(a.status);
+    Raw<T, VEC> raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * size + tid) * VEC;
+      raw[k].load(reinterpret_cast<const T*>(ring.at()) + col, col < a.cols);
+    }
+    const float2 st = row_stats<T, VEC, K>(raw, a, tid, size, group, red);
+    // the reductions are behind every thread's reads of the buffer
+    if (fill < a.rows) {
+      if (tid == 0) copy(ring.slot);
+      fill += step;
+    }
+    ring.next();
+    if (tid == 0) put_stats(a, row, st);
+    T* y = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * size + tid) * VEC;
+      if (col >= a.cols) continue;
+      float out[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[i] = fmaf((raw[k].get(i) - st.x) * st.y, g[k][i], b[k][i]);
+      store_vec<T, VEC>(y + col, out);
+    }
+  }
+  if (tid == 0) ring.drain((fill - first) / step);
 }
 
 // Rows longer than a block's registers: a block per row that reads it three times
@@ -135,69 +234,123 @@ __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
     float sum = 0.f;
     for (int col = begin; col < a.cols; col += step) {
       Raw<T, VEC> r;
-      r.load(x + col, a.cols - col);
+      r.load(x + col, true);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum += r.get(i);
     }
-    const float mean = row_sum<false>(sum, red[0]) * a.inv_cols;
+    const float mean = group_sum(sum, red[0], blockDim.x, 0) * a.inv_cols;
     float sq = 0.f;
     for (int col = begin; col < a.cols; col += step) {
       Raw<T, VEC> r;
-      r.load(x + col, a.cols - col);
+      r.load(x + col, true);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float d = col + i < a.cols ? r.get(i) - mean : 0.f;
+        const float d = r.get(i) - mean;
         sq = fmaf(d, d, sq);
       }
     }
-    const float rstd = 1.f / sqrtf(row_sum<false>(sq, red[1]) * a.inv_cols + a.eps);
-    if (threadIdx.x == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
-    }
+    const float rstd = 1.f / sqrtf(group_sum(sq, red[1], blockDim.x, 0) * a.inv_cols + a.eps);
+    if (threadIdx.x == 0) put_stats(a, row, make_float2(mean, rstd));
     T* y = static_cast<T*>(a.y) + row * a.ldy;
     for (int col = begin; col < a.cols; col += step) {
-      const int valid = a.cols - col;
       Raw<T, VEC> r;
-      r.load(x + col, valid);
+      r.load(x + col, true);
       float g[VEC], b[VEC], out[VEC];
-      load_param<P, VEC>(a.gamma, col, valid, 1.f, g);
-      load_param<P, VEC>(a.beta, col, valid, 0.f, b);
+      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
+      load_param<P, VEC>(a.beta, col, true, 0.f, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) out[i] = fmaf((r.get(i) - mean) * rstd, g[i], b[i]);
-      store_vec<T, VEC>(y + col, out, valid);
+      store_vec<T, VEC>(y + col, out);
     }
   }
 }
 
-// A row belongs to a group of 32..1024 threads, and a block holds several groups
-// where rows are short: enough loads are in flight with few blocks, and so few
-// partial rows. The next row's loads are issued before the reduction of this one.
+// ---------------------------------------------------------------- backward
+// A thread's columns across the rows of its group.
 template <typename T, typename P, int VEC, int K>
-__global__ void __launch_bounds__(K * VEC * int(sizeof(T)) <= 16 ? 1024 : 512) ln_backward(const LnArgs a, const int size) {
-  __shared__ float2 red[2][32];
-  extern __shared__ float col_sums[];  // [2][cols] when the block has several groups
-  const int groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
-  const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
-  const int lane = threadIdx.x & 31, warp0 = group * (size >> 5), warps = size >> 5;
+struct Columns {
   float gamma[K][VEC], dg[K][VEC], db[K][VEC];
+
+  __device__ __forceinline__ void init(const LnArgs& a, int tid, int size) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (k * size + tid) * VEC;
-    load_param<P, VEC>(a.gamma, col, a.cols - col, 1.f, gamma[k]);
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * size + tid) * VEC;
+      load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, gamma[k]);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dg[k][i] = db[k][i] = 0.f;
+      for (int i = 0; i < VEC; ++i) dg[k][i] = db[k][i] = 0.f;
+    }
   }
+  // Adds a row and returns its sums of w and w h. Beyond the row's end dy and gamma
+  // are zero, and so is what they add.
+  __device__ __forceinline__ float2 add(const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], float mean, float rstd) {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float dy = ry[k].get(i), h = (rx[k].get(i) - mean) * rstd, w = dy * gamma[k][i];
+        dg[k][i] = fmaf(dy, h, dg[k][i]);
+        db[k][i] += dy;
+        s.x += w;
+        s.y = fmaf(w, h, s.y);
+      }
+    return s;
+  }
+  // dx = rstd (w - c1 - h c2)
+  __device__ __forceinline__ void write(const LnArgs& a, const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], long long row, float mean,
+                                        float rstd, float c1, float c2, int tid, int size, int col0 = 0) {
+    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+    const float r1 = -rstd * c1, r2 = -rstd * c2 * rstd;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = col0 + (k * size + tid) * VEC;
+      if (col >= a.cols) continue;
+      float out[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[i] = fmaf(ry[k].get(i) * gamma[k][i], rstd, fmaf(rx[k].get(i) - mean, r2, r1));
+      store_vec<T, VEC>(dx + col, out);
+    }
+  }
+  // The block's partial row: its groups' column sums, added in group order.
+  __device__ __forceinline__ void finish(const LnArgs& a, int tid, int size, int group, int groups, float* sums) {
+    float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
+    for (int g = 0; g < groups; ++g) {
+      if (group == g) {
+        float* to = g == groups - 1 ? part : sums;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int col = (k * size + tid) * VEC + i;
+            if (col >= a.cols) continue;
+            to[col] = dg[k][i] + (g == 0 ? 0.f : sums[col]);
+            to[a.cols + col] = db[k][i] + (g == 0 ? 0.f : sums[a.cols + col]);
+          }
+      }
+      __syncthreads();
+    }
+  }
+};
+
+// Direct loads; the next row's are issued before this row's reduction.
+template <typename T, typename P, int VEC, int K>
+__global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
+  __shared__ float2 red[2][32];
+  extern __shared__ __align__(128) uint8_t ring_smem[];
+  const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
+  Columns<T, P, VEC, K> c;
+  c.init(a, tid, size);
   Raw<T, VEC> rx[K], ry[K], nx[K], ny[K];
-  float mean = 0.f, rstd = 0.f, next_mean = 0.f, next_rstd = 0.f;
+  float next_mean = 0.f, next_rstd = 0.f;
   auto fetch = [&](long long row) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int col = (k * size + tid) * VEC;
-      nx[k].load(x + col, a.cols - col);
-      ny[k].load(dy + col, a.cols - col);
+      nx[k].load(x + col, col < a.cols);
+      ny[k].load(dy + col, col < a.cols);
     }
     next_mean = a.mean[row], next_rstd = a.rstd[row];
   };
@@ -206,88 +359,80 @@ __global__ void __launch_bounds__(K * VEC * int(sizeof(T)) <= 16 ? 1024 : 512) l
   for (long long row = first; row < a.rows; row += step, flip ^= 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
-    mean = next_mean, rstd = next_rstd;
+    const float mean = next_mean, rstd = next_rstd;
     if (row + step < a.rows) fetch(row + step);
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        // beyond the row's end dy and gamma are zero, and so is what they add
-        const float dy = ry[k].get(i), h = (rx[k].get(i) - mean) * rstd, w = dy * gamma[k][i];
-        dg[k][i] = fmaf(dy, h, dg[k][i]);
-        db[k][i] += dy;
-        s.x += w;
-        s.y = fmaf(w, h, s.y);
-      }
-    s.x = warp_sum(s.x), s.y = warp_sum(s.y);
-    if (warps > 1) {
-      if (lane == 0) red[flip][threadIdx.x >> 5] = s;
-      named_barrier_sync(1 + group, size);
-      s = lane < warps ? red[flip][warp0 + lane] : make_float2(0.f, 0.f);
-      s.x = warp_sum(s.x), s.y = warp_sum(s.y);
-    }
-    const float c1 = s.x * a.inv_cols, c2 = s.y * a.inv_cols;
-    if (a.dx) {
-      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int col = (k * size + tid) * VEC, valid = a.cols - col;
-        if (valid <= 0) continue;
-        float out[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float h = (rx[k].get(i) - mean) * rstd;
-          out[i] = rstd * (ry[k].get(i) * gamma[k][i] - c1 - h * c2);
-        }
-        store_vec<T, VEC>(dx + col, out, valid);
-      }
-    }
+    const float2 s = group_sum2(c.add(rx, ry, mean, rstd), red[flip], size, group);
+    if (a.dx) c.write(a, rx, ry, row, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols, tid, size);
   }
   grid_dependents_launch();
-  // the groups' column sums, added in group order
-  float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
-  for (int g = 0; g < groups; ++g) {
-    if (group == g) {
-      const bool last = g == groups - 1;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int col = (k * size + tid) * VEC + i;
-          if (col >= a.cols) continue;
-          const float2 before = g == 0 ? make_float2(0.f, 0.f) : make_float2(col_sums[col], col_sums[a.cols + col]);
-          float* to = last ? part : col_sums;
-          to[col] = before.x + dg[k][i];
-          to[a.cols + col] = before.y + db[k][i];
-        }
-    }
-    __syncthreads();
-  }
+  c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
 }
 
-// Rows longer than a block's registers: x and dy are read twice (the second time
-// from L2) and the column sums live in this block's partial row of the workspace.
-template <typename T, typename P, int VEC>
-__global__ void __launch_bounds__(1024) ln_backward_long(const LnArgs a) {
+template <typename T, typename P, int VEC, int K>
+__global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_backward_ring(const LnArgs a) {
+  extern __shared__ __align__(128) uint8_t ring_smem[];
+  __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
   __shared__ float2 red[2][32];
-  const int step = blockDim.x * VEC, begin = threadIdx.x * VEC;
-  float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
+  const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
+  const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
+  Ring ring = make_ring(ring_smem, full, a, groups, group, 2 * bytes);
+  const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+  long long fill = first;
+  auto copy = [&](int slot) {
+    mbar_arrive_expect_tx(&ring.full[slot], 2 * bytes);
+    bulk_load(ring.buf + slot * 2 * bytes, x + fill * a.ldx, bytes, &ring.full[slot]);
+    bulk_load(ring.buf + slot * 2 * bytes + bytes, dy + fill * a.lddy, bytes, &ring.full[slot]);
+  };
+  for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
+    if (tid == 0) copy(i);
+  Columns<T, P, VEC, K> c;
+  c.init(a, tid, size);
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (first < a.rows) next_mean = a.mean[first], next_rstd = a.rstd[first];
   int flip = 0;
-  bool fresh = true;
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1, fresh = false) {
+  for (long long row = first; row < a.rows; row += step, flip ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < a.rows) next_mean = a.mean[row + step], next_rstd = a.rstd[row + step];
+    ring.wait(a.status);
+    Raw<T, VEC> rx[K], ry[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int col = (k * size + tid) * VEC;
+      rx[k].load(reinterpret_cast<const T*>(ring.at()) + col, col < a.cols);
+      ry[k].load(reinterpret_cast<const T*>(ring.at() + bytes) + col, col < a.cols);
+    }
+    const float2 s = group_sum2(c.add(rx, ry, mean, rstd), red[flip], size, group);
+    if (fill < a.rows) {
+      if (tid == 0) copy(ring.slot);
+      fill += step;
+    }
+    ring.next();
+    if (a.dx) c.write(a, rx, ry, row, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols, tid, size);
+  }
+  if (tid == 0) ring.drain((fill - first) / step);
+  grid_dependents_launch();
+  __syncthreads();  // the buffers are free: they take the groups' sums
+  c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
+}
+
+// Long rows, first pass: a block per row, its mean, rstd and two sums to `stats`.
+template <typename T, typename P, int VEC>
+__global__ void __launch_bounds__(1024) ln_row_sums(const LnArgs a) {
+  __shared__ float2 red[2][32];
+  int flip = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    const T* dyp = static_cast<const T*>(a.dy) + row * a.lddy;
-    T* dx = a.dx ? static_cast<T*>(a.dx) + row * a.lddx : nullptr;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float2 s = make_float2(0.f, 0.f);
-    for (int col = begin; col < a.cols; col += step) {
-      const int valid = a.cols - col;
+#pragma unroll 2
+    for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
       Raw<T, VEC> rx, ry;
-      rx.load(x + col, valid);
-      ry.load(dyp + col, valid);
+      rx.load(x + col, true);
+      ry.load(dy + col, true);
       float g[VEC];
-      load_param<P, VEC>(a.gamma, col, valid, 1.f, g);
+      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float w = ry.get(i) * g[i];
@@ -295,28 +440,44 @@ __global__ void __launch_bounds__(1024) ln_backward_long(const LnArgs a) {
         s.y = fmaf(w, (rx.get(i) - mean) * rstd, s.y);
       }
     }
-    s = row_sum2(s, red[flip]);
-    const float c1 = s.x * a.inv_cols, c2 = s.y * a.inv_cols;
-    for (int col = begin; col < a.cols; col += step) {
-      const int valid = a.cols - col;
-      Raw<T, VEC> rx, ry;
-      rx.load(x + col, valid);
-      ry.load(dyp + col, valid);
-      float g[VEC], out[VEC];
-      load_param<P, VEC>(a.gamma, col, valid, 1.f, g);
+    s = group_sum2(s, red[flip], 1024, 0);
+    if (threadIdx.x == 0) a.stats[row] = make_float4(mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+  }
+}
+
+// Long rows, second pass: blockIdx.y is a slab of columns, blockIdx.x a part of the
+// rows; the row sums are known, so threads own their columns without a reduction.
+constexpr int kSlabThreads = 256, kSlabRows = 4;
+template <typename T, typename P, int VEC>
+__global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
+  const int col0 = blockIdx.y * kSlabThreads * VEC, col = col0 + threadIdx.x * VEC;
+  const bool in = col < a.cols;
+  Columns<T, P, VEC, 1> c;
+  load_param<P, VEC>(a.gamma, col, in, 1.f, c.gamma[0]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float dy = ry.get(i), h = (rx.get(i) - mean) * rstd;
-        out[i] = rstd * (dy * g[i] - c1 - h * c2);
-        if (i < valid) {
-          part[col + i] = fresh ? dy * h : fmaf(dy, h, part[col + i]);
-          part[a.cols + col + i] = fresh ? dy : part[a.cols + col + i] + dy;
-        }
-      }
-      if (dx) store_vec<T, VEC>(dx + col, out, valid);
+  for (int i = 0; i < VEC; ++i) c.dg[0][i] = c.db[0][i] = 0.f;
+  for (long long row0 = (long long)blockIdx.x * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.x * kSlabRows) {
+    Raw<T, VEC> rx[kSlabRows][1], ry[kSlabRows][1];
+    float4 st[kSlabRows];
+#pragma unroll
+    for (int r = 0; r < kSlabRows; ++r) {
+      const long long row = row0 + r;
+      const bool here = row < a.rows;
+      rx[r][0].load(static_cast<const T*>(a.x) + row * a.ldx + col, in && here);
+      ry[r][0].load(static_cast<const T*>(a.dy) + row * a.lddy + col, in && here);
+      st[r] = here ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int r = 0; r < kSlabRows; ++r) {
+      if (row0 + r >= a.rows) break;
+      c.add(rx[r], ry[r], st[r].x, st[r].y);
+      if (a.dx) c.write(a, rx[r], ry[r], row0 + r, st[r].x, st[r].y, st[r].z, st[r].w, threadIdx.x, kSlabThreads, col0);
     }
   }
-  grid_dependents_launch();
+  if (!in) return;
+  float* part = a.part + (long long)blockIdx.x * 2 * a.cols + col;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) part[i] = c.dg[0][i], part[a.cols + i] = c.db[0][i];
 }
 
 // dgamma / dbeta = the partial rows added in order: 32 columns per block, the
@@ -347,99 +508,140 @@ __global__ void __launch_bounds__(1024) ln_column_sums(const float* part, int pa
 // ---------------------------------------------------------------- host side
 struct LnPlan {
   int vec;      // elements per access: 16 bytes of the row's type, or 1
-  int k;        // vectors per thread; 0: the long-row kernel
+  int k;        // vectors per thread; 0: the long-row kernels
   int size;     // threads per row
   int threads;  // per block
+  bool ring;    // rows through shared memory
+  int slots;    // row buffers per group
+  size_t smem;
 };
 
-// 16-byte accesses need every row of every tensor to start on a 16-byte boundary;
-// other rows go element by element.
+constexpr int kHeld = 8192;  // values of a row that the backward kernels hold at once
+
+// 16-byte accesses need every row of every tensor to start on a 16-byte boundary and
+// to end on one; other rows go element by element.
 LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   const int es = d.dtype == PKT_DTYPE_BF16 ? 2 : 4;
   auto rows_ok = [&](const void* p, long long ld) { return aligned_to(p, 16) && ld * es % 16 == 0; };
-  bool wide = rows_ok(d.x, d.ldx) && aligned_to(d.gamma, 16);
+  bool wide = (long long)d.cols * es % 16 == 0 && rows_ok(d.x, d.ldx) && aligned_to(d.gamma, 16);
   if (backward)
     wide = wide && rows_ok(d.dy, d.lddy) && (!d.dx || rows_ok(d.dx, d.lddx));
   else
     wide = wide && rows_ok(d.y, d.ldy) && aligned_to(d.beta, 16);
-  LnPlan p;
+  LnPlan p{};
   p.vec = wide ? 16 / es : 1;
-  const int nvec = (d.cols - 1) / p.vec + 1;
-  auto threads_for = [&](int k) {
+  const int nvec = d.cols / p.vec;
+  auto threads_for = [&](int k, int most) {
     int t = 32;
-    while (t < 1024 && (long long)t * k < nvec) t *= 2;
+    while (t < most && (long long)t * k < nvec) t *= 2;
     return t;
   };
-  if (!backward) {
-    // few rows: as many threads as the row has vectors; many rows: up to 4 vectors
-    // (8 single elements) each
-    const int ks[4] = {1, 2, wide ? 4 : 8, wide ? 4 : 16};
-    int i = d.rows >= 2LL * sms ? 2 : 0;
-    while (i > 0 && threads_for(ks[i - 1]) == threads_for(ks[i])) --i;
-    while (i < 3 && (long long)threads_for(ks[i]) * ks[i] < nvec) ++i;
-    p.k = ks[i];
-    p.size = threads_for(p.k);
-    p.threads = p.size > 32 ? p.size : 32 * kWarpsPerBlock;
-  } else {
-    // a block has 512 threads, or the 1024 of one row when 16 bytes per thread and
-    // tensor do (the kernel's register bound)
-    const int ks[3] = {wide ? 1 : 4, wide ? 2 : 8, wide ? 16 / p.vec : 16};
-    int i = 0;
-    auto fits = [&](int k) {
-      const int most = k * p.vec * es <= 16 ? 1024 : 512;
-      return threads_for(k) <= most && (long long)threads_for(k) * k >= nvec;
-    };
-    while (i < 3 && !fits(ks[i])) ++i;
-    p.k = i < 3 ? ks[i] : 0;
-    p.size = i < 3 ? threads_for(p.k) : 1024;
-    p.threads = std::max(512, p.size);
+  auto choose = [&](const int* ks, int count, int most) {  // the fewest vectors per thread that fit
+    for (int i = 0; i < count; ++i) {
+      p.k = ks[i], p.size = threads_for(ks[i], most);
+      if ((long long)p.size * p.k >= nvec) return true;
+    }
+    p.k = 0, p.size = p.threads = 1024;
+    return false;
+  };
+  if (!wide) {
+    const int few[3] = {1, 8, 16}, many[2] = {8, 16};
+    const bool lots = d.rows >= 2LL * sms;
+    if (backward ? choose(many, 2, 512) : lots ? choose(many, 2, 1024) : choose(few, 3, 1024))
+      p.threads = backward ? 512 : std::max(p.size, 32 * kWarpsPerBlock);
+    if (backward && p.size < 512) p.smem = size_t(2) * d.cols * sizeof(float);
+    return p;
   }
-  if (p.k == 0 || (long long)p.size * p.k < nvec) p.k = 0, p.size = p.threads = 1024;
+  const int ks[3] = {1, 2, 16 / p.vec};
+  // the ring pays from a few rows per group on
+  if (choose(ks, 3, 512)) {
+    const long long groups = 2LL * sms * (kRingThreads / p.size);
+    const size_t stage = size_t(kRingThreads / p.size) * d.cols * es * (backward ? 2 : 1);
+    p.slots = int(std::min<size_t>(kMaxSlots, (backward && p.k * p.vec > 8 ? 200 * 1024 : 100 * 1024) / stage));
+    if (d.rows >= 2 * groups && p.slots >= 2) {
+      p.ring = true;
+      p.threads = kRingThreads;
+      p.smem = std::max(p.slots * stage, backward && p.size < kRingThreads ? size_t(2) * d.cols * sizeof(float) : size_t(0));
+      return p;
+    }
+  }
+  if (backward) {
+    if (choose(ks, 3, 512)) p.threads = 512, p.smem = p.size < 512 ? size_t(2) * d.cols * sizeof(float) : 0;
+  } else {
+    const int direct[3] = {1, 2, 4};
+    if (choose(direct, 3, 1024)) p.threads = std::max(p.size, 32 * kWarpsPerBlock);
+  }
   return p;
 }
 
-// Blocks of the backward pass, each with one partial row of column sums: two per SM.
-// (From the sizes alone: the workspace is asked for before the pointers are known.)
+// Blocks along the rows in the backward pass, each with one partial row of column
+// sums: two per SM. (From the sizes alone: the workspace is asked for before the
+// pointers are known.)
 int ln_parts(long long rows, int sms) { return int(std::max(1LL, std::min(rows, 2LL * sms))); }
+// The partial rows, then (long rows) 4 values per row.
+size_t ln_part_floats(const pkt_layernorm_desc* d, int sms) { return (size_t(ln_parts(d->rows, sms)) * 2 * d->cols + 3) / 4 * 4; }
+size_t ln_workspace(const pkt_layernorm_desc* d, int sms) {
+  return (ln_part_floats(d, sms) + (d->cols > kHeld ? size_t(d->rows) * 4 : 0)) * sizeof(float);
+}
+
+template <typename... KArgs>
+int ln_launch_ring(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, int blocks, cudaStream_t st) {
+  const int rc = op_shared_memory(reinterpret_cast<const void*>(kernel), done, dev, 200 * 1024);
+  if (rc) return rc;
+  const cudaError_t e = op_launch(kernel, dim3(blocks), dim3(p.threads), p.smem, st, false, a);
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
+}
 
 template <typename T, typename P, int VEC, int K>
-cudaError_t ln_run(const LnArgs& a, const LnPlan& p, bool backward, cudaStream_t st) {
-  if constexpr (K * VEC <= 16) if (backward) {
-    const size_t smem = p.threads > p.size ? size_t(2) * a.cols * sizeof(float) : 0;
-    return op_launch(ln_backward<T, P, VEC, K>, dim3(a.parts), dim3(p.threads), smem, st, false, a, p.size);
+int ln_run(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
+  constexpr bool kBackward = K * VEC <= 16;  // the combinations that ln_plan gives
+  if constexpr (VEC > 1 && kBackward) {
+    static std::atomic<uint64_t> done[2];
+    if (p.ring && backward) return ln_launch_ring(ln_backward_ring<T, P, VEC, K>, &done[0], dev, a, p, a.parts, st);
+    if (p.ring) return ln_launch_ring(ln_forward_ring<T, P, VEC, K>, &done[1], dev, a, p, (K * VEC <= 8 ? 2 : 1) * sms, st);
   }
-  if constexpr (VEC == 1 ? K != 4 : true) {
-  if (backward) return cudaErrorInvalidConfiguration;
-  if (p.size == 32)
-    return op_launch(ln_forward<T, P, VEC, K, true>, dim3(unsigned(std::min((a.rows - 1) / kWarpsPerBlock + 1, 1LL << 30))),
-                     dim3(p.threads), 0, st, false, a);
-  return op_launch(ln_forward<T, P, VEC, K, false>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(p.threads), 0, st, false, a);
+  cudaError_t e = cudaErrorInvalidConfiguration;
+  if constexpr (kBackward && !(VEC == 1 && K < 8)) {
+    if (backward) e = op_launch(ln_backward<T, P, VEC, K>, dim3(a.parts), dim3(p.threads), p.smem, st, false, a);
   }
-  return cudaErrorInvalidConfiguration;
+  if (!backward) {
+    const long long blocks = (a.rows - 1) / (p.threads / p.size) + 1;
+    e = op_launch(ln_forward<T, P, VEC, K>, dim3(unsigned(std::min(blocks, 1LL << 30))), dim3(p.threads), 0, st, false, a);
+  }
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
 }
 
 template <typename T, typename P, int VEC>
-cudaError_t ln_pick(const LnArgs& a, const LnPlan& p, bool backward, cudaStream_t st) {
-  if (p.k == 0) {
-    if (backward) return op_launch(ln_backward_long<T, P, VEC>, dim3(a.parts), dim3(1024), 0, st, false, a);
-    return op_launch(ln_forward_long<T, P, VEC>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(1024), 0, st, false, a);
-  }
+int ln_pick(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
   switch (p.k) {
-    case 1: return ln_run<T, P, VEC, 1>(a, p, backward, st);
-    case 2: return ln_run<T, P, VEC, 2>(a, p, backward, st);
-    case 4: return ln_run<T, P, VEC, 4>(a, p, backward, st);
-    case 8: if (VEC == 1) return ln_run<T, P, 1, 8>(a, p, backward, st); break;
-    case 16: if (VEC == 1) return ln_run<T, P, 1, 16>(a, p, backward, st); break;
+    case 0: {
+      if (!backward) {
+        const cudaError_t e = op_launch(ln_forward_long<T, P, VEC>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(1024), 0, st, false, a);
+        return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
+      }
+      const int slabs = (a.cols - 1) / (kSlabThreads * VEC) + 1;
+      const long long want = std::max(1LL, 8LL * sms / slabs);  // about 8 blocks of 256 threads per SM
+      const int rows = int(std::min<long long>({want, a.parts, (a.rows - 1) / kSlabRows + 1}));
+      cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(1024), 0, st, false, a);
+      if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(rows, slabs), dim3(kSlabThreads), 0, st, false, a);
+      return e == cudaSuccess ? rows : cuda_fail(e, "launch layer norm");
+    }
+    case 1: return ln_run<T, P, VEC, 1>(a, p, backward, dev, sms, st);
+    case 2: if constexpr (VEC > 1) return ln_run<T, P, VEC, 2>(a, p, backward, dev, sms, st); break;
+    case 4: if constexpr (VEC > 1) return ln_run<T, P, VEC, 4>(a, p, backward, dev, sms, st); break;
+    case 8: if constexpr (VEC == 1) return ln_run<T, P, 1, 8>(a, p, backward, dev, sms, st); break;
+    case 16: if constexpr (VEC == 1) return ln_run<T, P, 1, 16>(a, p, backward, dev, sms, st); break;
   }
-  return cudaErrorInvalidConfiguration;
+  return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
 }
 
+// PKT_OK, an error, or (backward, long rows) the number of partial rows written.
 template <typename T>
-cudaError_t ln_dispatch(const LnArgs& a, const LnPlan& p, int param_dtype, bool backward, cudaStream_t st) {
+int ln_dispatch(const LnArgs& a, const LnPlan& p, int param_dtype, bool backward, int dev, int sms, cudaStream_t st) {
   constexpr int W = 16 / int(sizeof(T));
   if (param_dtype == PKT_DTYPE_F32)
-    return p.vec > 1 ? ln_pick<T, float, W>(a, p, backward, st) : ln_pick<T, float, 1>(a, p, backward, st);
-  return p.vec > 1 ? ln_pick<T, bf16_t, W>(a, p, backward, st) : ln_pick<T, bf16_t, 1>(a, p, backward, st);
+    return p.vec > 1 ? ln_pick<T, float, W>(a, p, backward, dev, sms, st) : ln_pick<T, float, 1>(a, p, backward, dev, sms, st);
+  return p.vec > 1 ? ln_pick<T, bf16_t, W>(a, p, backward, dev, sms, st) : ln_pick<T, bf16_t, 1>(a, p, backward, dev, sms, st);
 }
 
 int ln_check_common(const pkt_layernorm_desc* d) {
@@ -463,10 +665,9 @@ int ln_check_param(const void* p, const char* what, int dtype) {
   return PKT_OK;
 }
 
-size_t ln_workspace(const pkt_layernorm_desc* d, int sms) { return size_t(ln_parts(d->rows, sms)) * 2 * d->cols * sizeof(float); }
-
-LnArgs ln_args(const pkt_layernorm_desc& d) {
+LnArgs ln_args(const pkt_layernorm_desc& d, const LnPlan& p, int* status) {
   LnArgs a{};
+  a.size = p.size, a.slots = p.slots, a.status = status;
   a.rows = d.rows, a.cols = d.cols, a.eps = d.eps, a.inv_cols = 1.f / float(d.cols);
   a.x = d.x, a.gamma = d.gamma, a.beta = d.beta, a.dy = d.dy, a.y = d.y, a.dx = d.dx;
   a.ldx = d.ldx, a.ldy = d.ldy, a.lddy = d.lddy, a.lddx = d.lddx;
@@ -481,7 +682,7 @@ extern "C" {
 
 int pkt_layernorm_forward(const pkt_layernorm_desc* d, void* stream) {
   using namespace pkb;
-  int dev = 0, sms = 0, rc;
+  int dev = 0, sms = 0, rc, *status = nullptr;
   if ((rc = ln_check_common(d))) return rc;
   if (!(d->eps >= 0.f)) return fail(PKT_ERR_ARGS, "layer norm eps must be >= 0");
   if (d->rows == 0) return PKT_OK;
@@ -489,16 +690,15 @@ int pkt_layernorm_forward(const pkt_layernorm_desc* d, void* stream) {
       (rc = ln_check_param(d->gamma, "gamma", d->param_dtype)) || (rc = ln_check_param(d->beta, "beta", d->param_dtype)) ||
       (rc = ln_check_param(d->mean, "mean", PKT_DTYPE_F32)) || (rc = ln_check_param(d->rstd, "rstd", PKT_DTYPE_F32)))
     return rc;
-  if ((rc = op_device(&dev, &sms)) || (rc = op_check_memory(d->x, "x", dev)) || (rc = op_check_memory(d->y, "y", dev)) ||
+  if ((rc = op_device(&dev, &sms, &status)) || (rc = op_check_memory(d->x, "x", dev)) || (rc = op_check_memory(d->y, "y", dev)) ||
       (rc = op_check_memory(d->gamma, "gamma", dev)) || (rc = op_check_memory(d->beta, "beta", dev)) ||
       (rc = op_check_memory(d->mean, "mean", dev)) || (rc = op_check_memory(d->rstd, "rstd", dev)))
     return rc;
   const LnPlan p = ln_plan(*d, false, sms);
-  const LnArgs a = ln_args(*d);
+  const LnArgs a = ln_args(*d, p, status);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, false, st)
-                                                   : ln_dispatch<float>(a, p, d->param_dtype, false, st);
-  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm forward");
+  return d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, false, dev, sms, st)
+                                    : ln_dispatch<float>(a, p, d->param_dtype, false, dev, sms, st);
 }
 
 int pkt_layernorm_backward_workspace(const pkt_layernorm_desc* d, size_t* bytes) {
@@ -512,7 +712,7 @@ int pkt_layernorm_backward_workspace(const pkt_layernorm_desc* d, size_t* bytes)
 
 int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
   using namespace pkb;
-  int dev = 0, sms = 0, rc;
+  int dev = 0, sms = 0, rc, *status = nullptr;
   if ((rc = ln_check_common(d)) || (rc = ln_check_param(d->dgamma, "dgamma", PKT_DTYPE_F32)) ||
       (rc = ln_check_param(d->dbeta, "dbeta", PKT_DTYPE_F32)))
     return rc;
@@ -522,10 +722,10 @@ int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
       return rc;
     if (!d->mean || !d->rstd) return fail(PKT_ERR_ARGS, "layer norm backward needs the forward pass's mean and rstd");
     if ((rc = ln_check_param(d->mean, "mean", PKT_DTYPE_F32)) || (rc = ln_check_param(d->rstd, "rstd", PKT_DTYPE_F32)) ||
-        (rc = ln_check_param(d->workspace, "workspace", PKT_DTYPE_F32)))
+        (rc = aligned_to(d->workspace, 16) ? PKT_OK : fail(PKT_ERR_ARGS, "workspace is not 16-byte aligned")))
       return rc;
   }
-  if ((rc = op_device(&dev, &sms)) || (rc = op_check_memory(d->dgamma, "dgamma", dev)) || (rc = op_check_memory(d->dbeta, "dbeta", dev)))
+  if ((rc = op_device(&dev, &sms, &status)) || (rc = op_check_memory(d->dgamma, "dgamma", dev)) || (rc = op_check_memory(d->dbeta, "dbeta", dev)))
     return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d->rows == 0) {  // no rows: the sums over them are zero
@@ -542,16 +742,18 @@ int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
       (rc = op_check_memory(d->gamma, "gamma", dev)) || (rc = op_check_memory(d->mean, "mean", dev)) ||
       (rc = op_check_memory(d->rstd, "rstd", dev)) || (rc = op_check_memory(d->workspace, "workspace", dev)))
     return rc;
-  LnArgs a = ln_args(*d);
+  const LnPlan p = ln_plan(*d, true, sms);
+  LnArgs a = ln_args(*d, p, status);
   a.parts = ln_parts(d->rows, sms);
   a.part = static_cast<float*>(d->workspace);
-  const LnPlan p = ln_plan(*d, true, sms);
-  cudaError_t e = d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, true, st)
-                                             : ln_dispatch<float>(a, p, d->param_dtype, true, st);
-  if (e != cudaSuccess) return cuda_fail(e, "launch layer norm backward");
+  a.stats = reinterpret_cast<float4*>(a.part + ln_part_floats(d, sms));
+  rc = d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, true, dev, sms, st)
+                                  : ln_dispatch<float>(a, p, d->param_dtype, true, dev, sms, st);
+  if (rc < 0) return rc;
+  if (rc > 0) a.parts = rc;
   if (d->dgamma || d->dbeta) {
-    e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part), a.parts, a.cols,
-                  d->dgamma, d->dbeta);
+    const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part),
+                                    a.parts, a.cols, d->dgamma, d->dbeta);
     if (e != cudaSuccess) return cuda_fail(e, "launch layer norm column sums");
   }
   return PKT_OK;

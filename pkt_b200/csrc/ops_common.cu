@@ -5,6 +5,18 @@
 
 namespace pkb {
 
+static __device__ int g_ops_status;
+
+namespace {
+// First calls may come inside a stream capture, where some queries are only allowed in
+// relaxed mode; none of them touches the captured stream.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 static void* driver_entry(const char* name) {
   void* p = nullptr;
   cudaDriverEntryPointQueryResult q;
@@ -18,21 +30,40 @@ EncodeTiled op_encode_tiled() {
   return fn;
 }
 
-int op_device(int* dev, int* sms) {
+int op_device(int* dev, int* sms, int** status) {
   static std::atomic<int> known[64];  // SM count of a device that passed, 0: not looked at
+  static int* words[64];
   cudaError_t e = cudaGetDevice(dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (*dev < 0 || *dev >= 64) return fail(PKT_ERR_ARGS, "device id out of range");
-  int n = known[*dev].load(std::memory_order_relaxed);
+  int n = known[*dev].load(std::memory_order_acquire);
   if (n == 0) {
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    RelaxedCapture relaxed;
     int major = 0;
+    void* word = nullptr;
     e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
     if (major != 10) return fail(PKT_ERR_UNSUPPORTED, "device %d is sm_%dx; this build targets sm_100a", *dev, major);
-    known[*dev].store(n, std::memory_order_relaxed);
+    e = cudaGetSymbolAddress(&word, g_ops_status);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetSymbolAddress");
+    words[*dev] = static_cast<int*>(word);
+    known[*dev].store(n, std::memory_order_release);
   }
   *sms = n;
+  if (status) *status = words[*dev];
+  return PKT_OK;
+}
+
+int op_shared_memory(const void* kernel, std::atomic<uint64_t>* done, int dev, int bytes) {
+  const uint64_t bit = uint64_t(1) << dev;
+  if (done->load(std::memory_order_acquire) & bit) return PKT_OK;
+  RelaxedCapture relaxed;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared memory)");
+  done->fetch_or(bit, std::memory_order_acq_rel);
   return PKT_OK;
 }
 
@@ -55,3 +86,14 @@ int op_check_memory(const void* p, const char* what, int dev) {
 }
 
 }  // namespace pkb
+
+extern "C" int pkt_ops_status(int* code) {
+  using namespace pkb;
+  if (!code) return fail(PKT_ERR_ARGS, "null argument");
+  int dev = 0, sms = 0, rc, *word = nullptr;
+  if ((rc = op_device(&dev, &sms, &word))) return rc;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(code, word, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && *code) e = cudaMemset(word, 0, sizeof(int));
+  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "read the operators' status");
+}

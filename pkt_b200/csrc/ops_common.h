@@ -5,6 +5,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "runtime_impl.h"
 
 namespace pkb {
@@ -14,8 +16,12 @@ constexpr int kScaleBlock = 128;  // values of one 8-bit block along the contigu
 // from there on, largest value / magnitude stays far from fp32 overflow.
 constexpr float kScaleTiny = 7.888609052210118e-31f;
 
-// The current device, checked once to be one this build runs on, and its SM count.
-int op_device(int* dev, int* sms);
+// The current device, checked once to be one this build runs on, its SM count and
+// (where asked for) the address of its status word, which a kernel sets when one of
+// its bounded waits runs out.
+int op_device(int* dev, int* sms, int** status = nullptr);
+// Raises a kernel's shared-memory limit, once per kernel and device.
+int op_shared_memory(const void* kernel, std::atomic<uint64_t>* done, int dev, int bytes);
 // `p` is memory of device `dev` (or managed memory), so that a host pointer or
 // another GPU's buffer is an error here and not a fault in the kernel. Null passes.
 int op_check_memory(const void* p, const char* what, int dev);

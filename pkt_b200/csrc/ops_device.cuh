@@ -27,28 +27,23 @@ struct Raw {
   static constexpr int kWords = (kBytes + 3) / 4;
   uint32_t w[kWords];
 
-  // Elements [0, valid) of p; the rest are zero. A whole vector is one aligned
-  // access when VEC > 1 (the callers' rule), a partial one element by element.
-  __device__ __forceinline__ void load(const T* p, int valid) {
-    if (VEC > 1 && valid >= VEC) {
-      if (kBytes >= 16) {
+  // One aligned access (the callers' rule), or zeros.
+  __device__ __forceinline__ void load(const T* p, bool in) {
 #pragma unroll
-        for (int i = 0; i < kWords / 4; ++i) {
-          const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-        }
-      } else if (kBytes == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[kWords - 1] = v.y;
-      } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    if (!in) return;
+    if constexpr (VEC == 1) {
+      set(0, *p);
+    } else if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
       }
     } else {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = 0;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i < valid) set(i, p[i]);
+      static_assert(kBytes == 8, "2, 4 or 8 words");
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
     }
   }
   __device__ __forceinline__ void set(int i, float v) { w[i * int(sizeof(T)) / 4] = __float_as_uint(v); }
@@ -59,26 +54,24 @@ struct Raw {
   }
 };
 
-// Stores v[0..valid) to p, as one aligned access per 16 bytes where whole.
+// Stores VEC values to p, as one aligned access per 16 bytes.
 template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC], int valid) {
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   constexpr int kBytes = VEC * int(sizeof(T));
-  if (VEC > 1 && valid >= VEC) {
-    uint32_t w[(kBytes + 3) / 4];
+  if constexpr (VEC == 1) {
+    from_f32(v[0], p);
+  } else {
+    uint32_t w[kBytes / 4];
 #pragma unroll
-    for (int i = 0; i < (kBytes + 3) / 4; ++i)
-      w[i] = sizeof(T) == 4 ? __float_as_uint(v[i < VEC ? i : 0]) : pack_bf16x2(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
-    if (kBytes >= 16) {
+    for (int i = 0; i < kBytes / 4; ++i)
+      w[i] = sizeof(T) == 4 ? __float_as_uint(v[i % VEC]) : pack_bf16x2(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
+    if constexpr (kBytes >= 16) {
 #pragma unroll
       for (int i = 0; i < kBytes / 16; ++i)
         reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[kBytes / 4 - 1]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (i < valid) from_f32(v[i], p + i);
   }
 }
 
@@ -86,6 +79,42 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
+}
+
+// ---------------------------------------------------------------- bulk copies and bounded waits
+// Waits until the phase of `parity` has completed; false when it has not after 2^21
+// tries of up to a microsecond each (about 2 s). One block of assembly: the
+// compiler's own form of the loop kept the lanes apart (BSSY / BSYNC around each
+// try) and cost hot loops a third of their instructions.
+__device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "AGAIN:\n"
+      " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, 1000;\n"
+      " @p bra DONE;\n"
+      " add.u32 n, n, 1;\n"
+      " setp.lt.u32 q, n, 0x200000;\n"
+      " @q bra AGAIN;\n"
+      "DONE:\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The same for a converged warp (one answer for all lanes); a timeout is recorded.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* status) {
+  if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
+  *reinterpret_cast<volatile int*>(status) = 2;  // PKT_DEV_TIMEOUT_PIPE
+  return false;
+}
+// `bytes` (a multiple of 16, both addresses 16-byte aligned) global -> shared,
+// counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -45,10 +45,10 @@ def fp8_gemm(desc, stream=None):
     check(_lib.load().pkt_fp8_gemm(desc, stream))
 
 
-def fp8_gemm_status():
-    """0, or the code of a wait that ran out in an fp8_gemm launch since the last call (synchronises)."""
+def ops_status():
+    """0, or the code of a wait that ran out in an operator's kernel since the last call (synchronises)."""
     code = ctypes.c_int()
-    check(_lib.load().pkt_fp8_gemm_status(ctypes.byref(code)))
+    check(_lib.load().pkt_ops_status(ctypes.byref(code)))
     return code.value
 
 

@@ -192,7 +192,7 @@ def product(pk, M, N, K, a="e4m3", b="e4m3", ab=1, bb=128, out="bf16", seed=0, p
                        b_block_rows=bb, out=C.data_ptr(), ldo=ldo, out_dtype=kind(pk, out))
     (run or pk.fp8_gemm)(d)
     torch.cuda.synchronize()
-    assert pk.fp8_gemm_status() == 0
+    assert pk.ops_status() == 0
     assert torch.all(C[:, N:] == 5.0) and torch.all(flat[M * ldo:] == 5.0)
     vals = []
     for x, s, rows, blk in ((A, sa, M, ab), (B, sb, N, bb)):

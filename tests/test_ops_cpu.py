@@ -97,7 +97,7 @@ def test_null_arguments():
     for f in ("pkt_layernorm_forward", "pkt_layernorm_backward", "pkt_fp8_quantize", "pkt_fp8_gemm"):
         assert getattr(L, f)(None, None) == _lib.PKT_ERR_ARGS
     assert L.pkt_layernorm_backward_workspace(ln(), None) == _lib.PKT_ERR_ARGS
-    assert L.pkt_fp8_gemm_status(None) == _lib.PKT_ERR_ARGS
+    assert L.pkt_ops_status(None) == _lib.PKT_ERR_ARGS
     assert L.pkt_adamw_create(0, None, None) == _lib.PKT_ERR_ARGS
     assert L.pkt_adamw_step(None, 1.0, 1.0, None, None) == _lib.PKT_ERR_ARGS
     assert L.pkt_adamw_set_grads(None, None, None) == _lib.PKT_ERR_ARGS
