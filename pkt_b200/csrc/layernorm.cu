@@ -22,6 +22,7 @@
 // workspace and a second kernel (launched with programmatic dependency) adds the
 // partial rows in a fixed order, so results do not depend on timing. All sums are fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "ops_common.h"
 #include "ops_device.cuh"
@@ -48,25 +49,29 @@ constexpr int kWarpsPerBlock = 4;   // rows per block where a warp has a row (di
 constexpr int kRingThreads = 512;
 constexpr int kMaxSlots = 8;
 
-// The sums of `v` over the threads of a row group; `red` holds one word per warp of
-// the block. One barrier: callers alternate between two arrays, so that the barrier
-// of one reduction protects the other's words.
-__device__ __forceinline__ float group_sum(float v, float* red, int size, int group) {
-  v = warp_sum(v);
-  if (size == 32) return v;
-  const int lane = threadIdx.x & 31, nw = size >> 5;
-  if (lane == 0) red[threadIdx.x >> 5] = v;
-  named_barrier_sync(1 + group, size);
-  return warp_sum(lane < nw ? red[group * nw + lane] : 0.f);
+// The sums of `v` over the threads of a row group (a power of two of warps); `red`
+// holds one word per warp of the block. One barrier: callers alternate between two
+// arrays, so that the barrier of one reduction protects the other's words.
+__device__ __forceinline__ float add_to(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 add_to(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ float shuffled(float v, int off) { return __shfl_xor_sync(0xffffffffu, v, off); }
+__device__ __forceinline__ float2 shuffled(float2 v, int off) { return make_float2(shuffled(v.x, off), shuffled(v.y, off)); }
+__device__ __forceinline__ float4 add_to(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+__device__ __forceinline__ float4 shuffled(float4 v, int off) {
+  return make_float4(shuffled(v.x, off), shuffled(v.y, off), shuffled(v.z, off), shuffled(v.w, off));
 }
-__device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int size, int group) {
-  v.x = warp_sum(v.x), v.y = warp_sum(v.y);
+
+template <typename V>
+__device__ __forceinline__ V group_sum(V v, V* red, int size, int group) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v = add_to(v, shuffled(v, off));
   if (size == 32) return v;
   const int lane = threadIdx.x & 31, nw = size >> 5;
   if (lane == 0) red[threadIdx.x >> 5] = v;
   named_barrier_sync(1 + group, size);
-  const float2 r = lane < nw ? red[group * nw + lane] : make_float2(0.f, 0.f);
-  return make_float2(warp_sum(r.x), warp_sum(r.y));
+  v = red[group * nw + (lane & (nw - 1))];
+  for (int off = nw >> 1; off >= 1; off >>= 1) v = add_to(v, shuffled(v, off));
+  return v;
 }
 
 // VEC parameters at col (whole vectors: a row's columns are a multiple of VEC).
@@ -169,15 +174,26 @@ __device__ __forceinline__ Ring make_ring(uint8_t* smem, uint64_t (*full)[kMaxSl
   return Ring{smem + (size_t)group * a.slots * bytes, full[group], bytes, a.slots, 0, 0, false};
 }
 
-template <typename T, typename P, int VEC, int K>
-__global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_forward_ring(const LnArgs a) {
+// Two rows at a time, so that their reductions overlap, up to 32 values of each per
+// thread in pairs, the parameters as fp32 in shared memory. The kernel was bound by its
+// instructions: 30 per value with 8 values per thread (the fixed work of a row is two
+// thirds of that), 19 with 16, 12 like this (8192 x 4096 bf16: 43, 33 and 27 us).
+// EXACT: the group's threads cover the row without a rest.
+template <typename T, typename P, int VEC, int K, bool EXACT>
+__global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
-  __shared__ float red[2][32];
+  __shared__ float2 red[2][32];
+  constexpr int H = VEC / 2;
   const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
-  Ring ring = make_ring(ring_smem, full, a, groups, group, bytes);
+  float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols]
+  for (int c = threadIdx.x; c < a.cols; c += kRingThreads) {
+    params[c] = a.gamma ? to_f32(static_cast<const P*>(a.gamma)[c]) : 1.f;
+    params[a.cols + c] = a.beta ? to_f32(static_cast<const P*>(a.beta)[c]) : 0.f;
+  }
+  Ring ring = make_ring(ring_smem + 8 * (size_t)a.cols, full, a, groups, group, bytes);
   const T* x = static_cast<const T*>(a.x);
   long long fill = first;  // the next row to copy
   auto copy = [&](int slot) {
@@ -186,41 +202,73 @@ __global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_forward
   };
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
     if (tid == 0) copy(i);
-  float g[K][VEC], b[K][VEC];
+  bool in[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int col = (k * size + tid) * VEC;
-    load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, g[k]);
-    load_param<P, VEC>(a.beta, col, col < a.cols, 0.f, b[k]);
-  }
-  for (long long row = first; row < a.rows; row += step) {
-    ring.wait(a.status);
-    Raw<T, VEC> raw[K];
+  for (int k = 0; k < K; ++k) in[k] = EXACT || (k * size + tid) * VEC < a.cols;
+  params += tid * VEC;
+  T* y = static_cast<T*>(a.y) + first * a.ldy + tid * VEC;
+  const long long next_y = step * a.ldy;
+  for (long long row = first; row < a.rows; row += 2 * step, y += 2 * next_y) {
+    const bool two = row + step < a.rows;
+    Raw<T, VEC> raw[2][K];
+    int slot[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {  // a missing second row is zeros
+      slot[r] = ring.slot;
+      if (r == 0 || two) ring.wait(a.status);
+      const T* from = reinterpret_cast<const T*>(ring.at()) + tid * VEC;
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[r][k].load(from + k * size * VEC, in[k] && (r == 0 || two));
+      if (r == 0 || two) ring.next();
+    }
+    uint64_t s0 = 0, s1 = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < H; ++i) s0 = add2(s0, raw[0][k].get2(i)), s1 = add2(s1, raw[1][k].get2(i));
+    const float2 sum = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[0], size, group);
+    const float2 mean = make_float2(sum.x * a.inv_cols, sum.y * a.inv_cols);
+    const uint64_t m0 = pair_of(-mean.x, -mean.x), m1 = pair_of(-mean.y, -mean.y);
+    s0 = s1 = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      raw[k].load(reinterpret_cast<const T*>(ring.at()) + col, col < a.cols);
+      if (!in[k]) continue;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const uint64_t d0 = add2(raw[0][k].get2(i), m0), d1 = add2(raw[1][k].get2(i), m1);
+        s0 = fma2(d0, d0, s0);
+        s1 = fma2(d1, d1, s1);
+      }
     }
-    const float2 st = row_stats<T, VEC, K>(raw, a, tid, size, group, red);
-    // the reductions are behind every thread's reads of the buffer
-    if (fill < a.rows) {
-      if (tid == 0) copy(ring.slot);
+    const float2 sq = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[1], size, group);
+    const float2 rstd = make_float2(1.f / sqrtf(sq.x * a.inv_cols + a.eps), 1.f / sqrtf(sq.y * a.inv_cols + a.eps));
+    // the reductions are behind every thread's reads of the buffers
+    if (tid == 0) {
+      if (fill < a.rows) copy(slot[0]);
       fill += step;
+      if (two && fill < a.rows) copy(slot[1]);
+      fill += step;
+      put_stats(a, row, make_float2(mean.x, rstd.x));
+      if (two) put_stats(a, row + step, make_float2(mean.y, rstd.y));
     }
-    ring.next();
-    if (tid == 0) put_stats(a, row, st);
-    T* y = static_cast<T*>(a.y) + row * a.ldy;
+    const uint64_t r0 = pair_of(rstd.x, rstd.x), r1 = pair_of(rstd.y, rstd.y);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      if (col >= a.cols) continue;
-      float out[VEC];
+      if (!in[k]) continue;
+      Raw<float, VEC> g, b;
+      g.load(params + k * size * VEC, true);
+      b.load(params + a.cols + k * size * VEC, true);
+      uint64_t out[H];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = fmaf((raw[k].get(i) - st.x) * st.y, g[k][i], b[k][i]);
-      store_vec<T, VEC>(y + col, out);
+      for (int i = 0; i < H; ++i) out[i] = fma2(mul2(add2(raw[0][k].get2(i), m0), r0), g.get2(i), b.get2(i));
+      store_pairs<T, VEC>(y + k * size * VEC, out);
+      if (!two) continue;
+#pragma unroll
+      for (int i = 0; i < H; ++i) out[i] = fma2(mul2(add2(raw[1][k].get2(i), m1), r1), g.get2(i), b.get2(i));
+      store_pairs<T, VEC>(y + next_y + k * size * VEC, out);
     }
   }
-  if (tid == 0) ring.drain((fill - first) / step);
+  if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
 }
 
 // Rows longer than a block's registers: a block per row that reads it three times
@@ -266,68 +314,105 @@ __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
 }
 
 // ---------------------------------------------------------------- backward
-// A thread's columns across the rows of its group.
+// A thread's columns across the rows of its group, in pairs where it has vectors.
 template <typename T, typename P, int VEC, int K>
 struct Columns {
-  float gamma[K][VEC], dg[K][VEC], db[K][VEC];
+  static constexpr int kPair = VEC > 1 ? 2 : 1, H = VEC / kPair;
+  using V = std::conditional_t<VEC == 1, float, uint64_t>;
+  V gamma[K][H], dg[K][H], db[K][H];
 
-  __device__ __forceinline__ void init(const LnArgs& a, int tid, int size) {
+  static __device__ __forceinline__ float both(float v, float) { return v; }
+  static __device__ __forceinline__ uint64_t both(float v, uint64_t) { return pair_of(v, v); }
+  static __device__ __forceinline__ float add(float a, float b) { return a + b; }
+  static __device__ __forceinline__ uint64_t add(uint64_t a, uint64_t b) { return add2(a, b); }
+  static __device__ __forceinline__ float mul(float a, float b) { return a * b; }
+  static __device__ __forceinline__ uint64_t mul(uint64_t a, uint64_t b) { return mul2(a, b); }
+  static __device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
+  static __device__ __forceinline__ uint64_t fma(uint64_t a, uint64_t b, uint64_t c) { return fma2(a, b, c); }
+  static __device__ __forceinline__ float total(float v) { return v; }
+  static __device__ __forceinline__ float total(uint64_t v) { return sum_of(v); }
+  static __device__ __forceinline__ V value(const Raw<T, VEC>& r, int i) {
+    if constexpr (VEC > 1)
+      return r.get2(i);
+    else
+      return r.get(0);
+  }
+
+  __device__ __forceinline__ void init(const LnArgs& a, int col0, int size) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, gamma[k]);
+      const int col = col0 + k * size * VEC;
+      float g[VEC];
+      load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) dg[k][i] = db[k][i] = 0.f;
+      for (int i = 0; i < H; ++i) {
+        if constexpr (VEC > 1)
+          gamma[k][i] = pair_of(g[2 * i], g[2 * i + 1]);
+        else
+          gamma[k][i] = g[0];
+        dg[k][i] = db[k][i] = V(0);
+      }
     }
   }
   // Adds a row and returns its sums of w and w h. Beyond the row's end dy and gamma
   // are zero, and so is what they add.
   __device__ __forceinline__ float2 add(const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], float mean, float rstd) {
-    float2 s = make_float2(0.f, 0.f);
+    V s1 = V(0), s2 = V(0);
+    const V m = both(-mean, V(0)), r = both(rstd, V(0));
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float dy = ry[k].get(i), h = (rx[k].get(i) - mean) * rstd, w = dy * gamma[k][i];
-        dg[k][i] = fmaf(dy, h, dg[k][i]);
-        db[k][i] += dy;
-        s.x += w;
-        s.y = fmaf(w, h, s.y);
+      for (int i = 0; i < H; ++i) {
+        const V dy = value(ry[k], i), h = mul(add(value(rx[k], i), m), r), w = mul(dy, gamma[k][i]);
+        dg[k][i] = fma(dy, h, dg[k][i]);
+        db[k][i] = add(db[k][i], dy);
+        s1 = add(s1, w);
+        s2 = fma(w, h, s2);
       }
-    return s;
+    return make_float2(total(s1), total(s2));
   }
-  // dx = rstd (w - c1 - h c2)
-  __device__ __forceinline__ void write(const LnArgs& a, const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], long long row, float mean,
-                                        float rstd, float c1, float c2, int tid, int size, int col0 = 0) {
-    T* dx = static_cast<T*>(a.dx) + row * a.lddx;
-    const float r1 = -rstd * c1, r2 = -rstd * c2 * rstd;
+  // dx = rstd (w - c1 - h c2); `dx`: this thread's first column of the row
+  __device__ __forceinline__ void write(const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], const bool (&in)[K], T* dx, int size, float mean,
+                                        float rstd, float c1, float c2) {
+    const V m = both(-mean, V(0)), r = both(rstd, V(0)), r1 = both(-rstd * c1, V(0)), r2 = both(-rstd * c2 * rstd, V(0));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int col = col0 + (k * size + tid) * VEC;
-      if (col >= a.cols) continue;
-      float out[VEC];
+      if (!in[k]) continue;
+      V out[H];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = fmaf(ry[k].get(i) * gamma[k][i], rstd, fmaf(rx[k].get(i) - mean, r2, r1));
-      store_vec<T, VEC>(dx + col, out);
+      for (int i = 0; i < H; ++i) out[i] = fma(mul(value(ry[k], i), gamma[k][i]), r, fma(add(value(rx[k], i), m), r2, r1));
+      if constexpr (VEC > 1)
+        store_pairs<T, VEC>(dx + k * size * VEC, out);
+      else
+        from_f32(out[0], dx + k * size);
     }
   }
-  // The block's partial row: its groups' column sums, added in group order.
+  // The block's partial row: its groups' column sums, added in group order. `sums`:
+  // shared memory, [groups][2 K VEC][size].
   __device__ __forceinline__ void finish(const LnArgs& a, int tid, int size, int group, int groups, float* sums) {
+    constexpr int kHalf = K * VEC;
     float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
-    for (int g = 0; g < groups; ++g) {
-      if (group == g) {
-        float* to = g == groups - 1 ? part : sums;
+    float* mine = sums + group * 2 * kHalf * size + tid;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const int col = (k * size + tid) * VEC + i;
-            if (col >= a.cols) continue;
-            to[col] = dg[k][i] + (g == 0 ? 0.f : sums[col]);
-            to[a.cols + col] = db[k][i] + (g == 0 ? 0.f : sums[a.cols + col]);
-          }
+      for (int i = 0; i < H; ++i) {
+        if constexpr (VEC > 1) {
+          const float2 g = unpair(dg[k][i]), b = unpair(db[k][i]);
+          mine[(k * VEC + 2 * i) * size] = g.x, mine[(k * VEC + 2 * i + 1) * size] = g.y;
+          mine[(kHalf + k * VEC + 2 * i) * size] = b.x, mine[(kHalf + k * VEC + 2 * i + 1) * size] = b.y;
+        } else {
+          mine[k * size] = dg[k][i], mine[(kHalf + k) * size] = db[k][i];
+        }
       }
-      __syncthreads();
+    __syncthreads();
+    const int shift = 31 - __clz(size);
+    for (int j = threadIdx.x; j < 2 * kHalf * size; j += blockDim.x) {
+      float t = sums[j];
+      for (int g = 1; g < groups; ++g) t += sums[g * 2 * kHalf * size + j];
+      const int v = j >> shift, which = v >= kHalf, u = which ? v - kHalf : v;
+      const int col = (u / VEC * size + (j & (size - 1))) * VEC + u % VEC;
+      if (col < a.cols) part[which * a.cols + col] = t;
     }
   }
 };
@@ -340,8 +425,11 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   Columns<T, P, VEC, K> c;
-  c.init(a, tid, size);
+  c.init(a, tid * VEC, size);
   Raw<T, VEC> rx[K], ry[K], nx[K], ny[K];
+  bool in[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) in[k] = (k * size + tid) * VEC < a.cols;
   float next_mean = 0.f, next_rstd = 0.f;
   auto fetch = [&](long long row) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -361,18 +449,19 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
     for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
     const float mean = next_mean, rstd = next_rstd;
     if (row + step < a.rows) fetch(row + step);
-    const float2 s = group_sum2(c.add(rx, ry, mean, rstd), red[flip], size, group);
-    if (a.dx) c.write(a, rx, ry, row, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols, tid, size);
+    const float2 s = group_sum(c.add(rx, ry, mean, rstd), red[flip], size, group);
+    if (a.dx)
+      c.write(rx, ry, in, static_cast<T*>(a.dx) + row * a.lddx + tid * VEC, size, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
   grid_dependents_launch();
   c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
 }
 
-template <typename T, typename P, int VEC, int K>
-__global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_backward_ring(const LnArgs a) {
+template <typename T, typename P, int VEC, int K, bool EXACT>
+__global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
-  __shared__ float2 red[2][32];
+  __shared__ float4 red[2][kRingThreads / 32];
   const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
@@ -387,28 +476,67 @@ __global__ void __launch_bounds__(kRingThreads, K * VEC <= 8 ? 2 : 1) ln_backwar
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
     if (tid == 0) copy(i);
   Columns<T, P, VEC, K> c;
-  c.init(a, tid, size);
-  float next_mean = 0.f, next_rstd = 0.f;
-  if (first < a.rows) next_mean = a.mean[first], next_rstd = a.rstd[first];
-  int flip = 0;
-  for (long long row = first; row < a.rows; row += step, flip ^= 1) {
-    const float mean = next_mean, rstd = next_rstd;
-    if (row + step < a.rows) next_mean = a.mean[row + step], next_rstd = a.rstd[row + step];
-    ring.wait(a.status);
-    Raw<T, VEC> rx[K], ry[K];
+  c.init(a, tid * VEC, size);
+  bool in[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      rx[k].load(reinterpret_cast<const T*>(ring.at()) + col, col < a.cols);
-      ry[k].load(reinterpret_cast<const T*>(ring.at() + bytes) + col, col < a.cols);
+  for (int k = 0; k < K; ++k) in[k] = EXACT || (k * size + tid) * VEC < a.cols;
+  // the rows of an iteration overlap their reductions; a missing row is zeros
+  constexpr int R = 1;
+  float next_mean[R], next_rstd[R];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool here = row + r * step < a.rows;
+      next_mean[r] = here ? a.mean[row + r * step] : 0.f;
+      next_rstd[r] = here ? a.rstd[row + r * step] : 0.f;
     }
-    const float2 s = group_sum2(c.add(rx, ry, mean, rstd), red[flip], size, group);
-    if (fill < a.rows) {
-      if (tid == 0) copy(ring.slot);
-      fill += step;
+  };
+  fetch(first);
+  T* dx = static_cast<T*>(a.dx) + (a.dx ? first * a.lddx + tid * VEC : 0);
+  const long long next_dx = step * a.lddx;
+  int flip = 0;
+  for (long long row = first; row < a.rows; row += R * step, flip ^= 1, dx += R * next_dx) {
+    float mean[R], rstd[R];
+    Raw<T, VEC> rx[R][K], ry[R][K];
+    int slot[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool here = r == 0 || row + r * step < a.rows;
+      mean[r] = next_mean[r], rstd[r] = next_rstd[r];
+      slot[r] = ring.slot;
+      if (here) ring.wait(a.status);
+      const T* from = reinterpret_cast<const T*>(ring.at()) + tid * VEC;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        rx[r][k].load(from + k * size * VEC, here && in[k]);
+        ry[r][k].load(from + a.cols + k * size * VEC, here && in[k]);
+      }
+      if (here) ring.next();
     }
-    ring.next();
-    if (a.dx) c.write(a, rx, ry, row, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols, tid, size);
+    fetch(row + R * step);
+    float2 s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = c.add(rx[r], ry[r], mean[r], rstd[r]);
+    if constexpr (R == 2) {
+      const float4 t = group_sum(make_float4(s[0].x, s[0].y, s[R - 1].x, s[R - 1].y), red[flip], size, group);
+      s[0] = make_float2(t.x, t.y), s[R - 1] = make_float2(t.z, t.w);
+    } else {
+      const float4 t = group_sum(make_float4(s[0].x, s[0].y, 0.f, 0.f), red[flip], size, group);
+      s[0] = make_float2(t.x, t.y);
+    }
+    // the reduction is behind every thread's reads of the buffers
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (fill < a.rows && (r == 0 || row + r * step < a.rows)) {
+        if (tid == 0) copy(slot[r]);
+        fill += step;
+      }
+    if (a.dx) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r == 0 || row + r * step < a.rows)
+          c.write(rx[r], ry[r], in, dx + r * next_dx, size, mean[r], rstd[r], s[r].x * a.inv_cols, s[r].y * a.inv_cols);
+    }
   }
   if (tid == 0) ring.drain((fill - first) / step);
   grid_dependents_launch();
@@ -440,7 +568,7 @@ __global__ void __launch_bounds__(1024) ln_row_sums(const LnArgs a) {
         s.y = fmaf(w, (rx.get(i) - mean) * rstd, s.y);
       }
     }
-    s = group_sum2(s, red[flip], 1024, 0);
+    s = group_sum(s, red[flip], 1024, 0);
     if (threadIdx.x == 0) a.stats[row] = make_float4(mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
 }
@@ -451,11 +579,9 @@ constexpr int kSlabThreads = 256, kSlabRows = 4;
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
   const int col0 = blockIdx.y * kSlabThreads * VEC, col = col0 + threadIdx.x * VEC;
-  const bool in = col < a.cols;
+  const bool in = col < a.cols, mine[1] = {in};
   Columns<T, P, VEC, 1> c;
-  load_param<P, VEC>(a.gamma, col, in, 1.f, c.gamma[0]);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) c.dg[0][i] = c.db[0][i] = 0.f;
+  c.init(a, col, kSlabThreads);
   for (long long row0 = (long long)blockIdx.x * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.x * kSlabRows) {
     Raw<T, VEC> rx[kSlabRows][1], ry[kSlabRows][1];
     float4 st[kSlabRows];
@@ -471,13 +597,20 @@ __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a)
     for (int r = 0; r < kSlabRows; ++r) {
       if (row0 + r >= a.rows) break;
       c.add(rx[r], ry[r], st[r].x, st[r].y);
-      if (a.dx) c.write(a, rx[r], ry[r], row0 + r, st[r].x, st[r].y, st[r].z, st[r].w, threadIdx.x, kSlabThreads, col0);
+      if (a.dx) c.write(rx[r], ry[r], mine, static_cast<T*>(a.dx) + (row0 + r) * a.lddx + col, kSlabThreads, st[r].x, st[r].y, st[r].z, st[r].w);
     }
   }
   if (!in) return;
   float* part = a.part + (long long)blockIdx.x * 2 * a.cols + col;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) part[i] = c.dg[0][i], part[a.cols + i] = c.db[0][i];
+  for (int i = 0; i < c.H; ++i) {
+    if constexpr (VEC > 1) {
+      const float2 g = unpair(c.dg[0][i]), b = unpair(c.db[0][i]);
+      part[2 * i] = g.x, part[2 * i + 1] = g.y, part[a.cols + 2 * i] = b.x, part[a.cols + 2 * i + 1] = b.y;
+    } else {
+      part[0] = c.dg[0][i], part[a.cols] = c.db[0][i];
+    }
+  }
 }
 
 // dgamma / dbeta = the partial rows added in order: 32 columns per block, the
@@ -531,6 +664,7 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   LnPlan p{};
   p.vec = wide ? 16 / es : 1;
   const int nvec = d.cols / p.vec;
+  auto sums_bytes = [](const LnPlan& q) { return size_t(512) * 2 * q.k * q.vec * sizeof(float); };
   auto threads_for = [&](int k, int most) {
     int t = 32;
     while (t < most && (long long)t * k < nvec) t *= 2;
@@ -547,26 +681,33 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   if (!wide) {
     const int few[3] = {1, 8, 16}, many[2] = {8, 16};
     const bool lots = d.rows >= 2LL * sms;
-    if (backward ? choose(many, 2, 512) : lots ? choose(many, 2, 1024) : choose(few, 3, 1024))
+    if (backward ? choose(many, 2, 512) : lots ? choose(many, 2, 1024) : choose(few, 3, 1024)) {
       p.threads = backward ? 512 : std::max(p.size, 32 * kWarpsPerBlock);
-    if (backward && p.size < 512) p.smem = size_t(2) * d.cols * sizeof(float);
+      if (backward) p.smem = sums_bytes(p);
+    }
     return p;
   }
+  // The ring pays from a few rows per group on; up to 32 values per thread in the forward
+  // pass, 16 in the backward pass (three more registers each), in as few threads as hold
+  // the row.
   const int ks[3] = {1, 2, 16 / p.vec};
-  // the ring pays from a few rows per group on
-  if (choose(ks, 3, 512)) {
-    const long long groups = 2LL * sms * (kRingThreads / p.size);
+  p.k = (backward ? 16 : 32) / p.vec;
+  while (p.k > 1 && 32 * (p.k / 2) >= nvec) p.k /= 2;
+  p.size = threads_for(p.k, kRingThreads);
+  if ((long long)p.size * p.k >= nvec) {
+    const long long groups = (long long)sms * (kRingThreads / p.size);
     const size_t stage = size_t(kRingThreads / p.size) * d.cols * es * (backward ? 2 : 1);
-    p.slots = int(std::min<size_t>(kMaxSlots, (backward && p.k * p.vec > 8 ? 200 * 1024 : 100 * 1024) / stage));
-    if (d.rows >= 2 * groups && p.slots >= 2) {
+    const size_t params = backward ? 0 : 8 * size_t(d.cols);
+    p.slots = int(std::min<size_t>(kMaxSlots, (200 * 1024 - params) / stage));
+    if (d.rows >= 2 * groups && p.slots >= 3) {
       p.ring = true;
       p.threads = kRingThreads;
-      p.smem = std::max(p.slots * stage, backward && p.size < kRingThreads ? size_t(2) * d.cols * sizeof(float) : size_t(0));
+      p.smem = std::max(p.slots * stage + params, backward ? sums_bytes(p) : size_t(0));
       return p;
     }
   }
   if (backward) {
-    if (choose(ks, 3, 512)) p.threads = 512, p.smem = p.size < 512 ? size_t(2) * d.cols * sizeof(float) : 0;
+    if (choose(ks, 3, 512)) p.threads = 512, p.smem = sums_bytes(p);
   } else {
     const int direct[3] = {1, 2, 4};
     if (choose(direct, 3, 1024)) p.threads = std::max(p.size, 32 * kWarpsPerBlock);
@@ -585,30 +726,45 @@ size_t ln_workspace(const pkt_layernorm_desc* d, int sms) {
 }
 
 template <typename... KArgs>
-int ln_launch_ring(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, int blocks, cudaStream_t st) {
+int ln_launch_shared(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, int blocks, cudaStream_t st) {
   const int rc = op_shared_memory(reinterpret_cast<const void*>(kernel), done, dev, 200 * 1024);
   if (rc) return rc;
   const cudaError_t e = op_launch(kernel, dim3(blocks), dim3(p.threads), p.smem, st, false, a);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
 }
 
+// The partial rows that a backward kernel wrote (as a positive result).
+template <typename T, typename P, int VEC, int K, bool EXACT>
+int ln_run_ring(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
+  static std::atomic<uint64_t> done[2];
+  if (!backward) return ln_launch_shared(ln_forward_ring<T, P, VEC, K, EXACT>, &done[1], dev, a, p, sms, st);
+  if constexpr (K * VEC <= 16) {
+    const int blocks = std::min(a.parts, sms), rc = ln_launch_shared(ln_backward_ring<T, P, VEC, K, EXACT>, &done[0], dev, a, p, blocks, st);
+    return rc ? rc : blocks;
+  }
+  return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
+}
+
 template <typename T, typename P, int VEC, int K>
 int ln_run(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
-  constexpr bool kBackward = K * VEC <= 16;  // the combinations that ln_plan gives
-  if constexpr (VEC > 1 && kBackward) {
-    static std::atomic<uint64_t> done[2];
-    if (p.ring && backward) return ln_launch_ring(ln_backward_ring<T, P, VEC, K>, &done[0], dev, a, p, a.parts, st);
-    if (p.ring) return ln_launch_ring(ln_forward_ring<T, P, VEC, K>, &done[1], dev, a, p, (K * VEC <= 8 ? 2 : 1) * sms, st);
+  if constexpr (VEC > 1) {
+    if (p.ring)
+      return a.cols == p.size * K * VEC ? ln_run_ring<T, P, VEC, K, true>(a, p, backward, dev, sms, st)
+                                        : ln_run_ring<T, P, VEC, K, false>(a, p, backward, dev, sms, st);
   }
-  cudaError_t e = cudaErrorInvalidConfiguration;
-  if constexpr (kBackward && !(VEC == 1 && K < 8)) {
-    if (backward) e = op_launch(ln_backward<T, P, VEC, K>, dim3(a.parts), dim3(p.threads), p.smem, st, false, a);
+  if constexpr (VEC == 1 || K <= 4) {
+    if (!backward) {
+      const long long blocks = (a.rows - 1) / (p.threads / p.size) + 1;
+      const cudaError_t e = op_launch(ln_forward<T, P, VEC, K>, dim3(unsigned(std::min(blocks, 1LL << 30))), dim3(p.threads), 0, st, false, a);
+      return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
+    }
   }
-  if (!backward) {
-    const long long blocks = (a.rows - 1) / (p.threads / p.size) + 1;
-    e = op_launch(ln_forward<T, P, VEC, K>, dim3(unsigned(std::min(blocks, 1LL << 30))), dim3(p.threads), 0, st, false, a);
+  if constexpr (K * VEC <= 16 && !(VEC == 1 && K < 8)) {
+    static std::atomic<uint64_t> done;
+    const int rc = ln_launch_shared(ln_backward<T, P, VEC, K>, &done, dev, a, p, a.parts, st);
+    return rc ? rc : a.parts;
   }
-  return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
+  return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
 }
 
 template <typename T, typename P, int VEC>
@@ -629,13 +785,12 @@ int ln_pick(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStre
     case 1: return ln_run<T, P, VEC, 1>(a, p, backward, dev, sms, st);
     case 2: if constexpr (VEC > 1) return ln_run<T, P, VEC, 2>(a, p, backward, dev, sms, st); break;
     case 4: if constexpr (VEC > 1) return ln_run<T, P, VEC, 4>(a, p, backward, dev, sms, st); break;
-    case 8: if constexpr (VEC == 1) return ln_run<T, P, 1, 8>(a, p, backward, dev, sms, st); break;
+    case 8: if constexpr (VEC != 8) return ln_run<T, P, VEC, 8>(a, p, backward, dev, sms, st); break;
     case 16: if constexpr (VEC == 1) return ln_run<T, P, 1, 16>(a, p, backward, dev, sms, st); break;
   }
   return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
 }
 
-// PKT_OK, an error, or (backward, long rows) the number of partial rows written.
 template <typename T>
 int ln_dispatch(const LnArgs& a, const LnPlan& p, int param_dtype, bool backward, int dev, int sms, cudaStream_t st) {
   constexpr int W = 16 / int(sizeof(T));
@@ -750,7 +905,7 @@ int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
   rc = d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, true, dev, sms, st)
                                   : ln_dispatch<float>(a, p, d->param_dtype, true, dev, sms, st);
   if (rc < 0) return rc;
-  if (rc > 0) a.parts = rc;
+  a.parts = rc;
   if (d->dgamma || d->dbeta) {
     const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part),
                                     a.parts, a.cols, d->dgamma, d->dbeta);

@@ -20,6 +20,38 @@ __device__ __forceinline__ void from_f32(float v, float* out) { *out = v; }
 // results are rounded to the tensor's type once, at the store
 __device__ __forceinline__ void from_f32(float v, bf16_t* out) { out->bits = f32_to_bf16_rn(v); }
 
+// Two fp32 values in one 64-bit register: one instruction for two results, each
+// rounded as by itself.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum_of(uint64_t v) {
+  const float2 f = unpair(v);
+  return f.x + f.y;
+}
+
 // VEC consecutive elements as raw words: one load of up to 16 bytes each.
 template <typename T, int VEC>
 struct Raw {
@@ -48,6 +80,8 @@ struct Raw {
   }
   __device__ __forceinline__ void set(int i, float v) { w[i * int(sizeof(T)) / 4] = __float_as_uint(v); }
   __device__ __forceinline__ void set(int i, bf16_t v) { w[i >> 1] |= uint32_t(v.bits) << (16 * (i & 1)); }
+  // elements 2 i and 2 i + 1
+  __device__ __forceinline__ uint64_t get2(int i) const { return pair_of(get(2 * i), get(2 * i + 1)); }
   __device__ __forceinline__ float get(int i) const {
     if (sizeof(T) == 4) return __uint_as_float(w[i]);
     return (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
@@ -81,20 +115,45 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pairs(T* p, const uint64_t (&v)[VEC / 2]) {
+  constexpr int kBytes = VEC * int(sizeof(T));
+  static_assert(kBytes == 16, "one access");
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) {
+    const float2 f = unpair(v[i]);
+    if constexpr (sizeof(T) == 2)
+      w[i] = pack_bf16x2(f.x, f.y);
+    else
+      w[2 * i] = __float_as_uint(f.x), w[2 * i + 1] = __float_as_uint(f.y);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ---------------------------------------------------------------- bulk copies and bounded waits
-// Waits until the phase of `parity` has completed; false when it has not after 2^21
-// tries of up to a microsecond each (about 2 s). One block of assembly: the
-// compiler's own form of the loop kept the lanes apart (BSSY / BSYNC around each
-// try) and cost hot loops a third of their instructions.
+// Waits until the phase of `parity` has completed; false when it has not after 2 s
+// (the timer is only looked at every 1024 tries). One block of assembly: the
+// compiler's own form of the loop kept the lanes apart (BSSY / BSYNC around each try)
+// and cost hot loops a third of their instructions. No suspend-time hint: it turns a
+// failed try into a sleep.
 __device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "{\n .reg .pred p, q;\n .reg .u32 n, m;\n .reg .u64 t, t0;\n"
+      " mov.u32 n, 0;\n mov.u64 t0, 0;\n"
       "AGAIN:\n"
-      " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, 1000;\n"
+      " mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
       " @p bra DONE;\n"
       " add.u32 n, n, 1;\n"
-      " setp.lt.u32 q, n, 0x200000;\n"
+      " and.b32 m, n, 1023;\n"
+      " setp.ne.u32 q, m, 0;\n"
+      " @q bra AGAIN;\n"
+      " mov.u64 t, %%globaltimer;\n"
+      " setp.eq.u64 q, t0, 0;\n"
+      " @q mov.u64 t0, t;\n"
+      " sub.u64 t, t, t0;\n"
+      " setp.lt.u64 q, t, 2000000000;\n"
       " @q bra AGAIN;\n"
       "DONE:\n"
       " selp.u32 %0, 1, 0, p;\n}\n"
