@@ -9,20 +9,20 @@
 // Both are bound by memory: 2 and 3 passes over the rows. A row is read once and stays
 // in registers between the statistics and the result (the variance is the mean square
 // of the centred values, not E x^2 - mean^2, which cancels). Rows belong to groups of
-// 32..512 threads, several groups to a block where rows are short.
+// 32..512 threads, several groups to a block where rows are short; a thread computes on
+// pairs of values (one instruction for two).
 //
-// Where there are many 16-byte aligned rows, each group runs its own ring of row
-// buffers in shared memory, filled by bulk copies several rows ahead: the bytes in
-// flight do not depend on the registers left over. Few rows, or unaligned ones, are
-// loaded directly. Rows of more than 8192 values take two passes in the backward
-// direction: the row sums first, then slabs of columns that need no reduction.
+// Where there are many rows, each group runs its own ring of row buffers in shared
+// memory, filled by bulk copies a few rows ahead, whatever the rows' alignment (a copy
+// takes the 16-byte granules that hold the row). Few rows are loaded directly. Rows of
+// more than 8192 values take two passes in the backward direction: the row sums first,
+// then slabs of columns that need no reduction.
 //
 // The column sums dgamma / dbeta are kept in the registers of the threads that own the
 // columns, across the rows of a block; every block writes one partial row to the
 // workspace and a second kernel (launched with programmatic dependency) adds the
 // partial rows in a fixed order, so results do not depend on timing. All sums are fp32.
 #include <algorithm>
-#include <type_traits>
 
 #include "ops_common.h"
 #include "ops_device.cuh"
@@ -42,27 +42,21 @@ struct LnArgs {
   float* part;    // backward: [parts][2][cols]
   float4* stats;  // backward, long rows: [rows] mean, rstd and the two row sums
   int parts, size, slots;
+  uint32_t pitch;  // bytes of a row buffer
   int* status;
 };
 
-constexpr int kWarpsPerBlock = 4;   // rows per block where a warp has a row (direct loads)
 constexpr int kRingThreads = 512;
 constexpr int kMaxSlots = 8;
 
 // The sums of `v` over the threads of a row group (a power of two of warps); `red`
 // holds one word per warp of the block. One barrier: callers alternate between two
 // arrays, so that the barrier of one reduction protects the other's words.
-__device__ __forceinline__ float add_to(float a, float b) { return a + b; }
 __device__ __forceinline__ float2 add_to(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
-__device__ __forceinline__ float shuffled(float v, int off) { return __shfl_xor_sync(0xffffffffu, v, off); }
-__device__ __forceinline__ float2 shuffled(float2 v, int off) { return make_float2(shuffled(v.x, off), shuffled(v.y, off)); }
-__device__ __forceinline__ float4 add_to(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
-__device__ __forceinline__ float4 shuffled(float4 v, int off) {
-  return make_float4(shuffled(v.x, off), shuffled(v.y, off), shuffled(v.z, off), shuffled(v.w, off));
+__device__ __forceinline__ float2 shuffled(float2 v, int off) {
+  return make_float2(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off));
 }
-
-template <typename V>
-__device__ __forceinline__ V group_sum(V v, V* red, int size, int group) {
+__device__ __forceinline__ float2 group_sum(float2 v, float2* red, int size, int group) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v = add_to(v, shuffled(v, off));
   if (size == 32) return v;
@@ -74,74 +68,95 @@ __device__ __forceinline__ V group_sum(V v, V* red, int size, int group) {
   return v;
 }
 
-// VEC parameters at col (whole vectors: a row's columns are a multiple of VEC).
-template <typename P, int VEC>
-__device__ __forceinline__ void load_param(const void* base, int col, bool in, float other, float (&v)[VEC]) {
-  Raw<P, VEC> r;
-  r.load(static_cast<const P*>(base) + col, in && base != nullptr);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = base != nullptr ? r.get(i) : in ? other : 0.f;
-}
+__device__ __forceinline__ uint64_t twice(float v) { return pair_of(v, v); }
 
-// ---------------------------------------------------------------- forward
-// Statistics of a row that a group holds as K vectors per thread.
-template <typename T, int VEC, int K>
-__device__ __forceinline__ float2 row_stats(const Raw<T, VEC> (&raw)[K], const LnArgs& a, int tid, int size, int group, float (*red)[32]) {
-  float sum = 0.f;
+// N values of a row in one thread, as raw words: N / VEC vectors of VEC consecutive
+// values, vector k at column (k * size + tid) * VEC; zeros past the row's end. EXACT:
+// the threads cover the row without a rest.
+template <typename T, int VEC, int N>
+struct Held {
+  static constexpr int K = N / VEC;
+  uint32_t w[N * int(sizeof(T)) / 4];
+
+  static __device__ __forceinline__ int col(int k, int tid, int size) { return (k * size + tid) * VEC; }
+  template <bool EXACT>
+  __device__ __forceinline__ void load(const T* row, int tid, int size, int cols, bool here = true) {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int i = 0; i < N * int(sizeof(T)) / 4; ++i) w[i] = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += raw[k].get(i);
-  const float mean = group_sum(sum, red[0], size, group) * a.inv_cols;
-  float sq = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if ((k * size + tid) * VEC < a.cols) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = raw[k].get(i) - mean;
-        sq = fmaf(d, d, sq);
+    for (int k = 0; k < K; ++k) {
+      const int c = col(k, tid, size);
+      if (!here || (!EXACT && c >= cols)) continue;
+      if constexpr (VEC > 1) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + c);
+        w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+      } else if constexpr (sizeof(T) == 4) {
+        w[k] = *reinterpret_cast<const uint32_t*>(row + c);
+      } else {
+        w[k / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(row + c)) << (16 * (k & 1));
       }
     }
   }
-  return make_float2(mean, 1.f / sqrtf(group_sum(sq, red[1], size, group) * a.inv_cols + a.eps));
-}
+  // values 2 p and 2 p + 1 of the thread
+  __device__ __forceinline__ uint64_t pair(int p) const {
+    if constexpr (sizeof(T) == 4) return pair_of(__uint_as_float(w[2 * p]), __uint_as_float(w[2 * p + 1]));
+    return pair_of(bf16_lo(w[p]), bf16_hi(w[p]));
+  }
+  // -mean for the values inside the row, 0 for the zeros past its end
+  template <bool EXACT>
+  static __device__ __forceinline__ uint64_t minus(float mean, int p, int tid, int size, int cols) {
+    if constexpr (EXACT) return twice(-mean);
+    const int c0 = col(2 * p / VEC, tid, size), c1 = col((2 * p + 1) / VEC, tid, size);
+    return pair_of(c0 < cols ? -mean : 0.f, c1 < cols ? -mean : 0.f);
+  }
+};
 
-__device__ __forceinline__ void put_stats(const LnArgs& a, long long row, float2 st) {
-  if (a.mean) a.mean[row] = st.x;
-  if (a.rstd) a.rstd[row] = st.y;
-}
-
-template <typename T, typename P, int VEC, int K>
-__global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
-  __shared__ float red[2][32];
-  const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
-  for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    Raw<T, VEC> raw[K];
+// The results of a row, rounded to its type once.
+template <typename T, int VEC, int N, bool EXACT>
+__device__ __forceinline__ void store_held(T* row, const uint64_t (&v)[N / 2], int tid, int size, int cols) {
+  using S = Held<T, VEC, N>;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      raw[k].load(x + col, col < a.cols);
-    }
-    const float2 st = row_stats<T, VEC, K>(raw, a, tid, size, group, red);
-    if (tid == 0) put_stats(a, row, st);
-    T* y = static_cast<T*>(a.y) + row * a.ldy;
+  for (int k = 0; k < S::K; ++k) {
+    const int c = S::col(k, tid, size);
+    if (!EXACT && c >= cols) continue;
+    if constexpr (VEC > 1) {
+      uint64_t q[VEC / 2];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      if (col >= a.cols) continue;
-      float g[VEC], b[VEC], out[VEC];
-      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
-      load_param<P, VEC>(a.beta, col, true, 0.f, b);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = fmaf((raw[k].get(i) - st.x) * st.y, g[i], b[i]);
-      store_vec<T, VEC>(y + col, out);
+      for (int i = 0; i < VEC / 2; ++i) q[i] = v[k * VEC / 2 + i];
+      store_pairs<T, VEC>(row + c, q);
+    } else {
+      const float2 f = unpair(v[k / 2]);
+      from_f32(k & 1 ? f.y : f.x, row + c);
     }
   }
 }
 
-// One ring of row buffers per group.
+// The thread's pairs of a parameter row (fp32 or bf16; `other` where there is none).
+template <typename P, int VEC, int N>
+__device__ __forceinline__ void load_params(const void* base, float other, int col0, int size, int cols, uint64_t (&out)[N / 2]) {
+#pragma unroll
+  for (int k = 0; k < N / (VEC > 1 ? VEC : 2); ++k) {
+    if constexpr (VEC > 1) {
+      const int c = col0 + k * size * VEC;
+      Raw<P, VEC> r;
+      r.load(static_cast<const P*>(base) + c, base && c < cols);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) out[k * VEC / 2 + i] = base ? r.get2(i) : twice(c < cols ? other : 0.f);
+    } else {
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = col0 + (2 * k + i) * size;
+        f[i] = c >= cols ? 0.f : base ? to_f32(static_cast<const P*>(base)[c]) : other;
+      }
+      out[k] = pair_of(f[0], f[1]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- rings of row buffers
+// The rows of a group: first, first + step, ... A buffer takes the 16-byte granules
+// that hold a row; shift() is where the row begins in it.
 struct Ring {
   uint8_t* buf;     // [slots][bytes]
   uint64_t* full;   // [slots]
@@ -153,7 +168,6 @@ struct Ring {
   __device__ __forceinline__ void wait(int* status) {
     if (!dead) dead = !wait_phase(&full[slot], phase, status);
   }
-  __device__ __forceinline__ const uint8_t* at() const { return buf + slot * bytes; }
   __device__ __forceinline__ void next() {
     if (++slot == slots) slot = 0, phase ^= 1;
   }
@@ -163,6 +177,12 @@ struct Ring {
     for (long long f = filled > slots ? filled - slots : 0; f < filled; ++f) try_phase(&full[f % slots], (f / slots) & 1);
   }
 };
+
+__device__ __forceinline__ uint32_t shift(const void* p) { return uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u; }
+__device__ __forceinline__ uint32_t granules(const void* p, uint32_t bytes) { return (shift(p) + bytes + 15u) & ~15u; }
+__device__ __forceinline__ const void* granule(const void* p) {
+  return reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+}
 
 __device__ __forceinline__ Ring make_ring(uint8_t* smem, uint64_t (*full)[kMaxSlots], const LnArgs& a, int groups, int group, uint32_t bytes) {
   if (threadIdx.x == 0) {
@@ -174,98 +194,142 @@ __device__ __forceinline__ Ring make_ring(uint8_t* smem, uint64_t (*full)[kMaxSl
   return Ring{smem + (size_t)group * a.slots * bytes, full[group], bytes, a.slots, 0, 0, false};
 }
 
+// ---------------------------------------------------------------- forward
+__device__ __forceinline__ void put_stats(const LnArgs& a, long long row, float mean, float rstd) {
+  if (a.mean) a.mean[row] = mean;
+  if (a.rstd) a.rstd[row] = rstd;
+}
+
+template <typename T, typename P, int VEC, int N>
+__global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
+  __shared__ float2 red[2][32];
+  const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
+    Held<T, VEC, N> x;
+    x.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, tid, size, a.cols);
+    uint64_t s = 0;
+#pragma unroll
+    for (int p = 0; p < N / 2; ++p) s = add2(s, x.pair(p));
+    const float mean = group_sum(make_float2(sum_of(s), 0.f), red[0], size, group).x * a.inv_cols;
+    s = 0;
+#pragma unroll
+    for (int p = 0; p < N / 2; ++p) {
+      const uint64_t d = add2(x.pair(p), x.template minus<false>(mean, p, tid, size, a.cols));
+      s = fma2(d, d, s);
+    }
+    const float rstd = 1.f / sqrtf(group_sum(make_float2(sum_of(s), 0.f), red[1], size, group).x * a.inv_cols + a.eps);
+    if (tid == 0) put_stats(a, row, mean, rstd);
+    uint64_t g[N / 2], b[N / 2], out[N / 2];
+    load_params<P, VEC, N>(a.gamma, 1.f, tid * VEC, size, a.cols, g);
+    load_params<P, VEC, N>(a.beta, 0.f, tid * VEC, size, a.cols, b);
+#pragma unroll
+    for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(add2(x.pair(p), twice(-mean)), twice(rstd)), g[p], b[p]);
+    store_held<T, VEC, N, false>(static_cast<T*>(a.y) + row * a.ldy, out, tid, size, a.cols);
+  }
+}
+
 // Two rows at a time, so that their reductions overlap, up to 32 values of each per
-// thread in pairs, the parameters as fp32 in shared memory. The kernel was bound by its
+// thread, the parameters as fp32 in shared memory. The kernel was bound by its
 // instructions: 30 per value with 8 values per thread (the fixed work of a row is two
-// thirds of that), 19 with 16, 12 like this (8192 x 4096 bf16: 43, 33 and 27 us).
-// EXACT: the group's threads cover the row without a rest.
-template <typename T, typename P, int VEC, int K, bool EXACT>
+// thirds of that), 19 with 16, 12 like this (8192 x 4096 bf16: 43, 33 and 26 us).
+template <typename T, typename P, int VEC, int N, bool EXACT>
 __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
   __shared__ float2 red[2][32];
-  constexpr int H = VEC / 2;
   const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
-  float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols]
+  float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols rounded up to 4]
+  const int pcols = (a.cols + 3) & ~3;
   for (int c = threadIdx.x; c < a.cols; c += kRingThreads) {
     params[c] = a.gamma ? to_f32(static_cast<const P*>(a.gamma)[c]) : 1.f;
-    params[a.cols + c] = a.beta ? to_f32(static_cast<const P*>(a.beta)[c]) : 0.f;
+    params[pcols + c] = a.beta ? to_f32(static_cast<const P*>(a.beta)[c]) : 0.f;
   }
-  Ring ring = make_ring(ring_smem + 8 * (size_t)a.cols, full, a, groups, group, bytes);
+  Ring ring = make_ring(ring_smem + 8 * (size_t)pcols, full, a, groups, group, a.pitch);
   const T* x = static_cast<const T*>(a.x);
   long long fill = first;  // the next row to copy
   auto copy = [&](int slot) {
-    mbar_arrive_expect_tx(&ring.full[slot], bytes);
-    bulk_load(ring.buf + slot * bytes, x + fill * a.ldx, bytes, &ring.full[slot]);
+    const T* from = x + fill * a.ldx;
+    const uint32_t n = granules(from, bytes);
+    mbar_arrive_expect_tx(&ring.full[slot], n);
+    bulk_load(ring.buf + slot * ring.bytes, granule(from), n, &ring.full[slot]);
   };
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
     if (tid == 0) copy(i);
-  bool in[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) in[k] = EXACT || (k * size + tid) * VEC < a.cols;
-  params += tid * VEC;
-  T* y = static_cast<T*>(a.y) + first * a.ldy + tid * VEC;
-  const long long next_y = step * a.ldy;
-  for (long long row = first; row < a.rows; row += 2 * step, y += 2 * next_y) {
+  T* y = static_cast<T*>(a.y) + first * a.ldy;
+  const T* at = x + first * a.ldx;
+  const long long next_y = step * a.ldy, next_x = step * a.ldx;
+  for (long long row = first; row < a.rows; row += 2 * step, y += 2 * next_y, at += 2 * next_x) {
     const bool two = row + step < a.rows;
-    Raw<T, VEC> raw[2][K];
-    int slot[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {  // a missing second row is zeros
-      slot[r] = ring.slot;
-      if (r == 0 || two) ring.wait(a.status);
-      const T* from = reinterpret_cast<const T*>(ring.at()) + tid * VEC;
-#pragma unroll
-      for (int k = 0; k < K; ++k) raw[r][k].load(from + k * size * VEC, in[k] && (r == 0 || two));
-      if (r == 0 || two) ring.next();
-    }
+    Held<T, VEC, N> x0, x1;  // a missing second row is zeros
+    const int slot0 = ring.slot;
+    ring.wait(a.status);
+    x0.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at))), tid, size, a.cols);
+    ring.next();
+    const int slot1 = ring.slot;
+    if (two) ring.wait(a.status);
+    x1.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at + next_x))), tid, size, a.cols,
+                            two);
+    if (two) ring.next();
     uint64_t s0 = 0, s1 = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < H; ++i) s0 = add2(s0, raw[0][k].get2(i)), s1 = add2(s1, raw[1][k].get2(i));
+    for (int p = 0; p < N / 2; ++p) s0 = add2(s0, x0.pair(p)), s1 = add2(s1, x1.pair(p));
     const float2 sum = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[0], size, group);
     const float2 mean = make_float2(sum.x * a.inv_cols, sum.y * a.inv_cols);
-    const uint64_t m0 = pair_of(-mean.x, -mean.x), m1 = pair_of(-mean.y, -mean.y);
     s0 = s1 = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (!in[k]) continue;
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        const uint64_t d0 = add2(raw[0][k].get2(i), m0), d1 = add2(raw[1][k].get2(i), m1);
-        s0 = fma2(d0, d0, s0);
-        s1 = fma2(d1, d1, s1);
-      }
+    for (int p = 0; p < N / 2; ++p) {
+      const uint64_t d0 = add2(x0.pair(p), x0.template minus<EXACT>(mean.x, p, tid, size, a.cols));
+      const uint64_t d1 = add2(x1.pair(p), x1.template minus<EXACT>(mean.y, p, tid, size, a.cols));
+      s0 = fma2(d0, d0, s0);
+      s1 = fma2(d1, d1, s1);
     }
     const float2 sq = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[1], size, group);
     const float2 rstd = make_float2(1.f / sqrtf(sq.x * a.inv_cols + a.eps), 1.f / sqrtf(sq.y * a.inv_cols + a.eps));
     // the reductions are behind every thread's reads of the buffers
     if (tid == 0) {
-      if (fill < a.rows) copy(slot[0]);
+      if (fill < a.rows) copy(slot0);
       fill += step;
-      if (two && fill < a.rows) copy(slot[1]);
+      if (two && fill < a.rows) copy(slot1);
       fill += step;
-      put_stats(a, row, make_float2(mean.x, rstd.x));
-      if (two) put_stats(a, row + step, make_float2(mean.y, rstd.y));
+      put_stats(a, row, mean.x, rstd.x);
+      if (two) put_stats(a, row + step, mean.y, rstd.y);
     }
-    const uint64_t r0 = pair_of(rstd.x, rstd.x), r1 = pair_of(rstd.y, rstd.y);
+    const uint64_t m0 = twice(-mean.x), m1 = twice(-mean.y), r0 = twice(rstd.x), r1 = twice(rstd.y);
+    constexpr int C = VEC > 1 ? VEC : 2;  // values stored together
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (!in[k]) continue;
-      Raw<float, VEC> g, b;
-      g.load(params + k * size * VEC, true);
-      b.load(params + a.cols + k * size * VEC, true);
-      uint64_t out[H];
+    for (int q = 0; q < N / C; ++q) {
+      const int c0 = Held<T, VEC, N>::col(q * C / VEC, tid, size), c1 = VEC > 1 ? c0 + 1 : Held<T, VEC, N>::col(2 * q + 1, tid, size);
+      if (!EXACT && c0 >= a.cols) continue;
+      uint64_t g[C / 2], b[C / 2], out[C / 2];
+      if constexpr (VEC > 1) {
 #pragma unroll
-      for (int i = 0; i < H; ++i) out[i] = fma2(mul2(add2(raw[0][k].get2(i), m0), r0), g.get2(i), b.get2(i));
-      store_pairs<T, VEC>(y + k * size * VEC, out);
-      if (!two) continue;
+        for (int i = 0; i < C / 4; ++i) {
+          const float4 u = *reinterpret_cast<const float4*>(params + c0 + 4 * i), v = *reinterpret_cast<const float4*>(params + pcols + c0 + 4 * i);
+          g[2 * i] = pair_of(u.x, u.y), g[2 * i + 1] = pair_of(u.z, u.w);
+          b[2 * i] = pair_of(v.x, v.y), b[2 * i + 1] = pair_of(v.z, v.w);
+        }
+      } else {
+        const bool in = c1 < a.cols;
+        g[0] = pair_of(params[c0], in ? params[c1] : 0.f);
+        b[0] = pair_of(params[pcols + c0], in ? params[pcols + c1] : 0.f);
+      }
 #pragma unroll
-      for (int i = 0; i < H; ++i) out[i] = fma2(mul2(add2(raw[1][k].get2(i), m1), r1), g.get2(i), b.get2(i));
-      store_pairs<T, VEC>(y + next_y + k * size * VEC, out);
+      for (int r = 0; r < 2; ++r) {
+        if (r == 1 && !two) break;
+#pragma unroll
+        for (int i = 0; i < C / 2; ++i)
+          out[i] = fma2(mul2(add2((r ? x1 : x0).pair(q * C / 2 + i), r ? m1 : m0), r ? r1 : r0), g[i], b[i]);
+        T* to = y + (r ? next_y : 0);
+        if constexpr (VEC > 1) {
+          store_pairs<T, VEC>(to + c0, out);
+        } else {
+          const float2 f = unpair(out[0]);
+          from_f32(f.x, to + c0);
+          if (c1 < a.cols) from_f32(f.y, to + c1);
+        }
+      }
     }
   }
   if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
@@ -275,270 +339,190 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
 // (the second and third time from L2).
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
-  __shared__ float red[2][32];
-  const int step = blockDim.x * VEC, begin = threadIdx.x * VEC;
+  constexpr int N = VEC > 1 ? VEC : 2;
+  __shared__ float2 red[2][32];
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    float sum = 0.f;
-    for (int col = begin; col < a.cols; col += step) {
-      Raw<T, VEC> r;
-      r.load(x + col, true);
+    T* y = static_cast<T*>(a.y) + row * a.ldy;
+    uint64_t s = 0;
+#pragma unroll 4
+    for (int c = 0; c < a.cols; c += 1024 * N) {
+      Held<T, VEC, N> v;
+      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += r.get(i);
+      for (int p = 0; p < N / 2; ++p) s = add2(s, v.pair(p));
     }
-    const float mean = group_sum(sum, red[0], blockDim.x, 0) * a.inv_cols;
-    float sq = 0.f;
-    for (int col = begin; col < a.cols; col += step) {
-      Raw<T, VEC> r;
-      r.load(x + col, true);
+    const float mean = group_sum(make_float2(sum_of(s), 0.f), red[0], 1024, 0).x * a.inv_cols;
+    s = 0;
+#pragma unroll 4
+    for (int c = 0; c < a.cols; c += 1024 * N) {
+      Held<T, VEC, N> v;
+      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = r.get(i) - mean;
-        sq = fmaf(d, d, sq);
+      for (int p = 0; p < N / 2; ++p) {
+        const uint64_t d = add2(v.pair(p), v.template minus<false>(mean, p, threadIdx.x, 1024, a.cols - c));
+        s = fma2(d, d, s);
       }
     }
-    const float rstd = 1.f / sqrtf(group_sum(sq, red[1], blockDim.x, 0) * a.inv_cols + a.eps);
-    if (threadIdx.x == 0) put_stats(a, row, make_float2(mean, rstd));
-    T* y = static_cast<T*>(a.y) + row * a.ldy;
-    for (int col = begin; col < a.cols; col += step) {
-      Raw<T, VEC> r;
-      r.load(x + col, true);
-      float g[VEC], b[VEC], out[VEC];
-      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
-      load_param<P, VEC>(a.beta, col, true, 0.f, b);
+    const float rstd = 1.f / sqrtf(group_sum(make_float2(sum_of(s), 0.f), red[1], 1024, 0).x * a.inv_cols + a.eps);
+    if (threadIdx.x == 0) put_stats(a, row, mean, rstd);
+#pragma unroll 2
+    for (int c = 0; c < a.cols; c += 1024 * N) {
+      Held<T, VEC, N> v;
+      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
+      uint64_t g[N / 2], b[N / 2], out[N / 2];
+      load_params<P, VEC, N>(a.gamma, 1.f, c + threadIdx.x * VEC, 1024, a.cols, g);
+      load_params<P, VEC, N>(a.beta, 0.f, c + threadIdx.x * VEC, 1024, a.cols, b);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = fmaf((r.get(i) - mean) * rstd, g[i], b[i]);
-      store_vec<T, VEC>(y + col, out);
+      for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(add2(v.pair(p), twice(-mean)), twice(rstd)), g[p], b[p]);
+      store_held<T, VEC, N, false>(y + c, out, threadIdx.x, 1024, a.cols - c);
     }
   }
 }
 
 // ---------------------------------------------------------------- backward
-// A thread's columns across the rows of its group, in pairs where it has vectors.
-template <typename T, typename P, int VEC, int K>
+// A thread's columns across the rows of its group.
+template <typename T, typename P, int VEC, int N>
 struct Columns {
-  static constexpr int kPair = VEC > 1 ? 2 : 1, H = VEC / kPair;
-  using V = std::conditional_t<VEC == 1, float, uint64_t>;
-  V gamma[K][H], dg[K][H], db[K][H];
-
-  static __device__ __forceinline__ float both(float v, float) { return v; }
-  static __device__ __forceinline__ uint64_t both(float v, uint64_t) { return pair_of(v, v); }
-  static __device__ __forceinline__ float add(float a, float b) { return a + b; }
-  static __device__ __forceinline__ uint64_t add(uint64_t a, uint64_t b) { return add2(a, b); }
-  static __device__ __forceinline__ float mul(float a, float b) { return a * b; }
-  static __device__ __forceinline__ uint64_t mul(uint64_t a, uint64_t b) { return mul2(a, b); }
-  static __device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
-  static __device__ __forceinline__ uint64_t fma(uint64_t a, uint64_t b, uint64_t c) { return fma2(a, b, c); }
-  static __device__ __forceinline__ float total(float v) { return v; }
-  static __device__ __forceinline__ float total(uint64_t v) { return sum_of(v); }
-  static __device__ __forceinline__ V value(const Raw<T, VEC>& r, int i) {
-    if constexpr (VEC > 1)
-      return r.get2(i);
-    else
-      return r.get(0);
-  }
+  uint64_t gamma[N / 2], dg[N / 2], db[N / 2];
 
   __device__ __forceinline__ void init(const LnArgs& a, int col0, int size) {
+    load_params<P, VEC, N>(a.gamma, 1.f, col0, size, a.cols, gamma);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = col0 + k * size * VEC;
-      float g[VEC];
-      load_param<P, VEC>(a.gamma, col, col < a.cols, 1.f, g);
+    for (int p = 0; p < N / 2; ++p) dg[p] = db[p] = 0;
+  }
+  // Adds a row and returns its sums of w and w h. Past the row's end dy and gamma are
+  // zero, and so is what they add.
+  __device__ __forceinline__ float2 add(const Held<T, VEC, N>& x, const Held<T, VEC, N>& y, float mean, float rstd) {
+    uint64_t s1 = 0, s2 = 0;
+    const uint64_t m = twice(-mean), r = twice(rstd);
 #pragma unroll
-      for (int i = 0; i < H; ++i) {
-        if constexpr (VEC > 1)
-          gamma[k][i] = pair_of(g[2 * i], g[2 * i + 1]);
-        else
-          gamma[k][i] = g[0];
-        dg[k][i] = db[k][i] = V(0);
-      }
+    for (int p = 0; p < N / 2; ++p) {
+      const uint64_t dy = y.pair(p), h = mul2(add2(x.pair(p), m), r), w = mul2(dy, gamma[p]);
+      dg[p] = fma2(dy, h, dg[p]);
+      db[p] = add2(db[p], dy);
+      s1 = add2(s1, w);
+      s2 = fma2(w, h, s2);
     }
+    return make_float2(sum_of(s1), sum_of(s2));
   }
-  // Adds a row and returns its sums of w and w h. Beyond the row's end dy and gamma
-  // are zero, and so is what they add.
-  __device__ __forceinline__ float2 add(const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], float mean, float rstd) {
-    V s1 = V(0), s2 = V(0);
-    const V m = both(-mean, V(0)), r = both(rstd, V(0));
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        const V dy = value(ry[k], i), h = mul(add(value(rx[k], i), m), r), w = mul(dy, gamma[k][i]);
-        dg[k][i] = fma(dy, h, dg[k][i]);
-        db[k][i] = add(db[k][i], dy);
-        s1 = add(s1, w);
-        s2 = fma(w, h, s2);
-      }
-    return make_float2(total(s1), total(s2));
-  }
-  // dx = rstd (w - c1 - h c2); `dx`: this thread's first column of the row
-  __device__ __forceinline__ void write(const Raw<T, VEC> (&rx)[K], const Raw<T, VEC> (&ry)[K], const bool (&in)[K], T* dx, int size, float mean,
+  // dx = rstd (w - c1 - h c2)
+  template <bool EXACT>
+  __device__ __forceinline__ void write(const Held<T, VEC, N>& x, const Held<T, VEC, N>& y, T* dx, int tid, int size, int cols, float mean,
                                         float rstd, float c1, float c2) {
-    const V m = both(-mean, V(0)), r = both(rstd, V(0)), r1 = both(-rstd * c1, V(0)), r2 = both(-rstd * c2 * rstd, V(0));
+    const uint64_t m = twice(-mean), r = twice(rstd), r1 = twice(-rstd * c1), r2 = twice(-rstd * c2 * rstd);
+    uint64_t out[N / 2];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (!in[k]) continue;
-      V out[H];
-#pragma unroll
-      for (int i = 0; i < H; ++i) out[i] = fma(mul(value(ry[k], i), gamma[k][i]), r, fma(add(value(rx[k], i), m), r2, r1));
-      if constexpr (VEC > 1)
-        store_pairs<T, VEC>(dx + k * size * VEC, out);
-      else
-        from_f32(out[0], dx + k * size);
-    }
+    for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(y.pair(p), gamma[p]), r, fma2(add2(x.pair(p), m), r2, r1));
+    store_held<T, VEC, N, EXACT>(dx, out, tid, size, cols);
   }
   // The block's partial row: its groups' column sums, added in group order. `sums`:
-  // shared memory, [groups][2 K VEC][size].
+  // shared memory, [groups][2 N][size].
   __device__ __forceinline__ void finish(const LnArgs& a, int tid, int size, int group, int groups, float* sums) {
-    constexpr int kHalf = K * VEC;
     float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
-    float* mine = sums + group * 2 * kHalf * size + tid;
+    float* mine = sums + group * 2 * N * size + tid;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < H; ++i) {
-        if constexpr (VEC > 1) {
-          const float2 g = unpair(dg[k][i]), b = unpair(db[k][i]);
-          mine[(k * VEC + 2 * i) * size] = g.x, mine[(k * VEC + 2 * i + 1) * size] = g.y;
-          mine[(kHalf + k * VEC + 2 * i) * size] = b.x, mine[(kHalf + k * VEC + 2 * i + 1) * size] = b.y;
-        } else {
-          mine[k * size] = dg[k][i], mine[(kHalf + k) * size] = db[k][i];
-        }
-      }
+    for (int p = 0; p < N / 2; ++p) {
+      const float2 g = unpair(dg[p]), b = unpair(db[p]);
+      mine[2 * p * size] = g.x, mine[(2 * p + 1) * size] = g.y;
+      mine[(N + 2 * p) * size] = b.x, mine[(N + 2 * p + 1) * size] = b.y;
+    }
     __syncthreads();
-    const int shift = 31 - __clz(size);
-    for (int j = threadIdx.x; j < 2 * kHalf * size; j += blockDim.x) {
+    const int log = 31 - __clz(size);
+    for (int j = threadIdx.x; j < 2 * N * size; j += blockDim.x) {
       float t = sums[j];
-      for (int g = 1; g < groups; ++g) t += sums[g * 2 * kHalf * size + j];
-      const int v = j >> shift, which = v >= kHalf, u = which ? v - kHalf : v;
+      for (int g = 1; g < groups; ++g) t += sums[g * 2 * N * size + j];
+      const int v = j >> log, which = v >= N, u = which ? v - N : v;
       const int col = (u / VEC * size + (j & (size - 1))) * VEC + u % VEC;
       if (col < a.cols) part[which * a.cols + col] = t;
     }
   }
 };
 
-// Direct loads; the next row's are issued before this row's reduction.
-template <typename T, typename P, int VEC, int K>
+// Few rows: direct loads, the next row's issued before this row's reduction.
+template <typename T, typename P, int VEC, int N>
 __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
   __shared__ float2 red[2][32];
   extern __shared__ __align__(128) uint8_t ring_smem[];
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
-  Columns<T, P, VEC, K> c;
-  c.init(a, tid * VEC, size);
-  Raw<T, VEC> rx[K], ry[K], nx[K], ny[K];
-  bool in[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) in[k] = (k * size + tid) * VEC < a.cols;
+  Held<T, VEC, N> nx, ny;
   float next_mean = 0.f, next_rstd = 0.f;
   auto fetch = [&](long long row) {
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int col = (k * size + tid) * VEC;
-      nx[k].load(x + col, col < a.cols);
-      ny[k].load(dy + col, col < a.cols);
-    }
+    nx.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, tid, size, a.cols);
+    ny.template load<false>(static_cast<const T*>(a.dy) + row * a.lddy, tid, size, a.cols);
     next_mean = a.mean[row], next_rstd = a.rstd[row];
   };
   if (first < a.rows) fetch(first);
+  Columns<T, P, VEC, N> c;
+  c.init(a, tid * VEC, size);
   int flip = 0;
   for (long long row = first; row < a.rows; row += step, flip ^= 1) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
+    const Held<T, VEC, N> x = nx, y = ny;
     const float mean = next_mean, rstd = next_rstd;
     if (row + step < a.rows) fetch(row + step);
-    const float2 s = group_sum(c.add(rx, ry, mean, rstd), red[flip], size, group);
+    const float2 s = group_sum(c.add(x, y, mean, rstd), red[flip], size, group);
     if (a.dx)
-      c.write(rx, ry, in, static_cast<T*>(a.dx) + row * a.lddx + tid * VEC, size, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+      c.template write<false>(x, y, static_cast<T*>(a.dx) + row * a.lddx, tid, size, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
   grid_dependents_launch();
   c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
 }
 
-template <typename T, typename P, int VEC, int K, bool EXACT>
+// x and dy through the ring. The copies queued ahead of it make any other load slow
+// (a mean loaded one row ahead measured 3400 cycles of waiting per row), so mean and
+// rstd are loaded 32 rows at a time, one row per lane, 32 rows ahead.
+template <typename T, typename P, int VEC, int N, bool EXACT>
 __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
-  __shared__ float4 red[2][kRingThreads / 32];
-  const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
+  __shared__ float2 red[2][32];
+  const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size, lane = threadIdx.x & 31;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
-  Ring ring = make_ring(ring_smem, full, a, groups, group, 2 * bytes);
+  Columns<T, P, VEC, N> c;
+  c.init(a, tid * VEC, size);
+  float mean32, rstd32, next_mean32, next_rstd32;
+  auto fetch = [&](long long row) {
+    const bool here = row + lane * step < a.rows;
+    next_mean32 = here ? a.mean[row + lane * step] : 0.f;
+    next_rstd32 = here ? a.rstd[row + lane * step] : 0.f;
+  };
+  fetch(first);
+  Ring ring = make_ring(ring_smem, full, a, groups, group, 2 * a.pitch);
   const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
   long long fill = first;
   auto copy = [&](int slot) {
-    mbar_arrive_expect_tx(&ring.full[slot], 2 * bytes);
-    bulk_load(ring.buf + slot * 2 * bytes, x + fill * a.ldx, bytes, &ring.full[slot]);
-    bulk_load(ring.buf + slot * 2 * bytes + bytes, dy + fill * a.lddy, bytes, &ring.full[slot]);
+    const T *fx = x + fill * a.ldx, *fy = dy + fill * a.lddy;
+    const uint32_t nx = granules(fx, bytes), ny = granules(fy, bytes);
+    uint8_t* to = ring.buf + slot * ring.bytes;
+    mbar_arrive_expect_tx(&ring.full[slot], nx + ny);
+    bulk_load(to, granule(fx), nx, &ring.full[slot]);
+    bulk_load(to + a.pitch, granule(fy), ny, &ring.full[slot]);
   };
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
     if (tid == 0) copy(i);
-  Columns<T, P, VEC, K> c;
-  c.init(a, tid * VEC, size);
-  bool in[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) in[k] = EXACT || (k * size + tid) * VEC < a.cols;
-  // the rows of an iteration overlap their reductions; a missing row is zeros
-  constexpr int R = 1;
-  float next_mean[R], next_rstd[R];
-  auto fetch = [&](long long row) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool here = row + r * step < a.rows;
-      next_mean[r] = here ? a.mean[row + r * step] : 0.f;
-      next_rstd[r] = here ? a.rstd[row + r * step] : 0.f;
+  int flip = 0, at = 0;
+  for (long long row = first; row < a.rows; row += step, flip ^= 1, at = (at + 1) & 31) {
+    if (at == 0) {
+      mean32 = next_mean32, rstd32 = next_rstd32;
+      fetch(row + 32 * step);
     }
-  };
-  fetch(first);
-  T* dx = static_cast<T*>(a.dx) + (a.dx ? first * a.lddx + tid * VEC : 0);
-  const long long next_dx = step * a.lddx;
-  int flip = 0;
-  for (long long row = first; row < a.rows; row += R * step, flip ^= 1, dx += R * next_dx) {
-    float mean[R], rstd[R];
-    Raw<T, VEC> rx[R][K], ry[R][K];
-    int slot[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool here = r == 0 || row + r * step < a.rows;
-      mean[r] = next_mean[r], rstd[r] = next_rstd[r];
-      slot[r] = ring.slot;
-      if (here) ring.wait(a.status);
-      const T* from = reinterpret_cast<const T*>(ring.at()) + tid * VEC;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        rx[r][k].load(from + k * size * VEC, here && in[k]);
-        ry[r][k].load(from + a.cols + k * size * VEC, here && in[k]);
-      }
-      if (here) ring.next();
-    }
-    fetch(row + R * step);
-    float2 s[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) s[r] = c.add(rx[r], ry[r], mean[r], rstd[r]);
-    if constexpr (R == 2) {
-      const float4 t = group_sum(make_float4(s[0].x, s[0].y, s[R - 1].x, s[R - 1].y), red[flip], size, group);
-      s[0] = make_float2(t.x, t.y), s[R - 1] = make_float2(t.z, t.w);
-    } else {
-      const float4 t = group_sum(make_float4(s[0].x, s[0].y, 0.f, 0.f), red[flip], size, group);
-      s[0] = make_float2(t.x, t.y);
-    }
-    // the reduction is behind every thread's reads of the buffers
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (fill < a.rows && (r == 0 || row + r * step < a.rows)) {
-        if (tid == 0) copy(slot[r]);
-        fill += step;
-      }
-    if (a.dx) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (r == 0 || row + r * step < a.rows)
-          c.write(rx[r], ry[r], in, dx + r * next_dx, size, mean[r], rstd[r], s[r].x * a.inv_cols, s[r].y * a.inv_cols);
-    }
+    const float mean = __shfl_sync(0xffffffffu, mean32, at), rstd = __shfl_sync(0xffffffffu, rstd32, at);
+    ring.wait(a.status);
+    const uint8_t* from = ring.buf + ring.slot * ring.bytes;
+    Held<T, VEC, N> hx, hy;
+    hx.template load<EXACT>(reinterpret_cast<const T*>(from + (VEC > 1 ? 0 : shift(x + row * a.ldx))), tid, size, a.cols);
+    hy.template load<EXACT>(reinterpret_cast<const T*>(from + a.pitch + (VEC > 1 ? 0 : shift(dy + row * a.lddy))), tid, size, a.cols);
+    const float2 s = group_sum(c.add(hx, hy, mean, rstd), red[flip], size, group);
+    // the reduction is behind every thread's reads of the buffer
+    if (tid == 0 && fill < a.rows) copy(ring.slot);
+    fill += step;
+    ring.next();
+    if (a.dx)
+      c.template write<EXACT>(hx, hy, static_cast<T*>(a.dx) + row * a.lddx, tid, size, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
-  if (tid == 0) ring.drain((fill - first) / step);
+  if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
   grid_dependents_launch();
   __syncthreads();  // the buffers are free: they take the groups' sums
   c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
@@ -546,29 +530,31 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
 
 // Long rows, first pass: a block per row, its mean, rstd and two sums to `stats`.
 template <typename T, typename P, int VEC>
-__global__ void __launch_bounds__(1024) ln_row_sums(const LnArgs a) {
+__global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
+  constexpr int N = VEC > 1 ? VEC : 2;
   __shared__ float2 red[2][32];
   int flip = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
     const float mean = a.mean[row], rstd = a.rstd[row];
-    float2 s = make_float2(0.f, 0.f);
+    uint64_t s1 = 0, s2 = 0;
+    const uint64_t m = twice(-mean), r = twice(rstd);
 #pragma unroll 2
-    for (int col = threadIdx.x * VEC; col < a.cols; col += 1024 * VEC) {
-      Raw<T, VEC> rx, ry;
-      rx.load(x + col, true);
-      ry.load(dy + col, true);
-      float g[VEC];
-      load_param<P, VEC>(a.gamma, col, true, 1.f, g);
+    for (int c = 0; c < a.cols; c += 512 * N) {
+      Held<T, VEC, N> hx, hy;
+      hx.template load<false>(x + c, threadIdx.x, 512, a.cols - c);
+      hy.template load<false>(dy + c, threadIdx.x, 512, a.cols - c);
+      uint64_t g[N / 2];
+      load_params<P, VEC, N>(a.gamma, 1.f, c + threadIdx.x * VEC, 512, a.cols, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float w = ry.get(i) * g[i];
-        s.x += w;
-        s.y = fmaf(w, (rx.get(i) - mean) * rstd, s.y);
+      for (int p = 0; p < N / 2; ++p) {
+        const uint64_t w = mul2(hy.pair(p), g[p]);
+        s1 = add2(s1, w);
+        s2 = fma2(w, mul2(add2(hx.pair(p), m), r), s2);
       }
     }
-    s = group_sum(s, red[flip], 1024, 0);
+    const float2 s = group_sum(make_float2(sum_of(s1), sum_of(s2)), red[flip], 512, 0);
     if (threadIdx.x == 0) a.stats[row] = make_float4(mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
 }
@@ -578,38 +564,36 @@ __global__ void __launch_bounds__(1024) ln_row_sums(const LnArgs a) {
 constexpr int kSlabThreads = 256, kSlabRows = 4;
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
-  const int col0 = blockIdx.y * kSlabThreads * VEC, col = col0 + threadIdx.x * VEC;
-  const bool in = col < a.cols, mine[1] = {in};
-  Columns<T, P, VEC, 1> c;
-  c.init(a, col, kSlabThreads);
+  constexpr int N = VEC > 1 ? VEC : 2;
+  const int col0 = blockIdx.y * kSlabThreads * N, tid = threadIdx.x, cols = a.cols - col0;
+  Columns<T, P, VEC, N> c;
+  c.init(a, col0 + tid * VEC, kSlabThreads);
   for (long long row0 = (long long)blockIdx.x * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.x * kSlabRows) {
-    Raw<T, VEC> rx[kSlabRows][1], ry[kSlabRows][1];
+    Held<T, VEC, N> x[kSlabRows], y[kSlabRows];
     float4 st[kSlabRows];
 #pragma unroll
     for (int r = 0; r < kSlabRows; ++r) {
       const long long row = row0 + r;
       const bool here = row < a.rows;
-      rx[r][0].load(static_cast<const T*>(a.x) + row * a.ldx + col, in && here);
-      ry[r][0].load(static_cast<const T*>(a.dy) + row * a.lddy + col, in && here);
+      x[r].template load<false>(static_cast<const T*>(a.x) + row * a.ldx + col0, tid, kSlabThreads, cols, here);
+      y[r].template load<false>(static_cast<const T*>(a.dy) + row * a.lddy + col0, tid, kSlabThreads, cols, here);
       st[r] = here ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int r = 0; r < kSlabRows; ++r) {
       if (row0 + r >= a.rows) break;
-      c.add(rx[r], ry[r], st[r].x, st[r].y);
-      if (a.dx) c.write(rx[r], ry[r], mine, static_cast<T*>(a.dx) + (row0 + r) * a.lddx + col, kSlabThreads, st[r].x, st[r].y, st[r].z, st[r].w);
+      c.add(x[r], y[r], st[r].x, st[r].y);
+      if (a.dx)
+        c.template write<false>(x[r], y[r], static_cast<T*>(a.dx) + (row0 + r) * a.lddx + col0, tid, kSlabThreads, cols, st[r].x, st[r].y, st[r].z,
+                                st[r].w);
     }
   }
-  if (!in) return;
-  float* part = a.part + (long long)blockIdx.x * 2 * a.cols + col;
+  float* part = a.part + (long long)blockIdx.x * 2 * a.cols + col0;
 #pragma unroll
-  for (int i = 0; i < c.H; ++i) {
-    if constexpr (VEC > 1) {
-      const float2 g = unpair(c.dg[0][i]), b = unpair(c.db[0][i]);
-      part[2 * i] = g.x, part[2 * i + 1] = g.y, part[a.cols + 2 * i] = b.x, part[a.cols + 2 * i + 1] = b.y;
-    } else {
-      part[0] = c.dg[0][i], part[a.cols] = c.db[0][i];
-    }
+  for (int v = 0; v < N; ++v) {
+    const int col = (v / VEC * kSlabThreads + tid) * VEC + v % VEC;
+    const float2 g = unpair(c.dg[v / 2]), b = unpair(c.db[v / 2]);
+    if (col < cols) part[col] = v & 1 ? g.y : g.x, part[a.cols + col] = v & 1 ? b.y : b.x;
   }
 }
 
@@ -640,19 +624,22 @@ __global__ void __launch_bounds__(1024) ln_column_sums(const float* part, int pa
 
 // ---------------------------------------------------------------- host side
 struct LnPlan {
-  int vec;      // elements per access: 16 bytes of the row's type, or 1
-  int k;        // vectors per thread; 0: the long-row kernels
+  int vec;      // values per access: 16 bytes of the row's type, or 1
+  int n;        // values per thread; 0: the long-row kernels
   int size;     // threads per row
   int threads;  // per block
   bool ring;    // rows through shared memory
   int slots;    // row buffers per group
+  uint32_t pitch;
   size_t smem;
 };
 
 constexpr int kHeld = 8192;  // values of a row that the backward kernels hold at once
+constexpr int kRingBytes = 128 * 1024;  // copies in flight per SM; more only lengthens the queue for all loads
+constexpr int kSharedMax = 225 * 1024;
 
 // 16-byte accesses need every row of every tensor to start on a 16-byte boundary and
-// to end on one; other rows go element by element.
+// to end on one; other rows go value by value.
 LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   const int es = d.dtype == PKT_DTYPE_BF16 ? 2 : 4;
   auto rows_ok = [&](const void* p, long long ld) { return aligned_to(p, 16) && ld * es % 16 == 0; };
@@ -663,61 +650,47 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
     wide = wide && rows_ok(d.y, d.ldy) && aligned_to(d.beta, 16);
   LnPlan p{};
   p.vec = wide ? 16 / es : 1;
-  const int nvec = d.cols / p.vec;
-  auto sums_bytes = [](const LnPlan& q) { return size_t(512) * 2 * q.k * q.vec * sizeof(float); };
-  auto threads_for = [&](int k, int most) {
-    int t = 32;
-    while (t < most && (long long)t * k < nvec) t *= 2;
-    return t;
+  auto fit = [&](int n, int most) {  // threads that hold a row with n values each
+    p.n = n, p.size = 32;
+    while (p.size < most && (long long)p.size * n < d.cols) p.size *= 2;
+    return (long long)p.size * n >= d.cols;
   };
-  auto choose = [&](const int* ks, int count, int most) {  // the fewest vectors per thread that fit
-    for (int i = 0; i < count; ++i) {
-      p.k = ks[i], p.size = threads_for(ks[i], most);
-      if ((long long)p.size * p.k >= nvec) return true;
-    }
-    p.k = 0, p.size = p.threads = 1024;
-    return false;
-  };
-  if (!wide) {
-    const int few[3] = {1, 8, 16}, many[2] = {8, 16};
-    const bool lots = d.rows >= 2LL * sms;
-    if (backward ? choose(many, 2, 512) : lots ? choose(many, 2, 1024) : choose(few, 3, 1024)) {
-      p.threads = backward ? 512 : std::max(p.size, 32 * kWarpsPerBlock);
-      if (backward) p.smem = sums_bytes(p);
-    }
-    return p;
-  }
-  // The ring pays from a few rows per group on; up to 32 values per thread in the forward
-  // pass, 16 in the backward pass (three more registers each), in as few threads as hold
-  // the row.
-  const int ks[3] = {1, 2, 16 / p.vec};
-  p.k = (backward ? 16 : 32) / p.vec;
-  while (p.k > 1 && 32 * (p.k / 2) >= nvec) p.k /= 2;
-  p.size = threads_for(p.k, kRingThreads);
-  if ((long long)p.size * p.k >= nvec) {
-    const long long groups = (long long)sms * (kRingThreads / p.size);
-    const size_t stage = size_t(kRingThreads / p.size) * d.cols * es * (backward ? 2 : 1);
-    const size_t params = backward ? 0 : 8 * size_t(d.cols);
-    p.slots = int(std::min<size_t>(kMaxSlots, (200 * 1024 - params) / stage));
-    if (d.rows >= 2 * groups && p.slots >= 3) {
+  // The ring pays from a few rows per group on: up to 32 values per thread in the
+  // forward pass (16 one by one), 16 in the backward pass (three more registers each; 8
+  // one by one while they hold the row), in as few threads as hold the row.
+  const int most = wide && !backward ? 32 : backward && !wide && d.cols <= 8 * kRingThreads ? 8 : 16, least = wide ? p.vec : 8;
+  for (int n = most; n >= least; n /= 2)
+    if (n == most || 32 * n >= d.cols) fit(n, kRingThreads);
+  if ((long long)p.size * p.n >= d.cols) {
+    const int groups = kRingThreads / p.size;
+    p.pitch = (uint32_t(d.cols) * es + (wide ? 15 : 30)) & ~15u;
+    const size_t stage = size_t(groups) * p.pitch * (backward ? 2 : 1), params = backward ? 0 : 8 * size_t((d.cols + 3) & ~3);
+    p.slots = int(std::min<size_t>(kMaxSlots, std::max<size_t>(kRingBytes / stage, backward ? 3 : 4)));  // (forward: two rows in use)
+    p.smem = p.slots * stage + params;
+    if (backward) p.smem = std::max(p.smem, size_t(kRingThreads) * 2 * p.n * sizeof(float));
+    if (d.rows >= 2LL * sms * groups && p.smem <= kSharedMax) {
       p.ring = true;
       p.threads = kRingThreads;
-      p.smem = std::max(p.slots * stage + params, backward ? sums_bytes(p) : size_t(0));
       return p;
     }
   }
+  p.smem = 0;
   if (backward) {
-    if (choose(ks, 3, 512)) p.threads = 512, p.smem = sums_bytes(p);
+    // few rows: threads first, then values per thread
+    if (!(fit(8, 512) || fit(16, 512))) p.n = 0;
+    p.threads = 512;
+    p.smem = size_t(512) * 2 * p.n * sizeof(float);
   } else {
-    const int direct[3] = {1, 2, 4};
-    if (choose(direct, 3, 1024)) p.threads = std::max(p.size, 32 * kWarpsPerBlock);
+    const int few = wide ? p.vec : 2;
+    if (!(fit(few, 1024) || fit(8, 1024) || fit(16, 1024))) p.n = 0;
+    p.threads = std::max(p.size, 128);
   }
   return p;
 }
 
 // Blocks along the rows in the backward pass, each with one partial row of column
-// sums: two per SM. (From the sizes alone: the workspace is asked for before the
-// pointers are known.)
+// sums: at most two per SM. (From the sizes alone: the workspace is asked for before
+// the pointers are known.)
 int ln_parts(long long rows, int sms) { return int(std::max(1LL, std::min(rows, 2LL * sms))); }
 // The partial rows, then (long rows) 4 values per row.
 size_t ln_part_floats(const pkt_layernorm_desc* d, int sms) { return (size_t(ln_parts(d->rows, sms)) * 2 * d->cols + 3) / 4 * 4; }
@@ -725,68 +698,63 @@ size_t ln_workspace(const pkt_layernorm_desc* d, int sms) {
   return (ln_part_floats(d, sms) + (d->cols > kHeld ? size_t(d->rows) * 4 : 0)) * sizeof(float);
 }
 
+unsigned ln_blocks(long long n) { return unsigned(std::min(n, 1LL << 30)); }
+
 template <typename... KArgs>
-int ln_launch_shared(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, int blocks, cudaStream_t st) {
-  const int rc = op_shared_memory(reinterpret_cast<const void*>(kernel), done, dev, 200 * 1024);
+int ln_launch(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, unsigned blocks, cudaStream_t st) {
+  const int rc = done ? op_shared_memory(reinterpret_cast<const void*>(kernel), done, dev, kSharedMax) : PKT_OK;
   if (rc) return rc;
   const cudaError_t e = op_launch(kernel, dim3(blocks), dim3(p.threads), p.smem, st, false, a);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
 }
 
-// The partial rows that a backward kernel wrote (as a positive result).
-template <typename T, typename P, int VEC, int K, bool EXACT>
-int ln_run_ring(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
-  static std::atomic<uint64_t> done[2];
-  if (!backward) return ln_launch_shared(ln_forward_ring<T, P, VEC, K, EXACT>, &done[1], dev, a, p, sms, st);
-  if constexpr (K * VEC <= 16) {
-    const int blocks = std::min(a.parts, sms), rc = ln_launch_shared(ln_backward_ring<T, P, VEC, K, EXACT>, &done[0], dev, a, p, blocks, st);
+// The launches of one plan. In the backward direction the result is the number of
+// partial rows written.
+template <typename T, typename P, int VEC, int N>
+int ln_run(const LnArgs& a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
+  static std::atomic<uint64_t> done[5];
+  const bool exact = a.cols == p.size * N;
+  if (!backward) {
+    if constexpr (N >= 8) {
+      if (p.ring && VEC > 1 && exact) return ln_launch(ln_forward_ring<T, P, VEC, N, VEC != 1>, &done[0], dev, a, p, sms, st);
+      if (p.ring) return ln_launch(ln_forward_ring<T, P, VEC, N, false>, &done[1], dev, a, p, sms, st);
+    }
+    if constexpr (N <= 16) return ln_launch(ln_forward<T, P, VEC, N>, nullptr, dev, a, p, ln_blocks((a.rows - 1) / (p.threads / p.size) + 1), st);
+  } else if constexpr (N == 8 || N == 16) {
+    int blocks = std::min(a.parts, sms), rc;
+    if (p.ring && VEC > 1 && exact) {
+      rc = ln_launch(ln_backward_ring<T, P, VEC, N, VEC != 1>, &done[2], dev, a, p, blocks, st);
+    } else if (p.ring) {
+      rc = ln_launch(ln_backward_ring<T, P, VEC, N, false>, &done[3], dev, a, p, blocks, st);
+    } else {
+      blocks = int(std::min<long long>(a.parts, (a.rows - 1) / (p.threads / p.size) + 1));
+      rc = ln_launch(ln_backward<T, P, VEC, N>, &done[4], dev, a, p, blocks, st);
+    }
     return rc ? rc : blocks;
   }
   return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
 }
 
-template <typename T, typename P, int VEC, int K>
-int ln_run(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
-  if constexpr (VEC > 1) {
-    if (p.ring)
-      return a.cols == p.size * K * VEC ? ln_run_ring<T, P, VEC, K, true>(a, p, backward, dev, sms, st)
-                                        : ln_run_ring<T, P, VEC, K, false>(a, p, backward, dev, sms, st);
-  }
-  if constexpr (VEC == 1 || K <= 4) {
+template <typename T, typename P, int VEC>
+int ln_pick(const LnArgs& a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
+  if (p.n == 0) {
     if (!backward) {
-      const long long blocks = (a.rows - 1) / (p.threads / p.size) + 1;
-      const cudaError_t e = op_launch(ln_forward<T, P, VEC, K>, dim3(unsigned(std::min(blocks, 1LL << 30))), dim3(p.threads), 0, st, false, a);
+      const cudaError_t e = op_launch(ln_forward_long<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(1024), 0, st, false, a);
       return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
     }
+    const int slabs = (a.cols - 1) / (kSlabThreads * (VEC > 1 ? VEC : 2)) + 1;
+    const long long want = std::max(1LL, 8LL * sms / slabs);  // about 8 blocks of 256 threads per SM
+    const int rows = int(std::min<long long>({want, a.parts, (a.rows - 1) / kSlabRows + 1}));
+    cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(512), 0, st, false, a);
+    if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(rows, slabs), dim3(kSlabThreads), 0, st, false, a);
+    return e == cudaSuccess ? rows : cuda_fail(e, "launch layer norm");
   }
-  if constexpr (K * VEC <= 16 && !(VEC == 1 && K < 8)) {
-    static std::atomic<uint64_t> done;
-    const int rc = ln_launch_shared(ln_backward<T, P, VEC, K>, &done, dev, a, p, a.parts, st);
-    return rc ? rc : a.parts;
-  }
-  return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
-}
-
-template <typename T, typename P, int VEC>
-int ln_pick(LnArgs a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
-  switch (p.k) {
-    case 0: {
-      if (!backward) {
-        const cudaError_t e = op_launch(ln_forward_long<T, P, VEC>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(1024), 0, st, false, a);
-        return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
-      }
-      const int slabs = (a.cols - 1) / (kSlabThreads * VEC) + 1;
-      const long long want = std::max(1LL, 8LL * sms / slabs);  // about 8 blocks of 256 threads per SM
-      const int rows = int(std::min<long long>({want, a.parts, (a.rows - 1) / kSlabRows + 1}));
-      cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(unsigned(std::min(a.rows, 1LL << 30))), dim3(1024), 0, st, false, a);
-      if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(rows, slabs), dim3(kSlabThreads), 0, st, false, a);
-      return e == cudaSuccess ? rows : cuda_fail(e, "launch layer norm");
-    }
-    case 1: return ln_run<T, P, VEC, 1>(a, p, backward, dev, sms, st);
-    case 2: if constexpr (VEC > 1) return ln_run<T, P, VEC, 2>(a, p, backward, dev, sms, st); break;
-    case 4: if constexpr (VEC > 1) return ln_run<T, P, VEC, 4>(a, p, backward, dev, sms, st); break;
-    case 8: if constexpr (VEC != 8) return ln_run<T, P, VEC, 8>(a, p, backward, dev, sms, st); break;
-    case 16: if constexpr (VEC == 1) return ln_run<T, P, 1, 16>(a, p, backward, dev, sms, st); break;
+  switch (p.n) {
+    case 2: if constexpr (VEC == 1) return ln_run<T, P, VEC, 2>(a, p, backward, dev, sms, st); break;
+    case 4: if constexpr (VEC == 4) return ln_run<T, P, VEC, 4>(a, p, backward, dev, sms, st); break;
+    case 8: return ln_run<T, P, VEC, 8>(a, p, backward, dev, sms, st);
+    case 16: return ln_run<T, P, VEC, 16>(a, p, backward, dev, sms, st);
+    case 32: if constexpr (VEC > 1) return ln_run<T, P, VEC, 32>(a, p, backward, dev, sms, st); break;
   }
   return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", a.cols);
 }
@@ -802,6 +770,7 @@ int ln_dispatch(const LnArgs& a, const LnPlan& p, int param_dtype, bool backward
 int ln_check_common(const pkt_layernorm_desc* d) {
   if (!d) return fail(PKT_ERR_ARGS, "null layer norm descriptor");
   if (d->rows < 0 || d->cols <= 0) return fail(PKT_ERR_ARGS, "layer norm of %lld rows x %d columns", d->rows, d->cols);
+  if (d->cols > (1 << 29)) return fail(PKT_ERR_UNSUPPORTED, "layer norm of %d columns", d->cols);
   if (d->dtype != PKT_DTYPE_BF16 && d->dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "layer norm dtype must be bf16 or f32");
   if (d->param_dtype != PKT_DTYPE_BF16 && d->param_dtype != PKT_DTYPE_F32)
     return fail(PKT_ERR_ARGS, "layer norm param_dtype must be bf16 or f32");
@@ -822,7 +791,7 @@ int ln_check_param(const void* p, const char* what, int dtype) {
 
 LnArgs ln_args(const pkt_layernorm_desc& d, const LnPlan& p, int* status) {
   LnArgs a{};
-  a.size = p.size, a.slots = p.slots, a.status = status;
+  a.size = p.size, a.slots = p.slots, a.pitch = p.pitch, a.status = status;
   a.rows = d.rows, a.cols = d.cols, a.eps = d.eps, a.inv_cols = 1.f / float(d.cols);
   a.x = d.x, a.gamma = d.gamma, a.beta = d.beta, a.dy = d.dy, a.y = d.y, a.dx = d.dx;
   a.ldx = d.ldx, a.ldy = d.ldy, a.lddy = d.lddy, a.lddx = d.lddx;
@@ -905,10 +874,9 @@ int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
   rc = d->dtype == PKT_DTYPE_BF16 ? ln_dispatch<bf16_t>(a, p, d->param_dtype, true, dev, sms, st)
                                   : ln_dispatch<float>(a, p, d->param_dtype, true, dev, sms, st);
   if (rc < 0) return rc;
-  a.parts = rc;
   if (d->dgamma || d->dbeta) {
-    const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part),
-                                    a.parts, a.cols, d->dgamma, d->dbeta);
+    const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part), rc,
+                                    a.cols, d->dgamma, d->dbeta);
     if (e != cudaSuccess) return cuda_fail(e, "launch layer norm column sums");
   }
   return PKT_OK;
