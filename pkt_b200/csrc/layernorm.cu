@@ -249,14 +249,14 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   Ring ring = make_ring(ring_smem + 8 * (size_t)pcols, full, a, groups, group, a.pitch);
   const T* x = static_cast<const T*>(a.x);
   long long fill = first;  // the next row to copy
-  auto copy = [&](int slot) {
-    const T* from = x + fill * a.ldx;
+  auto copy = [&](int slot, long long row) {
+    const T* from = x + row * a.ldx;
     const uint32_t n = granules(from, bytes);
     mbar_arrive_expect_tx(&ring.full[slot], n);
     bulk_load(ring.buf + slot * ring.bytes, granule(from), n, &ring.full[slot]);
   };
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
-    if (tid == 0) copy(i);
+    if (tid == 0) copy(i, fill);
   T* y = static_cast<T*>(a.y) + first * a.ldy;
   const T* at = x + first * a.ldx;
   const long long next_y = step * a.ldy, next_x = step * a.ldx;
@@ -277,6 +277,12 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     for (int p = 0; p < N / 2; ++p) s0 = add2(s0, x0.pair(p)), s1 = add2(s1, x1.pair(p));
     const float2 sum = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[0], size, group);
     const float2 mean = make_float2(sum.x * a.inv_cols, sum.y * a.inv_cols);
+    // the reduction is behind every thread's reads of the buffers
+    if (tid == 0) {
+      if (fill < a.rows) copy(slot0, fill);
+      if (two && fill + step < a.rows) copy(slot1, fill + step);
+    }
+    fill += 2 * step;
     s0 = s1 = 0;
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) {
@@ -287,12 +293,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     }
     const float2 sq = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[1], size, group);
     const float2 rstd = make_float2(1.f / sqrtf(sq.x * a.inv_cols + a.eps), 1.f / sqrtf(sq.y * a.inv_cols + a.eps));
-    // the reductions are behind every thread's reads of the buffers
     if (tid == 0) {
-      if (fill < a.rows) copy(slot0);
-      fill += step;
-      if (two && fill < a.rows) copy(slot1);
-      fill += step;
       put_stats(a, row, mean.x, rstd.x);
       if (two) put_stats(a, row + step, mean.y, rstd.y);
     }
@@ -659,20 +660,20 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   // forward pass (16 one by one), 16 in the backward pass (three more registers each; 8
   // one by one while they hold the row), in as few threads as hold the row.
   const int most = wide && !backward ? 32 : backward && !wide && d.cols <= 8 * kRingThreads ? 8 : 16, least = wide ? p.vec : 8;
-  for (int n = most; n >= least; n /= 2)
-    if (n == most || 32 * n >= d.cols) fit(n, kRingThreads);
-  if ((long long)p.size * p.n >= d.cols) {
+  for (int n = most; n >= least; n /= 2) {
+    if (!fit(n, kRingThreads)) break;
+    if (p.size == 32 && 32 * (n / 2) >= d.cols && n / 2 >= least) continue;
     const int groups = kRingThreads / p.size;
     p.pitch = (uint32_t(d.cols) * es + (wide ? 15 : 30)) & ~15u;
     const size_t stage = size_t(groups) * p.pitch * (backward ? 2 : 1), params = backward ? 0 : 8 * size_t((d.cols + 3) & ~3);
-    p.slots = int(std::min<size_t>(kMaxSlots, std::max<size_t>(kRingBytes / stage, backward ? 3 : 4)));  // (forward: two rows in use)
+    p.slots = int(std::min<size_t>(kMaxSlots, std::max<size_t>(kRingBytes / stage, 3)));
     p.smem = p.slots * stage + params;
     if (backward) p.smem = std::max(p.smem, size_t(kRingThreads) * 2 * p.n * sizeof(float));
-    if (d.rows >= 2LL * sms * groups && p.smem <= kSharedMax) {
-      p.ring = true;
-      p.threads = kRingThreads;
-      return p;
-    }
+    if (p.smem > kSharedMax) continue;  // fewer values per thread: fewer groups, fewer buffers
+    p.ring = d.rows >= 2LL * sms * groups;
+    p.threads = kRingThreads;
+    if (p.ring) return p;
+    break;
   }
   p.smem = 0;
   if (backward) {
