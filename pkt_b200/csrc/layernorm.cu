@@ -666,10 +666,10 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
     const int groups = kRingThreads / p.size;
     p.pitch = (uint32_t(d.cols) * es + (wide ? 15 : 30)) & ~15u;
     const size_t stage = size_t(groups) * p.pitch * (backward ? 2 : 1), params = backward ? 0 : 8 * size_t((d.cols + 3) & ~3);
-    p.slots = int(std::min<size_t>(kMaxSlots, std::max<size_t>(kRingBytes / stage, 3)));
+    if (params + 3 * stage > kSharedMax) continue;  // fewer values per thread: fewer groups, fewer buffers
+    p.slots = int(std::min({size_t(kMaxSlots), std::max<size_t>(kRingBytes / stage, 3), (kSharedMax - params) / stage}));
     p.smem = p.slots * stage + params;
     if (backward) p.smem = std::max(p.smem, size_t(kRingThreads) * 2 * p.n * sizeof(float));
-    if (p.smem > kSharedMax) continue;  // fewer values per thread: fewer groups, fewer buffers
     p.ring = d.rows >= 2LL * sms * groups;
     p.threads = kRingThreads;
     if (p.ring) return p;
