@@ -6,7 +6,14 @@
 // block of K only: the MMA issuer writes each block's product to the next of
 // several TMEM buffers (4 MMAs of K = 32) and the epilogue warps read it back,
 // multiply by the block's scales and add to accumulators in their registers, while
-// the MMAs of the next blocks run. One fp32 FMA per output value and block of 128.
+// the MMAs of the next blocks run. One fp32 FMA per output value and block of 128, or a
+// product more where the columns have a scale each.
+//
+// A lane holds a row and all the warp's columns when the columns share a scale. When
+// they do not, it holds 4 rows and a quarter of the columns (TMEM loads of 16 lanes x
+// 256 bits): each lane then needs a quarter of the columns' scales, and it is their
+// delivery from shared memory, 128 bytes a cycle for all warps, that bounds this case
+// (8192 x 4096 x 4096: 215 us with a row per lane).
 //
 // Roles of a CTA: warps 0..3 (0..7) epilogue, one per 32 TMEM lanes (and half of the
 // columns); then one TMA producer warp, one MMA issuer warp and one that copies the
@@ -51,9 +58,11 @@ struct alignas(64) Fp8Args {
 
 template <int BN, int PAIR>
 struct Shape {
-  static constexpr int kHalves = BN > 128 ? 2 : 1;   // epilogue warps per 32 lanes
-  static constexpr int kCols = BN / kHalves;         // columns of an epilogue warp
-  static constexpr int kEpiWarps = 4 * kHalves;
+  static constexpr int kHalves = BN > 128 ? 2 : 1;   // MMA issuers, each with its part of the columns
+  static constexpr int kPart = BN / kHalves;         // columns of an issuer
+  static constexpr int kSides = BN > 64 ? 2 : 1;     // epilogue warps per 32 lanes
+  static constexpr int kCols = BN / kSides;          // columns of an epilogue warp
+  static constexpr int kEpiWarps = 4 * kSides;
   static constexpr int kThreads = 32 * (kEpiWarps + 4);
   static constexpr int kRowBytes = kRows * kKBytes;
   static constexpr int kColBytes = BN / PAIR * kKBytes;
@@ -165,6 +174,29 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
   return v;
 }
 
+// 16 lanes x 8 N columns: a thread gets, for each 8 columns, those at 2 (lane % 4) and
+// the next one, of rows lane / 4 and lane / 4 + 8.
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
 // Tiles in groups of 8 tile rows swept column by column: what runs at the same time
 // shares operand tiles in L2.
 __device__ __forceinline__ void tile_at(int t, int tiles_r, int tiles_c, int* tr, int* tc) {
@@ -217,7 +249,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
     for (int i = 0; i < S::kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], S::kHalves);
     for (int i = 0; i < S::kScales; ++i) mbar_init(&s.sfull[i], 32), mbar_init(&s.sempty[i], S::kEpiWarps);
     for (int h = 0; h < S::kHalves; ++h)
-      for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[h][i], 1), mbar_init(&s.tempty[h][i], 4 * PAIR);
+      for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[h][i], 1), mbar_init(&s.tempty[h][i], S::kEpiWarps / S::kHalves * PAIR);
     for (int h = 0; h < S::kHalves; ++h) mbar_init(&s.drain[h], 1);
     s.abort = 0;
     fence_mbar_init();
@@ -249,7 +281,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
     for (int t = first; ok && t < tiles; t += step) {
       int tr, tc;
       tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
-      const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (S::kCols / PAIR);
+      const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (S::kPart / PAIR);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = wait_phase(&s.empty[stage], phase ^ 1, a.status, &s.abort))) break;
         if (elect_one()) {
@@ -260,7 +292,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
             tma_load_2d_pair(to, &a.map_r, bar, kb * kKBytes, r0);
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)  // each half's columns come from both CTAs
-              tma_load_2d_pair(to + S::kRowBytes + h * (S::kColBytes / S::kHalves), &a.map_c, bar, kb * kKBytes, c0 + h * S::kCols);
+              tma_load_2d_pair(to + S::kRowBytes + h * (S::kColBytes / S::kHalves), &a.map_c, bar, kb * kKBytes, c0 + h * S::kPart);
           } else {
             tma_load_2d(to, &a.map_r, &s.full[stage], kb * kKBytes, r0);
             tma_load_2d(to + S::kRowBytes, &a.map_c, &s.full[stage], kb * kKBytes, c0);
@@ -295,7 +327,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
           if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[h][buf], bphase ^ 1, a.status, &s.abort);
           if (!ok) break;
           const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes + h * (S::kColBytes / S::kHalves);
-          const uint32_t to = tmem + (buf * S::kHalves + h) * S::kCols;
+          const uint32_t to = tmem + (buf * S::kHalves + h) * S::kPart;
           const uint32_t now = stage, nbuf = buf;
           if (++stage == S::kStages) stage = 0, phase ^= 1;
           if (++buf == S::kBufs) buf = 0, bphase ^= 1;
@@ -330,24 +362,31 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   } else if (warp < S::kEpiWarps) {
     // ---- epilogue
     if (S::kHalves == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int quad = warp & 3, side = warp >> 2;
+    const int quad = warp & 3, side = warp >> 2, part_h = side * S::kCols / S::kPart;
+    // where this lane's values lie in the warp's 32 rows: value v of chunk j
+    auto row_of = [&](int v) { return COLV ? v / (S::kChunk / 2) * 16 + (v >> 1 & 1) * 8 + (lane >> 2) : lane; };
+    auto col_of = [&](int j, int v) {
+      return j * S::kChunk + (COLV ? v % (S::kChunk / 2) / 4 * 8 + 2 * (lane & 3) + (v & 1) : v);
+    };
+    constexpr int R = COLV ? 4 : 1;  // rows of a lane
     uint32_t buf = 0, bphase = 0, slot = 0, sphase = 0;
     bool ok = true;
     for (int t = first; ok && t < tiles; t += step) {
       int tr, tc;
       tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
-      const int row = (tr * PAIR + int(half)) * kRows + quad * 32 + lane, col0 = tc * BN + side * S::kCols;
-      float acc[S::kCols];
+      const int row0 = (tr * PAIR + int(half)) * kRows + quad * 32, col0 = tc * BN + side * S::kCols;
+      uint64_t acc[S::kCols / 2];  // values 2 i and 2 i + 1
 #pragma unroll
-      for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
+      for (int i = 0; i < S::kCols / 2; ++i) acc[i] = 0;
       // the scales of a block are fetched while the block before it is added, and its
       // barrier is asked for
-      float next_r = 0.f, next_c = 1.f;
+      float next_r[R], next_c = 1.f;
       auto fetch = [&](int kb, uint32_t at, uint32_t ph) {
         const int in = (kb - kb0) % S::kGroup;
         if (in == 0 && !wait_phase(&s.sfull[at], ph, a.status, &s.abort)) return false;
-        next_r = s.row_scale[at][in][quad * 32 + lane];
-        if (!COLV) next_c = s.col_scale[at][in][side];
+#pragma unroll
+        for (int i = 0; i < R; ++i) next_r[i] = s.row_scale[at][in][quad * 32 + (COLV ? 8 * i + (lane >> 2) : lane)];
+        if (!COLV) next_c = s.col_scale[at][in][part_h];
         return true;
       };
       uint32_t ready = 0;
@@ -355,55 +394,64 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       for (int kb = kb0; ok && kb < kb1; ++kb) {
         const int in = (kb - kb0) % S::kGroup;
         const bool last = in == S::kGroup - 1 || kb == kb1 - 1;
-        const float scale = next_r * next_c;
-        const float* cs = &s.col_scale[slot][in][side * S::kCols];
-        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[side][buf], bphase, a.status, &s.abort);
+        float scale[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) scale[i] = next_r[i] * next_c;
+        const float* cs = &s.col_scale[slot][in][side * S::kCols + 2 * (lane & 3)];
+        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[part_h][buf], bphase, a.status, &s.abort);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t from = tmem + (buf * S::kHalves + side) * S::kCols + (uint32_t(quad * 32) << 16);
-        constexpr int kLoads = S::kCols / S::kChunk;
-        // the next load is in flight while one is added; with a scale per column the
-        // registers hold the chunk's scales instead, loaded under the TMEM load
-        uint32_t v[COLV ? 1 : 2][S::kChunk];
-        tmem_load(from, v[0]);
+        const uint32_t from = tmem + buf * BN + side * S::kCols + (uint32_t(quad * 32) << 16);
+        constexpr int kLoads = S::kCols / S::kChunk, kSplit = COLV ? 2 : 1, kRegs = S::kChunk / kSplit;
+        uint32_t v[2][kSplit][kRegs];  // the next load is in flight while one chunk is added
+        auto load = [&](int j) {
+          if constexpr (COLV) {
+            tmem_load16(from + j * S::kChunk, v[j & 1][0]);
+            tmem_load16(from + j * S::kChunk + (16u << 16), v[j & 1][kSplit - 1]);
+          } else {
+            tmem_load(from + j * S::kChunk, v[j & 1][0]);
+          }
+        };
+        load(0);
         if (kb + 1 < kb1) {
           const bool wrap = slot + 1 == S::kScales;
           ok = fetch(kb + 1, last ? (wrap ? 0 : slot + 1) : slot, last && wrap ? sphase ^ 1 : sphase);
         }
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-          float4 c[COLV ? S::kChunk / 4 : 1];
-          if (COLV) {
+          float2 c[COLV ? S::kChunk / 8 : 1];
+          if constexpr (COLV) {
 #pragma unroll
-            for (int i = 0; i < S::kChunk / 4; ++i) c[i] = *reinterpret_cast<const float4*>(cs + j * S::kChunk + 4 * i);
+            for (int i = 0; i < S::kChunk / 8; ++i) c[i] = *reinterpret_cast<const float2*>(cs + j * S::kChunk + 8 * i);
           }
-          uint32_t(&u)[S::kChunk] = v[COLV ? 0 : j & 1];
-          tmem_wait(u);
+#pragma unroll
+          for (int h = 0; h < kSplit; ++h) tmem_wait(v[j & 1][h]);
           if (j + 1 == kLoads) {  // all of the buffer is in registers
-            ready = peek_phase(&s.tfull[side][buf + 1 == S::kBufs ? 0 : buf + 1], buf + 1 == S::kBufs ? bphase ^ 1 : bphase);
+            ready = peek_phase(&s.tfull[part_h][buf + 1 == S::kBufs ? 0 : buf + 1], buf + 1 == S::kBufs ? bphase ^ 1 : bphase);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
               if (PAIR == 2 && half != 0)
-                arrive_peer(mapa_shared(smem_u32(&s.tempty[side][buf]), 0));
+                arrive_peer(mapa_shared(smem_u32(&s.tempty[part_h][buf]), 0));
               else
-                mbar_arrive(&s.tempty[side][buf]);
+                mbar_arrive(&s.tempty[part_h][buf]);
             }
-          } else if (!COLV) {
-            tmem_load(from + (j + 1) * S::kChunk, v[(j + 1) & 1]);
+          } else {
+            load(j + 1);
           }
 #pragma unroll
-          for (int i = 0; i < S::kChunk; ++i) {
-            const float p = __uint_as_float(u[i]);
-            float& to = acc[j * S::kChunk + i];
-            if (COLV) {
-              const float4& q = c[i / 4];
-              to = fmaf(p * (i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w), scale, to);
+          for (int i = 0; i < S::kChunk; i += 2) {
+            const float p0 = __uint_as_float(v[j & 1][i / kRegs][i % kRegs]), p1 = __uint_as_float(v[j & 1][i / kRegs][i % kRegs + 1]);
+            uint64_t& to = acc[(j * S::kChunk + i) / 2];
+            if constexpr (COLV) {
+              const float2 q = c[i % kRegs / 4];
+              const float r = scale[i / kRegs * 2 + (i >> 1 & 1)];
+              to = fma2(mul2(pair_of(p0, p1), pair_of(q.x, q.y)), pair_of(r, r), to);
             } else {
-              to = fmaf(p, scale, to);
+              const float2 f = unpair(to);
+              to = pair_of(fmaf(p0, scale[0], f.x), fmaf(p1, scale[0], f.y));
             }
           }
-          if (COLV && j + 1 < kLoads) tmem_load(from + (j + 1) * S::kChunk, v[0]);
         }
         if (last) {
           __syncwarp();
@@ -418,34 +466,51 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
         // bytes (the operand stages have all been consumed: the last block's product
         // has been read)
         float* sums = reinterpret_cast<float*>(s.stages);
-        const int at = quad * 32 + lane;
-        if (a.swap) {
 #pragma unroll
-          for (int i = 0; i < S::kCols; ++i) sums[(side * S::kCols + i) * kRows + at] = acc[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < S::kCols; i += 4)
-            *reinterpret_cast<float4*>(sums + at * (BN + 4) + side * S::kCols + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        for (int i = 0; i < S::kCols; i += 2) {
+          const int v = i % S::kChunk, r = quad * 32 + row_of(v), c = side * S::kCols + col_of(i / S::kChunk, v);
+          const float2 f = unpair(acc[i / 2]);
+          if (a.swap) {
+            sums[c * kRows + r] = f.x;
+            sums[(c + 1) * kRows + r] = f.y;
+          } else {
+            *reinterpret_cast<float2*>(sums + r * (BN + 4) + c) = f;
+          }
         }
       } else if (S::kStore && a.tma_out) {
         // 32 rows x 128 bytes at a time through swizzled shared memory
         uint8_t* to = s.staging[S::kStore ? warp : 0];
-        const int row0 = row - lane, per = a.out_bf16 ? 64 : 32;
+        const int per = a.out_bf16 ? 64 : 32;
 #pragma unroll
         for (int j = 0; j < S::kCols / 32; ++j) {
           if (!a.out_bf16 || (j & 1) == 0) {
             if (lane == 0) bulk_wait_read_all();  // the last store has left the staging
             __syncwarp();
           }
+          if constexpr (COLV) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            const float* v = acc + j * 32 + i;
-            if (a.out_bf16) {
-              *reinterpret_cast<uint4*>(to + lane * 128 + ((((j & 1) * 4 + i / 8) ^ (lane & 7)) << 4)) =
-                  make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-            } else {
-              *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4) ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
-              *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4 + 1) ^ (lane & 7)) << 4)) = make_float4(v[4], v[5], v[6], v[7]);
+            for (int i = 0; i < 32; i += 2) {
+              const int r = row_of(i), c = col_of(0, i);
+              const float2 f = unpair(acc[j * 16 + i / 2]);
+              if (a.out_bf16) {
+                const int at = (j & 1) * 64 + c * 2;
+                *reinterpret_cast<uint32_t*>(to + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15)) = pack_bf16x2(f.x, f.y);
+              } else {
+                *reinterpret_cast<float2*>(to + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4) = f;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              const uint64_t* v = acc + j * 16 + i / 2;
+              const float2 f0 = unpair(v[0]), f1 = unpair(v[1]), f2 = unpair(v[2]), f3 = unpair(v[3]);
+              if (a.out_bf16) {
+                *reinterpret_cast<uint4*>(to + lane * 128 + ((((j & 1) * 4 + i / 8) ^ (lane & 7)) << 4)) =
+                    make_uint4(pack_bf16x2(f0.x, f0.y), pack_bf16x2(f1.x, f1.y), pack_bf16x2(f2.x, f2.y), pack_bf16x2(f3.x, f3.y));
+              } else {
+                *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4) ^ (lane & 7)) << 4)) = make_float4(f0.x, f0.y, f1.x, f1.y);
+                *reinterpret_cast<float4*>(to + lane * 128 + (((i / 4 + 1) ^ (lane & 7)) << 4)) = make_float4(f2.x, f2.y, f3.x, f3.y);
+              }
             }
           }
           if (!a.out_bf16 || (j & 1) == 1) {
@@ -460,8 +525,12 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < S::kCols; ++i)
-          if (row < a.rows && col0 + i < a.cols) store_one(a, row, col0 + i, acc[i]);
+        for (int i = 0; i < S::kCols; i += 2) {
+          const int v = i % S::kChunk, r = row0 + row_of(v), c = col0 + col_of(i / S::kChunk, v);
+          const float2 f = unpair(acc[i / 2]);
+          if (r < a.rows && c < a.cols) store_one(a, r, c, f.x);
+          if (r < a.rows && c + 1 < a.cols) store_one(a, r, c + 1, f.y);
+        }
       }
     }
     if (S::kStore && a.tma_out && lane == 0) bulk_wait_all();
@@ -494,7 +563,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
               if (BN >= 32 || lane < BN) copy_word_async(&s.col_scale[slot][in][lane + i], pc + min(col, a.cols - 1), col < a.cols);
             }
           } else if (lane < S::kHalves) {
-            const int col = col0 + lane * S::kCols;
+            const int col = col0 + lane * S::kPart;
             copy_word_async(&s.col_scale[slot][in][lane], pc + (min(col, a.cols - 1) >> 7), col < a.cols);
           }
           if (in == S::kGroup - 1 || kb == kb1 - 1) {
