@@ -217,7 +217,7 @@ __device__ __forceinline__ void adam_blocks(const AdamArgs& a, const AdamTensor&
 }
 
 template <typename P, typename G, bool EIGHT>
-__global__ void __launch_bounds__(kAdamThreads) adam_step(const AdamArgs a) {
+__global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 2) adam_step(const AdamArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float lr = a.scales ? a.lr * a.scales[0] : a.lr;
   AdamStep u;
