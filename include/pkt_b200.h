@@ -492,6 +492,17 @@ int pkt_mlp_set_output_capture(pkt_mlp* m, int enabled);
  * (1/world_size turns the summed per-rank mean gradients into the global mean). */
 int pkt_mlp_grad_buffer(pkt_mlp* m, float** ptr, long long* count);
 int pkt_mlp_set_grad_scale(pkt_mlp* m, float scale);
+/* AdamW (pkt_adamw) in the place of SGD, in grad_mode 1: pkt_mlp_train and
+ * pkt_mlp_apply_update then update the fp32 masters (and their bf16 copies) with it,
+ * with the engine's lr and gradient scale; weight decay is for the weights, not the
+ * biases. Starts with empty states and step 0; cfg = NULL goes back to SGD.
+ * Synchronises the device. */
+typedef struct pkt_mlp_adamw {
+  double beta1, beta2, eps;
+  float weight_decay;
+  int state_dtype; /* PKT_DTYPE_F32 or PKT_DTYPE_E4M3 (8-bit states) */
+} pkt_mlp_adamw;
+int pkt_mlp_set_adamw(pkt_mlp* m, const pkt_mlp_adamw* cfg);
 int pkt_mlp_forward_backward(pkt_mlp* m, void* stream);
 int pkt_mlp_apply_update(pkt_mlp* m, void* stream);
 /* The same step as pkt_mlp_forward_backward in L launches (grad_mode 1), so the

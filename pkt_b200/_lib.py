@@ -94,6 +94,11 @@ class AdamWConfig(ctypes.Structure):
                 ("eps", ctypes.c_double), ("step", c_longlong)]
 
 
+class MlpAdamW(ctypes.Structure):
+    _fields_ = [("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", c_float), ("state_dtype", c_int)]
+
+
 _P = c_void_p
 _SIGS = {
     "pkt_last_error": ([], ctypes.c_char_p),
@@ -155,6 +160,7 @@ _SIGS = {
     "pkt_mlp_set_grad_scale": ([_P, c_float], c_int),
     "pkt_mlp_dp_handle": ([_P, _P], c_int),
     "pkt_mlp_dp_connect": ([_P, c_int, c_int, _P], c_int),
+    "pkt_mlp_set_adamw": ([_P, ctypes.POINTER(MlpAdamW)], c_int),
     "pkt_mlp_forward_backward": ([_P, _P], c_int),
     "pkt_mlp_apply_update": ([_P, _P], c_int),
     "pkt_mlp_backward_segments": ([_P, ctypes.POINTER(c_int)], c_int),

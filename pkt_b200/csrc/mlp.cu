@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <new>
 #include <vector>
 
 #include "../../include/pk/detail/internal.h"
@@ -139,6 +140,7 @@ struct Mlp {
 
   ~Mlp() {
     if (rt) cudaSetDevice(rt->device);
+    drop_adamw();
     auto F = [](void* p) { cudaFree(p); };
     for (int k = 0; k < 2; ++k) {
       F(Xs[k]);
@@ -208,6 +210,24 @@ struct Mlp {
 
   // Tile width of layer l's weight-gradient GEMM.
   int wgrad_bn(int l) const { return pick_bn(dims[l + 1], dims[l], true); }
+
+  // grad_mode 1: the update by AdamW (pkt_mlp_set_adamw) instead of SGD. It updates the
+  // masters of the current weight parity in place, so the parity stays.
+  pkt_adamw* adamw = nullptr;
+  void* adamw_state = nullptr;  // m, v and their scales of every tensor
+  void drop_adamw() {
+    if (adamw) pkt_adamw_destroy(adamw);
+    cudaFree(adamw_state);
+    adamw = nullptr;
+    adamw_state = nullptr;
+  }
+  int set_adamw(const pkt_mlp_adamw& c);
+  int update_weights(cudaStream_t st) {
+    if (adamw) return pkt_adamw_step(adamw, lr, grad_scale, nullptr, st);
+    const int rc = launch_list(d_update[parity], int(update[parity].size()), st);
+    if (rc == PKT_OK) parity ^= 1;
+    return rc;
+  }
 
   int alloc(void** p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, std::max<size_t>(bytes, 16));
@@ -1068,6 +1088,56 @@ int Mlp::launch_list(pkt_task* d, int n, cudaStream_t st) {
   return PKT_OK;
 }
 
+// One tensor per layer's weights (with their padded columns: values and gradients stay
+// zero there) and per bias; all states in one allocation.
+int Mlp::set_adamw(const pkt_mlp_adamw& c) {
+  drop_adamw();
+  const bool eight = c.state_dtype == PKT_DTYPE_E4M3;
+  if (!eight && c.state_dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "AdamW state_dtype must be f32 or e4m3");
+  std::vector<pkt_adamw_tensor> ts;
+  for (int l = 0; l < L; ++l) {
+    pkt_adamw_tensor t{};
+    t.param = Wmaster(l, parity);
+    t.grad = grads + dW_off[l];
+    t.copy_bf16 = bf ? Wbf[parity][l] : nullptr;
+    t.n = (long long)dims[l + 1] * ld[l];
+    t.weight_decay = c.weight_decay;
+    ts.push_back(t);
+    if (!has_bias) continue;
+    t = pkt_adamw_tensor{};
+    t.param = bias[l];
+    t.grad = grads + db_off[l];
+    t.n = dims[l + 1];
+    ts.push_back(t);
+  }
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  auto values = [&](const pkt_adamw_tensor& t) { return up(size_t(t.n) * (eight ? 1 : 4)); };
+  auto scales = [&](const pkt_adamw_tensor& t) { return eight ? up(size_t(t.n + 127) / 128 * 4) : size_t(0); };
+  size_t total = 0;
+  for (const pkt_adamw_tensor& t : ts) total += 2 * values(t) + 2 * scales(t);
+  int rc = alloc(&adamw_state, total);
+  if (rc) return rc;
+  uint8_t* at = static_cast<uint8_t*>(adamw_state);
+  auto take = [&](size_t n) {
+    uint8_t* p = n ? at : nullptr;
+    at += n;
+    return p;
+  };
+  for (pkt_adamw_tensor& t : ts) {
+    t.m = take(values(t));
+    t.v = take(values(t));
+    t.m_scale = reinterpret_cast<float*>(take(scales(t)));
+    t.v_scale = reinterpret_cast<float*>(take(scales(t)));
+  }
+  const pkt_adamw_config cfg{int(ts.size()), ts.data(), PKT_DTYPE_F32, PKT_DTYPE_F32, c.state_dtype, c.beta1, c.beta2, c.eps, 0};
+  rc = pkt_adamw_create(rt->device, &cfg, &adamw);
+  if (rc) {
+    adamw = nullptr;
+    drop_adamw();
+  }
+  return rc;
+}
+
 }  // namespace pkb
 
 using pkb::Mlp;
@@ -1251,10 +1321,11 @@ int pkt_mlp_train(pkt_mlp* h, int steps, void* stream) {
     if (rc) return rc;
     if (m->grad_mode == 2) m->dp_step++;
     if (m->grad_mode == 1) {
-      rc = m->launch_list(m->d_update[p], int(m->update[p].size()), st);
+      rc = m->update_weights(st);
       if (rc) return rc;
+    } else {
+      m->parity ^= 1;
     }
-    m->parity ^= 1;
     m->losses_enqueued++;
   }
   return PKT_OK;
@@ -1276,11 +1347,7 @@ int pkt_mlp_apply_update(pkt_mlp* h, void* stream) {
   Mlp* m = h->m;
   if (m->grad_mode != 1) return pkb::fail(PKT_ERR_ARGS, "apply_update needs grad_mode 1");
   cudaSetDevice(m->rt->device);
-  const int p = m->parity;
-  int rc = m->launch_list(m->d_update[p], int(m->update[p].size()), static_cast<cudaStream_t>(stream));
-  if (rc) return rc;
-  m->parity ^= 1;
-  return PKT_OK;
+  return m->update_weights(static_cast<cudaStream_t>(stream));
 }
 
 int pkt_mlp_backward_segments(pkt_mlp* h, int* count) {
@@ -1352,6 +1419,24 @@ int pkt_mlp_dp_connect(pkt_mlp* h, int rank, int world, const void* handles) {
   int rc = m->connect(rank, world, static_cast<const uint8_t*>(handles));
   if (rc) return rc;
   return rebuild(m);  // task lists depend on which tiles this rank owns
+}
+
+int pkt_mlp_set_adamw(pkt_mlp* h, const pkt_mlp_adamw* cfg) {
+  if (!h) return pkb::fail(PKT_ERR_ARGS, "null argument");
+  Mlp* m = h->m;
+  if (m->grad_mode != 1) return pkb::fail(PKT_ERR_ARGS, "AdamW needs the stored gradients of grad_mode 1");
+  cudaSetDevice(m->rt->device);
+  cudaError_t e = cudaDeviceSynchronize();  // no step uses the states that go
+  if (e != cudaSuccess) return pkb::cuda_fail(e, "sync");
+  if (!cfg) {
+    m->drop_adamw();
+    return PKT_OK;
+  }
+  try {
+    return m->set_adamw(*cfg);
+  } catch (const std::bad_alloc&) {
+    return pkb::fail(PKT_ERR_ARGS, "out of host memory");
+  }
 }
 
 int pkt_mlp_set_grad_scale(pkt_mlp* h, float scale) {

@@ -185,6 +185,17 @@ class MLP:
     def set_grad_scale(self, s):
         check(self._L.pkt_mlp_set_grad_scale(self._h, float(s)))
 
+    def set_adamw(self, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, state_dtype="f32"):
+        """AdamW instead of SGD for train() and apply_update() (grad_mode 1), from empty
+        states; state_dtype "f32" or "e4m3" (8-bit states)."""
+        cfg = _lib.MlpAdamW(float(beta1), float(beta2), float(eps), float(weight_decay),
+                            {"f32": _lib.PKT_DTYPE_F32, "e4m3": _lib.PKT_DTYPE_E4M3}[state_dtype])
+        check(self._L.pkt_mlp_set_adamw(self._h, ctypes.byref(cfg)))
+
+    def set_sgd(self):
+        """Back to SGD (after set_adamw)."""
+        check(self._L.pkt_mlp_set_adamw(self._h, None))
+
     def set_output_capture(self, on=True):
         check(self._L.pkt_mlp_set_output_capture(self._h, int(bool(on))))
 

@@ -1,0 +1,262 @@
+"""The operators together, as a training step uses them: the MLP engine under AdamW, and
+a normalised linear layer (norm -> 8-bit operands -> products -> gradients -> AdamW)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from tests._gpu import require_gpu, torch  # noqa: E402
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def pk():
+    require_gpu()
+    import pkt_b200
+    return pkt_b200
+
+
+def engine(pk, dims, batch, dtype, bias=True, seed=3, lr=1e-2):
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((batch, dims[0])).astype(np.float32)
+    t = rng.standard_normal((batch, dims[-1])).astype(np.float32)
+    Ws = [rng.uniform(-1, 1, (dims[i + 1], dims[i])).astype(np.float32) * np.float32(np.sqrt(6.0 / dims[i])) for i in range(len(dims) - 1)]
+    bs = [rng.uniform(-0.1, 0.1, dims[i + 1]).astype(np.float32) for i in range(len(dims) - 1)] if bias else None
+    m = pk.MLP(dims, batch, dtype=dtype, lr=lr, bias=bias, grad_mode=1)
+    m.set_params(Ws, bs)
+    m.load_batch(m.storage_array(x), m.storage_array(t))
+    return m
+
+
+def adamw64(p, g, m, v, t, lr, decay, b1=0.9, b2=0.999, eps=1e-8):
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    step = lr / (1 - b1 ** t) * m / (np.sqrt(v) / np.sqrt(1 - b2 ** t) + eps)
+    return p * (1 - lr * decay) - step, m, v
+
+
+@pytest.mark.parametrize("dtype,dims,bias", [("bf16", [256, 512, 128], True), ("tf32", [100, 300, 77, 10], True), ("bf16", [100, 72, 33], False)])
+def test_mlp_engine_under_adamw(pk, dtype, dims, bias):
+    """Each update against the 64-bit formula on the gradients that the engine reports.
+
+    A parameter carries 3 u |p| + 16 u |step| per update (9 fp32 operations, rounded
+    constants), and states that were computed in fp32 as long: 8 u per step of theirs."""
+    m = engine(pk, dims, 256, dtype, bias)
+    m.set_adamw(weight_decay=0.05)
+    W, b = m.get_params()
+    P = [x.astype(np.float64) for x in list(W) + (list(b) if bias else [])]
+    M, V = [np.zeros_like(x) for x in P], [np.zeros_like(x) for x in P]
+    steps = 4
+    for t in range(1, steps + 1):
+        m.forward_backward()
+        dW, db = m.get_grads()
+        m.apply_update()
+        G = [x.astype(np.float64) for x in list(dW) + (list(db) if bias else [])]
+        W, b = m.get_params()
+        got = list(W) + (list(b) if bias else [])
+        for i in range(len(P)):
+            before = P[i]
+            P[i], M[i], V[i] = adamw64(P[i], G[i], M[i], V[i], t, 1e-2, 0.05 if i < len(dims) - 1 else 0.0)
+            tol = t * (4 * U * np.abs(before) + (16 + 8 * t) * U * 1e-2 * 10)
+            assert np.all(np.abs(got[i] - P[i]) <= tol), (t, i, np.max(np.abs(got[i] - P[i]) / tol))
+    # the weights the next forward pass reads are the updated ones: the same loss as a fresh engine with them
+    m.reset_losses()
+    m.forward_backward()
+    other = engine(pk, dims, 256, dtype, bias)
+    other.set_params(W, b if bias else None)
+    other.forward_backward()
+    assert m.losses()[0] == other.losses()[0]
+    m.close(), other.close()
+
+
+def test_mlp_engine_switches_optimizers(pk):
+    """train() under 8-bit AdamW moves the weights; SGD afterwards is SGD from where they are."""
+    dims = [256, 256, 64]
+    m = engine(pk, dims, 256, "bf16")
+    m.train(3)                      # SGD, an odd number of parity flips
+    m.set_adamw(state_dtype="e4m3")
+    m.train(3)
+    W, b = m.get_params()
+    assert len(m.losses()) == 6
+    m.set_sgd()
+    ref = engine(pk, dims, 256, "bf16")
+    ref.set_params(W, b)
+    m.train(2)
+    ref.train(2)
+    for x, y in zip(m.get_params(), ref.get_params()):
+        for p, q in zip(x, y):
+            assert np.array_equal(p, q)
+    m.close(), ref.close()
+
+
+def test_mlp_engine_refuses_adamw_without_gradients(pk):
+    m = pk.MLP([64, 64], 128, grad_mode=0)
+    with pytest.raises(pk.PktError, match="grad_mode 1"):
+        m.set_adamw()
+    m = engine(pk, [64, 64], 128, "bf16")
+    with pytest.raises(pk.PktError, match="betas"):
+        m.set_adamw(beta1=1.5)
+    m.train(1)  # SGD as before
+    assert len(m.losses()) == 1
+
+
+# ---------------------------------------------------------------- a normalised linear layer
+def q8(pk, x, block_rows, plain=True, transposed=False):
+    """(q, scale), (qt, scale_t) of a contiguous matrix."""
+    rows, cols = x.shape
+    up = lambda n: -(-n // 16) * 16  # noqa: E731
+    q = torch.zeros(rows, up(cols), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.zeros(-(-cols // 128), -(-rows // block_rows), device="cuda")
+    qt = torch.zeros(cols, up(rows), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    st = torch.zeros(-(-rows // 128), -(-cols // block_rows), device="cuda")
+    d = pk.Fp8QuantizeDesc(rows=rows, cols=cols, dtype=pk.DTYPE_BF16 if x.dtype == torch.bfloat16 else pk.DTYPE_F32, q_dtype=pk.DTYPE_E4M3,
+                           block_rows=block_rows, x=x.data_ptr(), ldx=x.stride(0))
+    if plain:
+        d.q, d.ldq, d.scale, d.ld_scale = q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0)
+    if transposed:
+        d.qt, d.ldqt, d.scale_t, d.ld_scale_t = qt.data_ptr(), qt.stride(0), st.data_ptr(), st.stride(0)
+    pk.fp8_quantize(d, torch.cuda.current_stream().cuda_stream)
+    return (q, s), (qt, st)
+
+
+def product(pk, a, b, a_rows, b_rows, M, N, K, out):
+    (qa, sa), (qb, sb) = a, b
+    C = torch.empty(M, N, dtype=out, device="cuda")
+    pk.fp8_gemm(pk.Fp8GemmDesc(M=M, N=N, K=K, a_dtype=pk.DTYPE_E4M3, b_dtype=pk.DTYPE_E4M3, a=qa.data_ptr(), lda=qa.stride(0), scale_a=sa.data_ptr(),
+                               ld_scale_a=sa.stride(0), a_block_rows=a_rows, b=qb.data_ptr(), ldb=qb.stride(0), scale_b=sb.data_ptr(),
+                               ld_scale_b=sb.stride(0), b_block_rows=b_rows, out=C.data_ptr(), ldo=N,
+                               out_dtype=pk.DTYPE_BF16 if out == torch.bfloat16 else pk.DTYPE_F32), torch.cuda.current_stream().cuda_stream)
+    return C
+
+
+def layer_step(pk, x, dy, W, gamma, beta):
+    """Forward and backward of y = norm(x) W^T with 8-bit products; returns y, dx, dW, dgamma, dbeta and the stored h."""
+    st = torch.cuda.current_stream().cuda_stream
+    rows, k = x.shape
+    n = W.shape[0]
+    h, dh, dx = torch.empty_like(x), None, torch.empty_like(x)
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    dgamma, dbeta = torch.empty(k, device="cuda"), torch.empty(k, device="cuda")
+    d = pk.LayerNormDesc(rows=rows, cols=k, dtype=pk.DTYPE_BF16, param_dtype=pk.DTYPE_F32, eps=1e-5, x=x.data_ptr(), ldx=k, gamma=gamma.data_ptr(),
+                         beta=beta.data_ptr(), y=h.data_ptr(), ldy=k, mean=mean.data_ptr(), rstd=rstd.data_ptr())
+    pk.layernorm_forward(d, st)
+    hq, hqt = q8(pk, h, 1, True, True)
+    wq, wqt = q8(pk, W, 128, True, True)
+    y = product(pk, hq, wq, 1, 128, rows, n, k, torch.bfloat16)
+    dq, dqt = q8(pk, dy, 1, True, True)
+    dh = product(pk, dq, wqt, 1, 128, rows, k, n, torch.bfloat16)
+    dW = product(pk, dqt, hqt, 1, 1, n, k, rows, torch.float32)
+    work = torch.empty(pk.layernorm_backward_workspace(d), dtype=torch.uint8, device="cuda")
+    d.dy, d.lddy, d.dx, d.lddx = dh.data_ptr(), k, dx.data_ptr(), k
+    d.dgamma, d.dbeta, d.workspace, d.workspace_bytes = dgamma.data_ptr(), dbeta.data_ptr(), work.data_ptr(), work.numel()
+    pk.layernorm_backward(d, st)
+    return y, dx, dW, dgamma, dbeta, h, dh, work
+
+
+@pytest.mark.parametrize("rows,k,n", [(256, 512, 384), (333, 200, 130)])
+def test_normalised_linear_layer(pk, rows, k, n):
+    """Every result against 64 bits. Quantising moves a value by at most 2^-4 of itself, or
+    (below the type's normal range) by 2^-10 of its block's scale, 2^-18 of the block's
+    largest value; a product of two is off by 2 2^-4 + 2^-8 of sum |a b|, rounded up to
+    2 2^-4 + 2^-7 for the small values, plus the result's own rounding. The norm's backward
+    pass starts from the stored dh: its sums carry 2^-14 at most (test_layernorm_gpu)."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, k, generator=g, device="cuda") * 2 + 0.5).bfloat16()
+    dy = (torch.randn(rows, n, generator=g, device="cuda") * 1e-2).bfloat16()
+    W = torch.randn(n, k, generator=g, device="cuda") * k ** -0.5
+    gamma = 1 + 0.1 * torch.randn(k, generator=g, device="cuda")
+    beta = 0.1 * torch.randn(k, generator=g, device="cuda")
+    y, dx, dW, dgamma, dbeta, h, dh, _ = layer_step(pk, x, dy, W, gamma, beta)
+    torch.cuda.synchronize()
+    assert pk.ops_status() == 0
+
+    def near(got, a, b):
+        want, mag = a @ b.t(), a.abs() @ b.abs().t()
+        assert torch.all((got.double() - want).abs() <= (2 * 2.0 ** -4 + 2.0 ** -7) * mag + 2.0 ** -8 * want.abs())
+
+    near(y, h.double(), W.double())
+    near(dh, dy.double(), W.double().t().contiguous())
+    near(dW, dy.double().t().contiguous(), h.double().t().contiguous())
+    X, D = x.double(), dh.double()
+    mean = X.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((X - mean) ** 2).mean(1, keepdim=True) + 1e-5)
+    hat, w = (X - mean) * rstd, D * gamma.double()
+    want = rstd * (w - w.mean(1, keepdim=True) - hat * (w * hat).mean(1, keepdim=True))
+    big = rstd * (w.abs() + w.abs().mean(1, keepdim=True) + hat.abs() * (w * hat).abs().mean(1, keepdim=True))
+    assert torch.all((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * big)
+    assert torch.all((dgamma.double() - (D * hat).sum(0)).abs() <= 2.0 ** -14 * (D * hat).abs().sum(0))
+    assert torch.all((dbeta.double() - D.sum(0)).abs() <= 2.0 ** -14 * D.abs().sum(0))
+
+
+def test_layer_step_with_update_in_a_graph(pk):
+    """The whole step with its AdamW update, captured once and replayed: the same weights as
+    the same number of steps called one by one."""
+    rows, k, n = 256, 256, 128
+    outs = []
+    for graph in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(1)
+        x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+        dy = (torch.randn(rows, n, generator=g, device="cuda") * 1e-2).bfloat16()
+        W = torch.randn(n, k, generator=g, device="cuda") * k ** -0.5
+        gamma, beta = torch.ones(k, device="cuda"), torch.zeros(k, device="cuda")
+        params = [W, gamma, beta]
+        grads = [torch.zeros_like(p) for p in params]
+        m, v = [torch.zeros_like(p) for p in params], [torch.zeros_like(p) for p in params]
+        plan = pk.AdamW([pk.AdamWTensor(param=p.data_ptr(), grad=q.data_ptr(), m=a.data_ptr(), v=b.data_ptr(), n=p.numel(),
+                                        weight_decay=0.01 if p is W else 0.0) for p, q, a, b in zip(params, grads, m, v)])
+        keep = []
+
+        def step():
+            r = layer_step(pk, x, dy, W, gamma, beta)
+            keep.append(r)
+            for to, src in zip(grads, (r[2], r[3], r[4])):
+                to.copy_(src)
+            plan.step(1e-2, stream=torch.cuda.current_stream().cuda_stream)
+
+        if graph:
+            st = torch.cuda.Stream()
+            torch.cuda.synchronize()
+            cg = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(cg, stream=st):
+                step()
+            for _ in range(3):
+                cg.replay()
+        else:
+            for _ in range(3):
+                step()
+        torch.cuda.synchronize()
+        assert plan.get_step() == 3
+        outs.append([p.clone() for p in params])
+    for p, q in zip(*outs):
+        assert torch.equal(p, q)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured into a graph."""
+    import subprocess
+    import sys
+    code = """
+import torch, pkt_b200 as pk
+x = torch.randn(64, 256, device="cuda").bfloat16(); y = torch.empty_like(x)
+q = torch.zeros(64, 256, dtype=torch.uint8, device="cuda"); s = torch.zeros(2, 64, device="cuda"); out = torch.zeros(64, 64, device="cuda")
+big = torch.zeros(64 * 4096, dtype=torch.uint8, device="cuda"); bs = torch.ones(32, 64, device="cuda"); big_out = torch.zeros(64, 64, device="cuda")
+d = pk.LayerNormDesc(rows=64, cols=256, dtype=pk.DTYPE_BF16, param_dtype=pk.DTYPE_F32, eps=1e-5, x=x.data_ptr(), ldx=256, y=y.data_ptr(), ldy=256)
+Q = pk.Fp8QuantizeDesc(rows=64, cols=256, dtype=pk.DTYPE_BF16, q_dtype=pk.DTYPE_E4M3, block_rows=1, x=y.data_ptr(), ldx=256, q=q.data_ptr(), ldq=256,
+                       scale=s.data_ptr(), ld_scale=64)
+G = pk.Fp8GemmDesc(M=64, N=64, K=256, a_dtype=pk.DTYPE_E4M3, b_dtype=pk.DTYPE_E4M3, a=q.data_ptr(), lda=256, scale_a=s.data_ptr(), ld_scale_a=64,
+                   a_block_rows=1, b=q.data_ptr(), ldb=256, scale_b=s.data_ptr(), ld_scale_b=64, b_block_rows=1, out=out.data_ptr(), ldo=64,
+                   out_dtype=pk.DTYPE_F32)
+st = torch.cuda.Stream(); torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st):
+    pk.layernorm_forward(d, st.cuda_stream)
+    pk.fp8_quantize(Q, st.cuda_stream)
+    pk.fp8_gemm(G, st.cuda_stream)
+g.replay(); torch.cuda.synchronize()
+h = q.view(torch.float8_e4m3fn).double() * s.double().t().repeat_interleave(128, 1)
+assert torch.allclose(out.double(), h @ h.t(), rtol=1e-5, atol=1e-4), (out.double() - h @ h.t()).abs().max()
+print("ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
