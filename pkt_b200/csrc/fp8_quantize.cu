@@ -1,15 +1,19 @@
 // pkt_fp8_quantize: block-scaled 8-bit operands, plain and transposed, from one read.
 //
 // Bound by memory: a value is read once (2 or 4 bytes) and written once or twice as
-// one byte, with one fp32 scale per 128 or 128 x 128 values.
+// one byte, with one fp32 scale per 128 or 128 x 128 values. Measured at 8192x4096:
+//   bf16, rows      17.1 us, 5.90 TB/s    bf16, both ways 24.0 us, 5.59 TB/s
+//   fp32, rows      26.4 us, 6.35 TB/s    fp32, both ways 33.6 us, 6.00 TB/s
+// (6.55 TB/s: a plain copy). What the bf16 forms lack is instruction issue: about 3 per
+// value with both results.
 //
 // A warp holds 128 columns of a row, 4 consecutive ones per lane. Rows alone
 // (block_rows 1, no transposed result) need nothing beyond a warp: the largest
-// magnitude is one warp reduction, and every warp takes 8 rows: their loads overlap and
-// their scales are computed at once, one per lane. Otherwise a block of 8 warps takes a 128 x 128 tile into registers
-// (a lane has 4 columns x 16 rows, so a column's 16 values of a warp are 16
-// consecutive bytes of the transposed result); column maxima meet in shared memory,
-// and the transposed bytes pass through it to leave as whole 128-byte rows.
+// magnitude is one warp reduction, and a warp takes 4 or 16 rows: their loads overlap and
+// their scales are computed at once, one per lane. Otherwise a block of 8 warps takes a
+// 128 x 128 tile into registers (a lane has 4 columns x 16 rows, so a column's 16 values
+// of a warp are 16 consecutive bytes of the transposed result); column maxima meet in
+// shared memory, and the transposed bytes pass through it to leave as whole 128-byte rows.
 #include <algorithm>
 
 #include "ops_common.h"
@@ -32,8 +36,6 @@ struct QuantArgs {
   long long ld_scale_t;
   float most;
 };
-
-constexpr int kRowsPerWarp = 8;
 
 // A lane's 4 consecutive values of a row as raw words.
 template <typename T>
@@ -77,16 +79,22 @@ __device__ __forceinline__ void load_rows(const QuantArgs& a, long long row0, in
   const T* p = static_cast<const T*>(a.x) + row0 * a.ldx + col;
   if (WIDE && whole) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i].load(p + i * a.ldx, true);
+    for (int i = 0; i < N; ++i, p += a.ldx) r[i].load(p, true);
     return;
   }
+  const bool four = WIDE && col + 4 <= a.cols;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < N; ++i, p += a.ldx) {
 #pragma unroll
     for (int k = 0; k < Row4<T>::kWords; ++k) r[i].w[k] = 0;
+    if (row0 + i >= a.rows) continue;
+    if (four) {
+      r[i].load(p, true);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (row0 + i < a.rows && col + k < a.cols) r[i].set(k, p[i * a.ldx + k]);
+      for (int k = 0; k < 4; ++k)
+        if (col + k < a.cols) r[i].set(k, p[k]);
+    }
   }
 }
 
@@ -102,8 +110,30 @@ __device__ __forceinline__ void store_cols4(uint8_t* row, int col, int cols, uin
 }
 
 template <bool E5M2>
-__device__ __forceinline__ uint32_t quantize4(float v0, float v1, float v2, float v3, float f) {
-  return pack_fp8x4<E5M2>(__fmul_rn(v0, f), __fmul_rn(v1, f), __fmul_rn(v2, f), __fmul_rn(v3, f));
+__device__ __forceinline__ uint32_t quantize4(uint64_t v01, uint64_t v23, uint64_t f) {
+  const float2 a = unpair(mul2(v01, f)), b = unpair(mul2(v23, f));
+  return pack_fp8x4<E5M2>(a.x, a.y, b.x, b.y);
+}
+template <typename T, bool E5M2>
+__device__ __forceinline__ uint32_t quantize_row4(const Row4<T>& r, float f) {
+  return quantize4<E5M2>(r.get2(0), r.get2(1), pair_of(f, f));
+}
+
+// N rows of 4 columns to q, row i with factor(i).
+template <typename T, bool E5M2, int N, typename F>
+__device__ __forceinline__ void store_rows(const QuantArgs& a, long long row0, int col, bool whole, const Row4<T> (&r)[N], F factor) {
+  uint8_t* q = a.q + row0 * a.ldq;
+  if (whole) {
+    q += col;
+#pragma unroll
+    for (int i = 0; i < N; ++i, q += a.ldq) *reinterpret_cast<uint32_t*>(q) = quantize_row4<T, E5M2>(r[i], factor(i));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i, q += a.ldq) {
+    const uint32_t w = quantize_row4<T, E5M2>(r[i], factor(i));
+    if (row0 + i < a.rows) store_cols4(q, col, a.cols, w);
+  }
 }
 
 // Quantises N rows of a warp, each with its own scale: one reduction per row, then the
@@ -119,32 +149,29 @@ __device__ __forceinline__ void quantize_each_row(const QuantArgs& a, long long 
   float f, s;
   block_scale(big, a.most, &f, &s);
   if (lane < N && row0 + lane < a.rows) a.scale[kb * a.ld_scale + row0 + lane] = s;
-  uint8_t* q = a.q + row0 * a.ldq;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t w = quantize4<E5M2>(r[i].get(0), r[i].get(1), r[i].get(2), r[i].get(3), __shfl_sync(0xffffffffu, f, i));
-    if (whole)
-      *reinterpret_cast<uint32_t*>(q + i * a.ldq + col) = w;
-    else if (row0 + i < a.rows)
-      store_cols4(q + i * a.ldq, col, a.cols, w);
-  }
+  store_rows<T, E5M2>(a, row0, col, whole, r, [&](int i) { return __shfl_sync(0xffffffffu, f, i); });
 }
 
-template <typename T, bool WIDE, bool E5M2>
-__global__ void __launch_bounds__(128) quantize_rows(const QuantArgs a) {
+// Registers follow the blocks per SM that hide the most latency. 16 rows, 8192x4096: bf16
+// 17.2 us with 8 blocks and 17.7 us with 6; fp32 32.6 us with 8 and 26.4 us with 6.
+template <typename T, bool WIDE, bool E5M2, int N>
+__global__ void __launch_bounds__(128, N < 16 ? 1 : sizeof(T) == 2 ? 8 : 6) quantize_rows(const QuantArgs a) {
   const int lane = threadIdx.x & 31, kb = blockIdx.x, col = kb * kScaleBlock + 4 * lane;
-  const long long groups = ((long long)a.rows + kRowsPerWarp - 1) / kRowsPerWarp;
+  const long long groups = ((long long)a.rows + N - 1) / N;
   for (long long g = (long long)blockIdx.y * 4 + (threadIdx.x >> 5); g < groups; g += (long long)gridDim.y * 4) {
-    const long long row0 = g * kRowsPerWarp;
-    const bool whole = row0 + kRowsPerWarp <= a.rows && (kb + 1) * kScaleBlock <= a.cols;
-    Row4<T> r[kRowsPerWarp];
+    const long long row0 = g * N;
+    const bool whole = row0 + N <= a.rows && (kb + 1LL) * kScaleBlock <= a.cols;
+    Row4<T> r[N];
     load_rows<T, WIDE>(a, row0, col, whole, r);
     quantize_each_row<T, E5M2>(a, row0, col, kb, whole, r, lane);
   }
 }
 
+// Blocks per SM with both results, 8192x4096: bf16 31.4 us with 2, 26.7 us with 3 and
+// 25.5 us with 4; fp32 34.2, 33.8 and 48.5 us (4 blocks leave too few registers), but
+// 4096x1024 in 128 x 128 blocks 6.6 us with 2 and 6.9 us with 3, which spill.
 template <typename T, bool WIDE, bool E5M2>
-__global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile(const QuantArgs a) {
   __shared__ __align__(16) uint32_t col_big[8][128];
   __shared__ __align__(16) float col_factor[128];
   __shared__ uint32_t tile_big[8];
@@ -173,17 +200,7 @@ __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
         if (a.q) a.scale[kb * a.ld_scale + rt] = s;
         if (a.qt) a.scale_t[rt * a.ld_scale_t + kb] = s;
       }
-      if (a.q) {
-        uint8_t* q = a.q + row0 * a.ldq;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t w = quantize4<E5M2>(r[i].get(0), r[i].get(1), r[i].get(2), r[i].get(3), f);
-          if (whole)
-            *reinterpret_cast<uint32_t*>(q + i * a.ldq + col) = w;
-          else if (row0 + i < a.rows)
-            store_cols4(q + i * a.ldq, col, a.cols, w);
-        }
-      }
+      if (a.q) store_rows<T, E5M2>(a, row0, col, whole, r, [&](int) { return f; });
     } else {
       *reinterpret_cast<uint4*>(&col_big[warp][4 * lane]) = make_uint4(cbig[0], cbig[1], cbig[2], cbig[3]);
       __syncthreads();
@@ -207,7 +224,8 @@ __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          w[k] = quantize4<E5M2>(r[4 * k].get(i), r[4 * k + 1].get(i), r[4 * k + 2].get(i), r[4 * k + 3].get(i), cfs[i]);
+          w[k] = quantize4<E5M2>(pair_of(r[4 * k].get(i), r[4 * k + 1].get(i)), pair_of(r[4 * k + 2].get(i), r[4 * k + 3].get(i)),
+                                 pair_of(cfs[i], cfs[i]));
         // 16-byte pieces of a row are permuted by its column group: 8 lanes, 8 banks
         *reinterpret_cast<uint4*>(bytes + (4 * lane + i) * 128 + ((warp ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
@@ -235,20 +253,28 @@ __global__ void __launch_bounds__(256) quantize_tile(const QuantArgs a) {
 }
 
 template <typename T, bool WIDE, bool E5M2>
-cudaError_t quantize_run(const QuantArgs& a, cudaStream_t st) {
+cudaError_t quantize_run(const QuantArgs& a, int sms, cudaStream_t st) {
   const unsigned kbs = unsigned((a.cols - 1) / kScaleBlock + 1);
   if (a.block_rows == 1 && !a.qt) {
-    const long long blocks = ((long long)a.rows + 4 * kRowsPerWarp - 1) / (4 * kRowsPerWarp);
-    return op_launch(quantize_rows<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(blocks, 65535LL))), dim3(128), 0, st, false, a);
+    // 16 rows per warp keep more bytes in flight, 4 start more warps: bf16 256x4096 (54
+    // row blocks per SM) takes 2.4 us with 16 and 2.2 us with 4, 512x4096 2.8 and 3.1 us,
+    // 8192x4096 17.5 and 34 us. With one value per access 4 rows are the better:
+    // 4099x777 takes 7.3 us instead of 11.9 us.
+    const bool many = WIDE && (long long)kbs * a.rows >= 110LL * sms;
+    const int rows = many ? 64 : 16;
+    const dim3 grid(kbs, unsigned(std::min((a.rows - 1) / rows + 1, 65535)));
+    if constexpr (WIDE)
+      if (many) return op_launch(quantize_rows<T, true, E5M2, 16>, grid, dim3(128), 0, st, false, a);
+    return op_launch(quantize_rows<T, WIDE, E5M2, 4>, grid, dim3(128), 0, st, false, a);
   }
   const int tiles = (a.rows - 1) / 128 + 1;
   return op_launch(quantize_tile<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(tiles, 65535))), dim3(256), 0, st, false, a);
 }
 
 template <typename T>
-cudaError_t quantize_dispatch(const QuantArgs& a, bool wide, bool e5m2, cudaStream_t st) {
-  if (wide) return e5m2 ? quantize_run<T, true, true>(a, st) : quantize_run<T, true, false>(a, st);
-  return e5m2 ? quantize_run<T, false, true>(a, st) : quantize_run<T, false, false>(a, st);
+cudaError_t quantize_dispatch(const QuantArgs& a, bool wide, bool e5m2, int sms, cudaStream_t st) {
+  if (wide) return e5m2 ? quantize_run<T, true, true>(a, sms, st) : quantize_run<T, true, false>(a, sms, st);
+  return e5m2 ? quantize_run<T, false, true>(a, sms, st) : quantize_run<T, false, false>(a, sms, st);
 }
 
 int check_result(const char* name, const void* q, long long ld, const float* scale, long long ld_scale, int cols, long long scales) {
@@ -290,6 +316,6 @@ extern "C" int pkt_fp8_quantize(const pkt_fp8_quantize_desc* d, void* stream) {
   // 4 values in one access: every row of x starts on a boundary of 4 values
   const bool wide = aligned_to(d->x, 4 * es) && d->ldx % 4 == 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = d->dtype == PKT_DTYPE_BF16 ? quantize_dispatch<bf16_t>(a, wide, e5m2, st) : quantize_dispatch<float>(a, wide, e5m2, st);
+  const cudaError_t e = d->dtype == PKT_DTYPE_BF16 ? quantize_dispatch<bf16_t>(a, wide, e5m2, sms, st) : quantize_dispatch<float>(a, wide, e5m2, sms, st);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch quantize");
 }
