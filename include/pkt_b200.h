@@ -397,8 +397,10 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream);
  * of 8; a positive sqrt(v) is held as at least the smallest 8-bit value, so that it
  * never divides by eps alone. States start as zeros (scales too).
  * The plan keeps the pointers and, on the device, the step count: replaying a
- * captured step advances it. Steps of a plan are ordered by the caller (one
- * stream, or events). */
+ * captured step advances it. Calls on a plan are ordered by the caller (one
+ * stream, or events), also against replays of a captured step, and a plan outlives the
+ * graphs that captured it. Arrays that a step writes must not overlap one another or a
+ * gradient (PKT_ERR_ARGS); gradients may be shared. */
 typedef struct pkt_adamw pkt_adamw;
 typedef struct pkt_adamw_tensor {
   void* param;           /* [n], param_dtype, updated in place */
@@ -495,8 +497,9 @@ int pkt_mlp_set_grad_scale(pkt_mlp* m, float scale);
 /* AdamW (pkt_adamw) in the place of SGD, in grad_mode 1: pkt_mlp_train and
  * pkt_mlp_apply_update then update the fp32 masters (and their bf16 copies) with it,
  * with the engine's lr and gradient scale; weight decay is for the weights, not the
- * biases. Starts with empty states and step 0; cfg = NULL goes back to SGD.
- * Synchronises the device. */
+ * biases. Starts with empty states and step 0; cfg = NULL goes back to SGD. A call that
+ * fails leaves what was set before. pkt_mlp_set_params keeps the states. Synchronises
+ * the device. */
 typedef struct pkt_mlp_adamw {
   double beta1, beta2, eps;
   float weight_decay;

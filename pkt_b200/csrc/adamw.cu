@@ -20,7 +20,8 @@
 // 64 bits, so a captured step can be replayed.
 #include <algorithm>
 #include <cmath>
-#include <new>
+#include <exception>
+#include <utility>
 #include <vector>
 
 #include "ops_common.h"
@@ -245,6 +246,7 @@ __global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 2) adam_step(const A
 struct AdamW {
   int device = 0, sms = 0;
   std::vector<AdamTensor> tensors;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // begin and end of every array that a step writes, in order
   int num_chunks = 0;
   int param_dtype = 0, grad_dtype = 0, state_dtype = 0;
   double beta1 = 0, beta2 = 0, eps = 0;
@@ -253,6 +255,7 @@ struct AdamW {
   AdamState* d_state = nullptr;
 
   ~AdamW() {
+    RelaxedCapture relaxed;  // a plan may be dropped while some stream is being captured
     int before = 0;
     const bool back = cudaGetDevice(&before) == cudaSuccess && before != device;
     cudaSetDevice(device);
@@ -266,8 +269,25 @@ struct AdamW {
                  s = state_dtype == PKT_DTYPE_F32 ? 16 : 4;
     t->wide = aligned_to(t->param, p) && aligned_to(t->grad, g) && aligned_to(t->m, s) && aligned_to(t->v, s) && aligned_to(t->copy, 8);
   }
+  // Arrays that a step writes must not overlap (two chunks would race), nor a gradient
+  // with one of them; gradients may be shared.
+  void writes(const void* p, long long n, size_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (p && n > 0) written.push_back({at, at + size_t(n) * bytes});
+  }
+  int sort_written() {
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first < written[i - 1].second) return fail(PKT_ERR_ARGS, "arrays that an AdamW step writes overlap");
+    return PKT_OK;
+  }
   int check_grad(const void* g, size_t i) const {
-    if (!aligned_to(g, grad_dtype == PKT_DTYPE_F32 ? 4 : 2)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
+    const size_t bytes = grad_dtype == PKT_DTYPE_F32 ? 4 : 2;
+    if (!aligned_to(g, bytes)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
+    if (!g) return PKT_OK;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(g), end = at + size_t(tensors[i].n) * bytes;
+    const auto next = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const std::pair<uintptr_t, uintptr_t>& w) { return v < w.second; });
+    if (next != written.end() && next->first < end) return fail(PKT_ERR_ARGS, "grad of tensor %zu overlaps an array that the step writes", i);
     return op_check_memory(g, "grad", device);
   }
   int set_step(long long step, cudaStream_t st) {
@@ -302,16 +322,21 @@ int AdamW::setup(const pkt_adamw_config& c) {
         !aligned_to(s.copy_bf16, 2))
       return fail(PKT_ERR_ARGS, "an array of tensor %d is not aligned to its type", i);
     if ((rc = op_check_memory(s.param, "param", device)) || (rc = op_check_memory(s.m, "m", device)) || (rc = op_check_memory(s.v, "v", device)) ||
-        (rc = op_check_memory(s.copy_bf16, "copy_bf16", device)) || (rc = check_grad(s.grad, size_t(i))))
+        (rc = op_check_memory(s.copy_bf16, "copy_bf16", device)))
       return rc;
     if (eight && ((rc = op_check_memory(s.m_scale, "m_scale", device)) || (rc = op_check_memory(s.v_scale, "v_scale", device)))) return rc;
     AdamTensor t{s.param, s.grad, s.m, s.v, s.m_scale, s.v_scale, static_cast<uint16_t*>(s.copy_bf16), s.n, s.weight_decay, 0};
     set_wide(&t);
     tensors.push_back(t);
-    const long long count = (s.n + kChunk - 1) / kChunk;
+    writes(s.param, s.n, ps), writes(s.m, s.n, ss), writes(s.v, s.n, ss), writes(s.copy_bf16, s.n, 2);
+    if (eight) writes(s.m_scale, (s.n - 1) / kScaleBlock + 1, 4), writes(s.v_scale, (s.n - 1) / kScaleBlock + 1, 4);
+    const long long count = s.n > 0 ? (s.n - 1) / kChunk + 1 : 0;
     if (count + (long long)chunks.size() > 0x7fffffffLL) return fail(PKT_ERR_ARGS, "too many parameters for one AdamW plan");
     for (long long k = 0; k < count; ++k) chunks.push_back(make_int2(i, int(k)));
   }
+  if ((rc = sort_written())) return rc;
+  for (size_t i = 0; i < tensors.size(); ++i)
+    if ((rc = check_grad(tensors[i].grad, i))) return rc;
   num_chunks = int(chunks.size());
   cudaError_t e = cudaMalloc(&d_tensors, sizeof(AdamTensor) * std::max<size_t>(1, tensors.size()));
   if (e == cudaSuccess) e = cudaMalloc(&d_chunks, sizeof(int2) * std::max<size_t>(1, chunks.size()));
@@ -388,7 +413,7 @@ int pkt_adamw_create(int device, const pkt_adamw_config* cfg, pkt_adamw** out) {
     h = new pkt_adamw();
     h->plan.device = dev, h->plan.sms = sms;
     rc = h->plan.setup(*cfg);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {
     rc = fail(PKT_ERR_ARGS, "out of host memory");
   }
   if (rc) {
@@ -415,6 +440,11 @@ int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream) {
   if (!h || (!grads && !h->plan.tensors.empty())) return fail(PKT_ERR_ARGS, "null argument");
   AdamW& p = h->plan;
   OnDevice on(p.device);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus capturing;
+  cudaError_t e = cudaStreamIsCapturing(st, &capturing);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  if (capturing != cudaStreamCaptureStatusNone) return fail(PKT_ERR_ARGS, "AdamW gradients cannot be set inside a stream capture");
   int rc;
   for (size_t i = 0; i < p.tensors.size(); ++i)
     if ((rc = p.check_grad(grads[i], i))) return rc;
@@ -423,11 +453,6 @@ int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream) {
     p.set_wide(&p.tensors[i]);
   }
   if (p.tensors.empty()) return PKT_OK;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaStreamCaptureStatus capturing;
-  cudaError_t e = cudaStreamIsCapturing(st, &capturing);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-  if (capturing != cudaStreamCaptureStatusNone) return fail(PKT_ERR_ARGS, "AdamW gradients cannot be set inside a stream capture");
   e = cudaMemcpyAsync(p.d_tensors, p.tensors.data(), sizeof(AdamTensor) * p.tensors.size(), cudaMemcpyHostToDevice, st);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "copy AdamW gradients");
 }

@@ -689,6 +689,8 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
   using namespace pkb;
   if (!d) return fail(PKT_ERR_ARGS, "null fp8 gemm descriptor");
   if (d->M < 0 || d->N < 0 || d->K < 0) return fail(PKT_ERR_ARGS, "fp8 gemm of M=%d N=%d K=%d", d->M, d->N, d->K);
+  constexpr int kMost = 0x7fffffff - 255;  // the last tile's rows and columns are counted in 32 bits
+  if (d->M > kMost || d->N > kMost) return fail(PKT_ERR_UNSUPPORTED, "fp8 gemm of M=%d N=%d", d->M, d->N);
   if (d->out_dtype != PKT_DTYPE_BF16 && d->out_dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "fp8 gemm out_dtype must be bf16 or f32");
   if (d->M == 0 || d->N == 0) return PKT_OK;
   int dev = 0, sms = 0, rc;
@@ -714,7 +716,7 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
   int bn = 128, pair = 1, split = 1;
   if (swap) {
     bn = d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64;
-  } else if ((long long)((d->M + 255) / 256) * ((d->N + 255) / 256) * 2 > sms / 2) {
+  } else if (((d->M - 1) / 256 + 1LL) * ((d->N - 1) / 256 + 1) * 2 > sms / 2) {
     bn = 256, pair = 2;
   }
   Fp8Args a{};

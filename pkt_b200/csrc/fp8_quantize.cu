@@ -292,6 +292,8 @@ extern "C" int pkt_fp8_quantize(const pkt_fp8_quantize_desc* d, void* stream) {
   using namespace pkb;
   if (!d) return fail(PKT_ERR_ARGS, "null quantize descriptor");
   if (d->rows < 0 || d->cols < 0) return fail(PKT_ERR_ARGS, "quantize of %d x %d values", d->rows, d->cols);
+  constexpr int kMost = 0x7fffffff - 127;  // the last tile's columns are counted in 32 bits
+  if (d->rows > kMost || d->cols > kMost) return fail(PKT_ERR_UNSUPPORTED, "quantize of %d x %d values", d->rows, d->cols);
   if (d->dtype != PKT_DTYPE_BF16 && d->dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "quantize dtype must be bf16 or f32");
   if (d->q_dtype != PKT_DTYPE_E4M3 && d->q_dtype != PKT_DTYPE_E5M2) return fail(PKT_ERR_ARGS, "quantize q_dtype must be e4m3 or e5m2");
   if (d->block_rows != 1 && d->block_rows != 128) return fail(PKT_ERR_ARGS, "block_rows must be 1 or 128");

@@ -560,16 +560,16 @@ __global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
   }
 }
 
-// Long rows, second pass: blockIdx.y is a slab of columns, blockIdx.x a part of the
+// Long rows, second pass: blockIdx.x is a slab of columns, blockIdx.y a part of the
 // rows; the row sums are known, so threads own their columns without a reduction.
 constexpr int kSlabThreads = 256, kSlabRows = 4;
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
   constexpr int N = VEC > 1 ? VEC : 2;
-  const int col0 = blockIdx.y * kSlabThreads * N, tid = threadIdx.x, cols = a.cols - col0;
+  const int col0 = blockIdx.x * kSlabThreads * N, tid = threadIdx.x, cols = a.cols - col0;
   Columns<T, P, VEC, N> c;
   c.init(a, col0 + tid * VEC, kSlabThreads);
-  for (long long row0 = (long long)blockIdx.x * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.x * kSlabRows) {
+  for (long long row0 = (long long)blockIdx.y * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.y * kSlabRows) {
     Held<T, VEC, N> x[kSlabRows], y[kSlabRows];
     float4 st[kSlabRows];
 #pragma unroll
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a)
                                 st[r].w);
     }
   }
-  float* part = a.part + (long long)blockIdx.x * 2 * a.cols + col0;
+  float* part = a.part + (long long)blockIdx.y * 2 * a.cols + col0;
 #pragma unroll
   for (int v = 0; v < N; ++v) {
     const int col = (v / VEC * kSlabThreads + tid) * VEC + v % VEC;
@@ -659,7 +659,7 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
   // The ring pays from a few rows per group on: up to 32 values per thread in the
   // forward pass (16 one by one), 16 in the backward pass (three more registers each; 8
   // one by one while they hold the row), in as few threads as hold the row.
-  const int most = wide && !backward ? 32 : backward && !wide && d.cols <= 8 * kRingThreads ? 8 : 16, least = wide ? p.vec : 8;
+  const int most = wide && !backward ? 32 : backward && !wide && d.cols <= 8 * kRingThreads ? 8 : 16, least = 8;
   for (int n = most; n >= least; n /= 2) {
     if (!fit(n, kRingThreads)) break;
     if (p.size == 32 && 32 * (n / 2) >= d.cols && n / 2 >= least) continue;
@@ -713,7 +713,7 @@ int ln_launch(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, co
 // partial rows written.
 template <typename T, typename P, int VEC, int N>
 int ln_run(const LnArgs& a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
-  static std::atomic<uint64_t> done[5];
+  static std::atomic<uint64_t> done[5];  // one per kernel
   const bool exact = a.cols == p.size * N;
   if (!backward) {
     if constexpr (N >= 8) {
@@ -747,7 +747,7 @@ int ln_pick(const LnArgs& a, const LnPlan& p, bool backward, int dev, int sms, c
     const long long want = std::max(1LL, 8LL * sms / slabs);  // about 8 blocks of 256 threads per SM
     const int rows = int(std::min<long long>({want, a.parts, (a.rows - 1) / kSlabRows + 1}));
     cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(512), 0, st, false, a);
-    if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(rows, slabs), dim3(kSlabThreads), 0, st, false, a);
+    if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(slabs, rows), dim3(kSlabThreads), 0, st, false, a);
     return e == cudaSuccess ? rows : cuda_fail(e, "launch layer norm");
   }
   switch (p.n) {

@@ -1091,7 +1091,6 @@ int Mlp::launch_list(pkt_task* d, int n, cudaStream_t st) {
 // One tensor per layer's weights (with their padded columns: values and gradients stay
 // zero there) and per bias; all states in one allocation.
 int Mlp::set_adamw(const pkt_mlp_adamw& c) {
-  drop_adamw();
   const bool eight = c.state_dtype == PKT_DTYPE_E4M3;
   if (!eight && c.state_dtype != PKT_DTYPE_F32) return fail(PKT_ERR_ARGS, "AdamW state_dtype must be f32 or e4m3");
   std::vector<pkt_adamw_tensor> ts;
@@ -1115,9 +1114,10 @@ int Mlp::set_adamw(const pkt_mlp_adamw& c) {
   auto scales = [&](const pkt_adamw_tensor& t) { return eight ? up(size_t(t.n + 127) / 128 * 4) : size_t(0); };
   size_t total = 0;
   for (const pkt_adamw_tensor& t : ts) total += 2 * values(t) + 2 * scales(t);
-  int rc = alloc(&adamw_state, total);
+  void* state = nullptr;
+  int rc = alloc(&state, total);
   if (rc) return rc;
-  uint8_t* at = static_cast<uint8_t*>(adamw_state);
+  uint8_t* at = static_cast<uint8_t*>(state);
   auto take = [&](size_t n) {
     uint8_t* p = n ? at : nullptr;
     at += n;
@@ -1130,12 +1130,14 @@ int Mlp::set_adamw(const pkt_mlp_adamw& c) {
     t.v_scale = reinterpret_cast<float*>(take(scales(t)));
   }
   const pkt_adamw_config cfg{int(ts.size()), ts.data(), PKT_DTYPE_F32, PKT_DTYPE_F32, c.state_dtype, c.beta1, c.beta2, c.eps, 0};
-  rc = pkt_adamw_create(rt->device, &cfg, &adamw);
-  if (rc) {
-    adamw = nullptr;
-    drop_adamw();
+  pkt_adamw* plan = nullptr;
+  if ((rc = pkt_adamw_create(rt->device, &cfg, &plan))) {
+    cudaFree(state);
+    return rc;
   }
-  return rc;
+  drop_adamw();  // what was set before stays until the new one stands
+  adamw = plan, adamw_state = state;
+  return PKT_OK;
 }
 
 }  // namespace pkb

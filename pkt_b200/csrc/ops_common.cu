@@ -7,16 +7,6 @@ namespace pkb {
 
 static __device__ int g_ops_status;
 
-namespace {
-// First calls may come inside a stream capture, where some queries are only allowed in
-// relaxed mode; none of them touches the captured stream.
-struct RelaxedCapture {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
-}  // namespace
-
 static void* driver_entry(const char* name) {
   void* p = nullptr;
   cudaDriverEntryPointQueryResult q;

@@ -11,11 +11,6 @@
 
 namespace pkb {
 
-constexpr int kScaleBlock = 128;  // values of one 8-bit block along the contiguous dimension
-// A block whose largest magnitude is below 2^-100 is held as zeros with scale 0:
-// from there on, largest value / magnitude stays far from fp32 overflow.
-constexpr float kScaleTiny = 7.888609052210118e-31f;
-
 // The current device, checked once to be one this build runs on, its SM count and
 // (where asked for) the address of its status word, which a kernel sets when one of
 // its bounded waits runs out.
@@ -30,6 +25,14 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled op_encode_tiled();
+
+// First calls may come inside a stream capture, where some queries are only allowed in
+// relaxed mode; none of them touches the captured stream.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 

@@ -1,5 +1,5 @@
-// Device helpers of the stand-alone operators: typed vector loads and stores,
-// warp reductions, block-scaled 8-bit floats.
+// Device helpers of the stand-alone operators: typed vector loads and stores, bulk
+// copies and bounded waits, block-scaled 8-bit floats.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "../../include/pk/detail/ptx.cuh"
+#include "../../include/pkt_b200.h"
 
 namespace pkb {
 
@@ -109,12 +110,6 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
-}
-
 template <typename T, int VEC>
 __device__ __forceinline__ void store_pairs(T* p, const uint64_t (&v)[VEC / 2]) {
   constexpr int kBytes = VEC * int(sizeof(T));
@@ -165,7 +160,7 @@ __device__ __forceinline__ bool try_phase(uint64_t* bar, uint32_t parity) {
 // The same for a converged warp (one answer for all lanes); a timeout is recorded.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int* status) {
   if (__all_sync(0xffffffffu, try_phase(bar, parity))) return true;
-  *reinterpret_cast<volatile int*>(status) = 2;  // PKT_DEV_TIMEOUT_PIPE
+  *reinterpret_cast<volatile int*>(status) = PKT_DEV_TIMEOUT_PIPE;
   return false;
 }
 // `bytes` (a multiple of 16, both addresses 16-byte aligned) global -> shared,
@@ -185,10 +180,15 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 // in its scale.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+constexpr int kScaleBlock = 128;  // values of one 8-bit block along the contiguous dimension
+// A block whose largest magnitude is below 2^-100 is held as zeros with scale 0:
+// from there on, largest value / magnitude stays far from fp32 overflow.
+constexpr float kScaleTiny = 7.888609052210118e-31f;
+
 // Factor and scale of a block from its largest magnitude: q = rn(x * factor), x ~ q * scale.
 __device__ __forceinline__ void block_scale(uint32_t amax_bits, float most, float* factor, float* scale) {
   const float big = __uint_as_float(amax_bits);
-  const bool none = big < 7.888609052210118e-31f;  // kScaleTiny
+  const bool none = big < kScaleTiny;
   *factor = none ? 0.f : __fdiv_rn(most, big);
   *scale = none ? 0.f : __fdiv_rn(big, most);
 }

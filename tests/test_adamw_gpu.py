@@ -255,10 +255,10 @@ def test_state_from_a_long_run(pk):
 
 
 def test_refusals(pk):
-    t = torch.zeros(256, device="cuda")
+    t = torch.zeros(4, 256, device="cuda")
     host = torch.zeros(256)
-    ok = dict(param=t.data_ptr(), grad=t.data_ptr(), m=t.data_ptr(), v=t.data_ptr(), n=256)
-    for kw, word, opts in [(dict(param=None), "needs param", {}), (dict(n=-1), "values", {}), (dict(m=t.data_ptr() + 2), "aligned", {}),
+    ok = dict(param=t[0].data_ptr(), grad=t[1].data_ptr(), m=t[2].data_ptr(), v=t[3].data_ptr(), n=256)
+    for kw, word, opts in [(dict(param=None), "needs param", {}), (dict(n=-1), "values", {}), (dict(m=t[2].data_ptr() + 2), "aligned", {}),
                            (dict(grad=host.data_ptr()), "not device memory", {}), ({}, "m_scale", dict(state_dtype="e4m3")),
                            ({}, "betas", dict(beta1=1.0)), ({}, "eps", dict(eps=-1.0)), ({}, "step", dict(step=-1)), ({}, "out of range", dict(device=63))]:
         with pytest.raises(pk.PktError, match=word):
@@ -270,3 +270,68 @@ def test_refusals(pk):
         plan.set_grads([host.data_ptr()])
     with pytest.raises(pk.PktError):
         plan.set_step(-1)
+    with pytest.raises(pk.PktError, match="too many"):
+        pk.AdamW([pk.AdamWTensor(**{**ok, "n": (1 << 63) - 1})])
+
+
+def test_refuses_overlapping_arrays(pk):
+    """What a step writes twice, or writes while it is another chunk's gradient, would depend on timing."""
+    t = torch.zeros(8, 256, device="cuda")
+    at = [t[i].data_ptr() for i in range(8)]
+    ok = dict(param=at[0], grad=at[1], m=at[2], v=at[3], n=256)
+    other = dict(param=at[4], grad=at[1], m=at[5], v=at[6], n=256)  # a shared gradient
+    plan = pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**other)])
+    for kw in (dict(param=at[0]), dict(m=at[0] + 1020), dict(v=at[2]), dict(copy_bf16=at[3] + 512), dict(n=257)):
+        with pytest.raises(pk.PktError, match="writes overlap"):
+            pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**other, **kw})])
+    for g in (at[0], at[0] - 4, at[6] + 1020):
+        with pytest.raises(pk.PktError, match="grad of tensor 1 overlaps"):
+            pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**other, "grad": g})])
+        with pytest.raises(pk.PktError, match="grad of tensor 1 overlaps"):
+            plan.set_grads([at[1], g])
+    plan.set_grads([at[7], None])
+    t[7] = 1.0
+    plan.step(1e-2)
+    assert torch.all(t[2] != 0) and torch.all(t[5] == 0)
+    pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**ok, "n": 0})])  # nothing is written twice
+
+
+def test_gradients_stay_as_they_were_inside_a_capture(pk):
+    c = Case(pk, [3000])
+    before = c.snapshot()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        with pytest.raises(pk.PktError, match="stream capture"):
+            c.plan.set_grads([None], st.cuda_stream)
+        c.plan.step(1e-2, stream=st.cuda_stream)
+    g.replay()
+    torch.cuda.synchronize()
+    c.check(before, 1, 1e-2)
+
+
+def test_a_plan_may_be_dropped_while_a_stream_is_captured(pk):
+    a, b = Case(pk, [3000]), Case(pk, [500])
+    before = a.snapshot()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        a.plan.step(1e-2, stream=st.cuda_stream)
+        b.plan.close()
+    g.replay()
+    torch.cuda.synchronize()
+    a.check(before, 1, 1e-2)
+
+
+def test_two_plans_on_two_streams(pk):
+    a, b = Case(pk, [300000, 7], seed=1), Case(pk, [200000], state="e4m3", seed=2)
+    want = a.snapshot(), b.snapshot()
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    a.plan.step(1e-2, stream=s.cuda_stream)
+    b.plan.step(1e-2, stream=t.cuda_stream)
+    torch.cuda.synchronize()
+    a.check(want[0], 1, 1e-2)
+    b.check(want[1], 1, 1e-2)

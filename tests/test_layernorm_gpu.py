@@ -316,3 +316,59 @@ def test_refuses_what_it_cannot_reach(pk):
     d.workspace_bytes -= 1
     with pytest.raises(pk.PktError, match="workspace of"):
         pk.layernorm_backward(d)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(40000, 4), (20000, 8), (9001, 64), (5000, 96), (12000, 128), (30000, 7)])
+def test_many_short_rows(pk, rows, cols, dtype):
+    d, s = make(pk, rows, cols, dtype, seed=cols)
+    pk.layernorm_forward(d)
+    check_forward(s)
+    pk.layernorm_backward(d)
+    check_backward(s)
+
+
+@pytest.mark.parametrize("dtype,pad", [("bf16", 0), ("bf16", 1), ("f32", 0)])
+def test_rows_of_many_millions(pk, dtype, pad):
+    """More slabs of columns than one grid dimension but the first can count."""
+    d, s = make(pk, 2, 65536 * 512 + 1032, dtype, pad=pad, seed=pad)
+    pk.layernorm_forward(d)
+    check_forward(s)
+    pk.layernorm_backward(d)
+    check_backward(s)
+
+
+def test_in_place_through_the_rings(pk):
+    """Rows that share 16-byte granules with their neighbours, read ahead while earlier ones are written."""
+    for cols, dtype in ((777, "bf16"), (1024, "bf16"), (333, "f32")):
+        d, s = make(pk, 6000, cols, dtype)
+        pk.layernorm_forward(d)
+        want = s["y"].clone()
+        pk.layernorm_backward(d)
+        dx = s["dx"].clone()
+        for into in ("dy", "x"):
+            keep = s[into].clone()
+            d.dx = ptr(s[into])
+            pk.layernorm_backward(d)
+            assert torch.equal(s[into], dx)
+            s[into].copy_(keep)
+        d.y = d.x
+        pk.layernorm_forward(d)
+        assert torch.equal(s["x"], want)
+
+
+def test_two_calls_at_once(pk):
+    """Two streams, a workspace each."""
+    a, b = make(pk, 3000, 1000, seed=1), make(pk, 2500, 777, "f32", seed=2)
+    for d, s in (a, b):
+        pk.layernorm_forward(d)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        for (d, s), st in zip((a, b), streams):
+            pk.layernorm_backward(d, st.cuda_stream)
+            pk.layernorm_forward(d, st.cuda_stream)
+    torch.cuda.synchronize()
+    for d, s in (a, b):
+        check_forward(s)
+        check_backward(s)

@@ -113,3 +113,15 @@ def test_empty_problems_need_no_memory():
     pkt_b200.fp8_quantize(quant(cols=0))
     pkt_b200.fp8_gemm(gemm(M=0))
     pkt_b200.fp8_gemm(gemm(N=0))
+
+
+@pytest.mark.parametrize("kw", [dict(rows=2**31 - 1), dict(cols=2**31 - 100, ldx=2**31)])
+def test_quantize_of_more_than_it_can_count(kw):
+    with pytest.raises(pkt_b200.PktError, match="quantize of"):
+        pkt_b200.fp8_quantize(quant(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(M=2**31 - 1, ld_scale_a=2**31), dict(N=2**31 - 100, ldo=2**31, ld_scale_b=2**31)])
+def test_gemm_of_more_than_it_can_count(kw):
+    with pytest.raises(pkt_b200.PktError, match="fp8 gemm of"):
+        pkt_b200.fp8_gemm(gemm(**kw))

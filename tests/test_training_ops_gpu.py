@@ -101,6 +101,20 @@ def test_mlp_engine_refuses_adamw_without_gradients(pk):
     assert len(m.losses()) == 1
 
 
+def test_a_refused_adamw_leaves_the_one_before(pk):
+    a, b = engine(pk, [64, 64], 128, "bf16"), engine(pk, [64, 64], 128, "bf16")
+    for m in (a, b):
+        m.set_adamw()
+        m.train(2)
+    with pytest.raises(pk.PktError, match="betas"):
+        a.set_adamw(beta2=1.0)
+    for m in (a, b):
+        m.train(2)
+    for x, y in zip(a.get_params(), b.get_params()):
+        for p, q in zip(x, y):
+            assert np.array_equal(p, q)
+
+
 # ---------------------------------------------------------------- a normalised linear layer
 def q8(pk, x, block_rows, plain=True, transposed=False):
     """(q, scale), (qt, scale_t) of a contiguous matrix."""
