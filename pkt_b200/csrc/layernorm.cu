@@ -70,84 +70,88 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* red, int size, int
 
 __device__ __forceinline__ uint64_t twice(float v) { return pair_of(v, v); }
 
-// N values of a row in one thread, as raw words: N / VEC vectors of VEC consecutive
-// values, vector k at column (k * size + tid) * VEC; zeros past the row's end. EXACT:
-// the threads cover the row without a rest.
+// N values of a row in one thread, as raw words (as fp32 where they are loaded one by
+// one): N / VEC vectors of VEC consecutive values; zeros past the row's end. A warp's
+// columns are contiguous, vector k of lane l at (k * 32 + l) * VEC from its first one, so
+// that all distances are constants. EXACT: the threads cover the row without a rest.
 template <typename T, int VEC, int N>
 struct Held {
   static constexpr int K = N / VEC;
-  uint32_t w[N * int(sizeof(T)) / 4];
+  static constexpr int kWords = VEC == 1 ? N : N * int(sizeof(T)) / 4;
+  uint32_t w[kWords];
 
-  static __device__ __forceinline__ int col(int k, int tid, int size) { return (k * size + tid) * VEC; }
+  // the thread's first column
+  static __device__ __forceinline__ int first(int tid) { return ((tid >> 5) * K * 32 + (tid & 31)) * VEC; }
+  static __device__ __forceinline__ constexpr int at(int k) { return k * 32 * VEC; }
   template <bool EXACT>
-  __device__ __forceinline__ void load(const T* row, int tid, int size, int cols, bool here = true) {
+  __device__ __forceinline__ void load(const T* row, int c0, int cols) {
+    row += c0;
 #pragma unroll
-    for (int i = 0; i < N * int(sizeof(T)) / 4; ++i) w[i] = 0;
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = col(k, tid, size);
-      if (!here || (!EXACT && c >= cols)) continue;
+      if (!EXACT && c0 + at(k) >= cols) continue;
       if constexpr (VEC > 1) {
-        const uint4 v = *reinterpret_cast<const uint4*>(row + c);
+        const uint4 v = *reinterpret_cast<const uint4*>(row + at(k));
         w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
-      } else if constexpr (sizeof(T) == 4) {
-        w[k] = *reinterpret_cast<const uint32_t*>(row + c);
       } else {
-        w[k / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(row + c)) << (16 * (k & 1));
+        w[k] = __float_as_uint(to_f32(row[at(k)]));
       }
     }
   }
   // values 2 p and 2 p + 1 of the thread
   __device__ __forceinline__ uint64_t pair(int p) const {
-    if constexpr (sizeof(T) == 4) return pair_of(__uint_as_float(w[2 * p]), __uint_as_float(w[2 * p + 1]));
-    return pair_of(bf16_lo(w[p]), bf16_hi(w[p]));
+    if constexpr (VEC == 1 || sizeof(T) == 4)
+      return pair_of(__uint_as_float(w[2 * p]), __uint_as_float(w[2 * p + 1]));
+    else
+      return pair_of(bf16_lo(w[p]), bf16_hi(w[p]));
   }
   // -mean for the values inside the row, 0 for the zeros past its end
   template <bool EXACT>
-  static __device__ __forceinline__ uint64_t minus(float mean, int p, int tid, int size, int cols) {
+  static __device__ __forceinline__ uint64_t minus(float mean, int p, int c0, int cols) {
     if constexpr (EXACT) return twice(-mean);
-    const int c0 = col(2 * p / VEC, tid, size), c1 = col((2 * p + 1) / VEC, tid, size);
-    return pair_of(c0 < cols ? -mean : 0.f, c1 < cols ? -mean : 0.f);
+    return pair_of(c0 + at(2 * p / VEC) < cols ? -mean : 0.f, c0 + at((2 * p + 1) / VEC) < cols ? -mean : 0.f);
   }
 };
 
 // The results of a row, rounded to its type once.
 template <typename T, int VEC, int N, bool EXACT>
-__device__ __forceinline__ void store_held(T* row, const uint64_t (&v)[N / 2], int tid, int size, int cols) {
+__device__ __forceinline__ void store_held(T* row, const uint64_t (&v)[N / 2], int c0, int cols) {
   using S = Held<T, VEC, N>;
+  row += c0;
 #pragma unroll
   for (int k = 0; k < S::K; ++k) {
-    const int c = S::col(k, tid, size);
-    if (!EXACT && c >= cols) continue;
+    if (!EXACT && c0 + S::at(k) >= cols) continue;
     if constexpr (VEC > 1) {
       uint64_t q[VEC / 2];
 #pragma unroll
       for (int i = 0; i < VEC / 2; ++i) q[i] = v[k * VEC / 2 + i];
-      store_pairs<T, VEC>(row + c, q);
+      store_pairs<T, VEC>(row + S::at(k), q);
     } else {
       const float2 f = unpair(v[k / 2]);
-      from_f32(k & 1 ? f.y : f.x, row + c);
+      from_f32(k & 1 ? f.y : f.x, row + S::at(k));
     }
   }
 }
 
 // The thread's pairs of a parameter row (fp32 or bf16; `other` where there is none).
 template <typename P, int VEC, int N>
-__device__ __forceinline__ void load_params(const void* base, float other, int col0, int size, int cols, uint64_t (&out)[N / 2]) {
+__device__ __forceinline__ void load_params(const void* base, float other, int c0, int cols, uint64_t (&out)[N / 2]) {
+  const P* from = static_cast<const P*>(base) + c0;
 #pragma unroll
   for (int k = 0; k < N / (VEC > 1 ? VEC : 2); ++k) {
     if constexpr (VEC > 1) {
-      const int c = col0 + k * size * VEC;
+      const bool in = c0 + k * 32 * VEC < cols;
       Raw<P, VEC> r;
-      r.load(static_cast<const P*>(base) + c, base && c < cols);
+      r.load(from + k * 32 * VEC, base && in);
 #pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) out[k * VEC / 2 + i] = base ? r.get2(i) : twice(c < cols ? other : 0.f);
+      for (int i = 0; i < VEC / 2; ++i) out[k * VEC / 2 + i] = base ? r.get2(i) : twice(in ? other : 0.f);
     } else {
       float f[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int c = col0 + (2 * k + i) * size;
-        f[i] = c >= cols ? 0.f : base ? to_f32(static_cast<const P*>(base)[c]) : other;
+        const int c = (2 * k + i) * 32;
+        f[i] = c0 + c >= cols ? 0.f : base ? to_f32(from[c]) : other;
       }
       out[k] = pair_of(f[0], f[1]);
     }
@@ -205,8 +209,9 @@ __global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
   __shared__ float2 red[2][32];
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
+    const int c0 = Held<T, VEC, N>::first(tid);
     Held<T, VEC, N> x;
-    x.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, tid, size, a.cols);
+    x.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, c0, a.cols);
     uint64_t s = 0;
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) s = add2(s, x.pair(p));
@@ -214,17 +219,17 @@ __global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
     s = 0;
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) {
-      const uint64_t d = add2(x.pair(p), x.template minus<false>(mean, p, tid, size, a.cols));
+      const uint64_t d = add2(x.pair(p), x.template minus<false>(mean, p, c0, a.cols));
       s = fma2(d, d, s);
     }
     const float rstd = 1.f / sqrtf(group_sum(make_float2(sum_of(s), 0.f), red[1], size, group).x * a.inv_cols + a.eps);
     if (tid == 0) put_stats(a, row, mean, rstd);
     uint64_t g[N / 2], b[N / 2], out[N / 2];
-    load_params<P, VEC, N>(a.gamma, 1.f, tid * VEC, size, a.cols, g);
-    load_params<P, VEC, N>(a.beta, 0.f, tid * VEC, size, a.cols, b);
+    load_params<P, VEC, N>(a.gamma, 1.f, c0, a.cols, g);
+    load_params<P, VEC, N>(a.beta, 0.f, c0, a.cols, b);
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(add2(x.pair(p), twice(-mean)), twice(rstd)), g[p], b[p]);
-    store_held<T, VEC, N, false>(static_cast<T*>(a.y) + row * a.ldy, out, tid, size, a.cols);
+    store_held<T, VEC, N, false>(static_cast<T*>(a.y) + row * a.ldy, out, c0, a.cols);
   }
 }
 
@@ -240,6 +245,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
+  const int c0 = Held<T, VEC, N>::first(tid);
   float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols rounded up to 4]
   const int pcols = (a.cols + 3) & ~3;
   for (int c = threadIdx.x; c < a.cols; c += kRingThreads) {
@@ -265,12 +271,11 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     Held<T, VEC, N> x0, x1;  // a missing second row is zeros
     const int slot0 = ring.slot;
     ring.wait(a.status);
-    x0.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at))), tid, size, a.cols);
+    x0.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at))), c0, a.cols);
     ring.next();
     const int slot1 = ring.slot;
     if (two) ring.wait(a.status);
-    x1.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at + next_x))), tid, size, a.cols,
-                            two);
+    x1.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at + next_x))), c0, two ? a.cols : 0);
     if (two) ring.next();
     uint64_t s0 = 0, s1 = 0;
 #pragma unroll
@@ -286,8 +291,8 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     s0 = s1 = 0;
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) {
-      const uint64_t d0 = add2(x0.pair(p), x0.template minus<EXACT>(mean.x, p, tid, size, a.cols));
-      const uint64_t d1 = add2(x1.pair(p), x1.template minus<EXACT>(mean.y, p, tid, size, a.cols));
+      const uint64_t d0 = add2(x0.pair(p), x0.template minus<EXACT>(mean.x, p, c0, a.cols));
+      const uint64_t d1 = add2(x1.pair(p), x1.template minus<EXACT>(mean.y, p, c0, a.cols));
       s0 = fma2(d0, d0, s0);
       s1 = fma2(d1, d1, s1);
     }
@@ -301,20 +306,20 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     constexpr int C = VEC > 1 ? VEC : 2;  // values stored together
 #pragma unroll
     for (int q = 0; q < N / C; ++q) {
-      const int c0 = Held<T, VEC, N>::col(q * C / VEC, tid, size), c1 = VEC > 1 ? c0 + 1 : Held<T, VEC, N>::col(2 * q + 1, tid, size);
-      if (!EXACT && c0 >= a.cols) continue;
+      const int ca = c0 + Held<T, VEC, N>::at(q * C / VEC), cb = VEC > 1 ? ca + 1 : ca + Held<T, VEC, N>::at(1);
+      if (!EXACT && ca >= a.cols) continue;
       uint64_t g[C / 2], b[C / 2], out[C / 2];
       if constexpr (VEC > 1) {
 #pragma unroll
         for (int i = 0; i < C / 4; ++i) {
-          const float4 u = *reinterpret_cast<const float4*>(params + c0 + 4 * i), v = *reinterpret_cast<const float4*>(params + pcols + c0 + 4 * i);
+          const float4 u = *reinterpret_cast<const float4*>(params + ca + 4 * i), v = *reinterpret_cast<const float4*>(params + pcols + ca + 4 * i);
           g[2 * i] = pair_of(u.x, u.y), g[2 * i + 1] = pair_of(u.z, u.w);
           b[2 * i] = pair_of(v.x, v.y), b[2 * i + 1] = pair_of(v.z, v.w);
         }
       } else {
-        const bool in = c1 < a.cols;
-        g[0] = pair_of(params[c0], in ? params[c1] : 0.f);
-        b[0] = pair_of(params[pcols + c0], in ? params[pcols + c1] : 0.f);
+        const bool in = cb < a.cols;
+        g[0] = pair_of(params[ca], in ? params[cb] : 0.f);
+        b[0] = pair_of(params[pcols + ca], in ? params[pcols + cb] : 0.f);
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -324,11 +329,11 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
           out[i] = fma2(mul2(add2((r ? x1 : x0).pair(q * C / 2 + i), r ? m1 : m0), r ? r1 : r0), g[i], b[i]);
         T* to = y + (r ? next_y : 0);
         if constexpr (VEC > 1) {
-          store_pairs<T, VEC>(to + c0, out);
+          store_pairs<T, VEC>(to + ca, out);
         } else {
           const float2 f = unpair(out[0]);
-          from_f32(f.x, to + c0);
-          if (c1 < a.cols) from_f32(f.y, to + c1);
+          from_f32(f.x, to + ca);
+          if (cb < a.cols) from_f32(f.y, to + cb);
         }
       }
     }
@@ -342,6 +347,7 @@ template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
   constexpr int N = VEC > 1 ? VEC : 2;
   __shared__ float2 red[2][32];
+  const int c0 = Held<T, VEC, N>::first(threadIdx.x);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* y = static_cast<T*>(a.y) + row * a.ldy;
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
 #pragma unroll 4
     for (int c = 0; c < a.cols; c += 1024 * N) {
       Held<T, VEC, N> v;
-      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
+      v.template load<false>(x + c, c0, a.cols - c);
 #pragma unroll
       for (int p = 0; p < N / 2; ++p) s = add2(s, v.pair(p));
     }
@@ -358,10 +364,10 @@ __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
 #pragma unroll 4
     for (int c = 0; c < a.cols; c += 1024 * N) {
       Held<T, VEC, N> v;
-      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
+      v.template load<false>(x + c, c0, a.cols - c);
 #pragma unroll
       for (int p = 0; p < N / 2; ++p) {
-        const uint64_t d = add2(v.pair(p), v.template minus<false>(mean, p, threadIdx.x, 1024, a.cols - c));
+        const uint64_t d = add2(v.pair(p), v.template minus<false>(mean, p, c0, a.cols - c));
         s = fma2(d, d, s);
       }
     }
@@ -370,13 +376,13 @@ __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
 #pragma unroll 2
     for (int c = 0; c < a.cols; c += 1024 * N) {
       Held<T, VEC, N> v;
-      v.template load<false>(x + c, threadIdx.x, 1024, a.cols - c);
+      v.template load<false>(x + c, c0, a.cols - c);
       uint64_t g[N / 2], b[N / 2], out[N / 2];
-      load_params<P, VEC, N>(a.gamma, 1.f, c + threadIdx.x * VEC, 1024, a.cols, g);
-      load_params<P, VEC, N>(a.beta, 0.f, c + threadIdx.x * VEC, 1024, a.cols, b);
+      load_params<P, VEC, N>(a.gamma, 1.f, c + c0, a.cols, g);
+      load_params<P, VEC, N>(a.beta, 0.f, c + c0, a.cols, b);
 #pragma unroll
       for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(add2(v.pair(p), twice(-mean)), twice(rstd)), g[p], b[p]);
-      store_held<T, VEC, N, false>(y + c, out, threadIdx.x, 1024, a.cols - c);
+      store_held<T, VEC, N, false>(y + c, out, c0, a.cols - c);
     }
   }
 }
@@ -387,8 +393,8 @@ template <typename T, typename P, int VEC, int N>
 struct Columns {
   uint64_t gamma[N / 2], dg[N / 2], db[N / 2];
 
-  __device__ __forceinline__ void init(const LnArgs& a, int col0, int size) {
-    load_params<P, VEC, N>(a.gamma, 1.f, col0, size, a.cols, gamma);
+  __device__ __forceinline__ void init(const LnArgs& a, int c0) {
+    load_params<P, VEC, N>(a.gamma, 1.f, c0, a.cols, gamma);
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) dg[p] = db[p] = 0;
   }
@@ -409,33 +415,52 @@ struct Columns {
   }
   // dx = rstd (w - c1 - h c2)
   template <bool EXACT>
-  __device__ __forceinline__ void write(const Held<T, VEC, N>& x, const Held<T, VEC, N>& y, T* dx, int tid, int size, int cols, float mean,
+  __device__ __forceinline__ void write(const Held<T, VEC, N>& x, const Held<T, VEC, N>& y, T* dx, int c0, int cols, float mean,
                                         float rstd, float c1, float c2) {
     const uint64_t m = twice(-mean), r = twice(rstd), r1 = twice(-rstd * c1), r2 = twice(-rstd * c2 * rstd);
     uint64_t out[N / 2];
 #pragma unroll
     for (int p = 0; p < N / 2; ++p) out[p] = fma2(mul2(y.pair(p), gamma[p]), r, fma2(add2(x.pair(p), m), r2, r1));
-    store_held<T, VEC, N, EXACT>(dx, out, tid, size, cols);
+    store_held<T, VEC, N, EXACT>(dx, out, c0, cols);
+  }
+  // 4 of the thread's column sums (its values 4 q..4 q + 3) to a partial row.
+  static __device__ __forceinline__ void put4(float* part, int q, int c0, int cols, float4 v) {
+    const int c = c0 + (4 * q / VEC) * 32 * VEC + 4 * q % VEC;
+    if constexpr (VEC > 1) {
+      if (c < cols) *reinterpret_cast<float4*>(part + c) = v;
+    } else {
+      const float u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + 32 * i < cols) part[c + 32 * i] = u[i];
+    }
+  }
+  static __device__ __forceinline__ float4 four(const uint64_t (&v)[N / 2], int q) {
+    const float2 a = unpair(v[2 * q]), b = unpair(v[2 * q + 1]);
+    return make_float4(a.x, a.y, b.x, b.y);
   }
   // The block's partial row: its groups' column sums, added in group order. `sums`:
-  // shared memory, [groups][2 N][size].
-  __device__ __forceinline__ void finish(const LnArgs& a, int tid, int size, int group, int groups, float* sums) {
+  // shared memory, [groups][2 N / 4][size] (one group needs none).
+  __device__ __forceinline__ void finish(const LnArgs& a, int tid, int size, int group, int groups, float4* sums) {
     float* part = a.part + (long long)blockIdx.x * 2 * a.cols;
-    float* mine = sums + group * 2 * N * size + tid;
+    const int c0 = Held<T, VEC, N>::first(tid);
+    if (groups == 1) {
 #pragma unroll
-    for (int p = 0; p < N / 2; ++p) {
-      const float2 g = unpair(dg[p]), b = unpair(db[p]);
-      mine[2 * p * size] = g.x, mine[(2 * p + 1) * size] = g.y;
-      mine[(N + 2 * p) * size] = b.x, mine[(N + 2 * p + 1) * size] = b.y;
+      for (int q = 0; q < N / 4; ++q) put4(part, q, c0, a.cols, four(dg, q)), put4(part + a.cols, q, c0, a.cols, four(db, q));
+      return;
     }
+    const int step = N / 2 * size;
+    float4* mine = sums + group * step + tid;
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) mine[q * size] = four(dg, q), mine[(N / 4 + q) * size] = four(db, q);
     __syncthreads();
-    const int log = 31 - __clz(size);
-    for (int j = threadIdx.x; j < 2 * N * size; j += blockDim.x) {
-      float t = sums[j];
-      for (int g = 1; g < groups; ++g) t += sums[g * 2 * N * size + j];
-      const int v = j >> log, which = v >= N, u = which ? v - N : v;
-      const int col = (u / VEC * size + (j & (size - 1))) * VEC + u % VEC;
-      if (col < a.cols) part[which * a.cols + col] = t;
+    for (int q = group; q < N / 2; q += groups) {
+      float4 t = sums[q * size + tid];
+      for (int g = 1; g < groups; ++g) {
+        const float4 u = sums[g * step + q * size + tid];
+        t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+      }
+      put4(q < N / 4 ? part : part + a.cols, q < N / 4 ? q : q - N / 4, c0, a.cols, t);
     }
   }
 };
@@ -447,16 +472,17 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
   extern __shared__ __align__(128) uint8_t ring_smem[];
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
+  const int c0 = Held<T, VEC, N>::first(tid);
   Held<T, VEC, N> nx, ny;
   float next_mean = 0.f, next_rstd = 0.f;
   auto fetch = [&](long long row) {
-    nx.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, tid, size, a.cols);
-    ny.template load<false>(static_cast<const T*>(a.dy) + row * a.lddy, tid, size, a.cols);
+    nx.template load<false>(static_cast<const T*>(a.x) + row * a.ldx, c0, a.cols);
+    ny.template load<false>(static_cast<const T*>(a.dy) + row * a.lddy, c0, a.cols);
     next_mean = a.mean[row], next_rstd = a.rstd[row];
   };
   if (first < a.rows) fetch(first);
   Columns<T, P, VEC, N> c;
-  c.init(a, tid * VEC, size);
+  c.init(a, c0);
   int flip = 0;
   for (long long row = first; row < a.rows; row += step, flip ^= 1) {
     const Held<T, VEC, N> x = nx, y = ny;
@@ -464,10 +490,10 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
     if (row + step < a.rows) fetch(row + step);
     const float2 s = group_sum(c.add(x, y, mean, rstd), red[flip], size, group);
     if (a.dx)
-      c.template write<false>(x, y, static_cast<T*>(a.dx) + row * a.lddx, tid, size, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+      c.template write<false>(x, y, static_cast<T*>(a.dx) + row * a.lddx, c0, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
   grid_dependents_launch();
-  c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
+  c.finish(a, tid, size, group, groups, reinterpret_cast<float4*>(ring_smem));
 }
 
 // x and dy through the ring. The copies queued ahead of it make any other load slow
@@ -481,8 +507,9 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
   const int size = a.size, groups = kRingThreads / size, group = threadIdx.x / size, tid = threadIdx.x - group * size, lane = threadIdx.x & 31;
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
+  const int c0 = Held<T, VEC, N>::first(tid);
   Columns<T, P, VEC, N> c;
-  c.init(a, tid * VEC, size);
+  c.init(a, c0);
   float mean32, rstd32, next_mean32, next_rstd32;
   auto fetch = [&](long long row) {
     const bool here = row + lane * step < a.rows;
@@ -513,20 +540,20 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
     ring.wait(a.status);
     const uint8_t* from = ring.buf + ring.slot * ring.bytes;
     Held<T, VEC, N> hx, hy;
-    hx.template load<EXACT>(reinterpret_cast<const T*>(from + (VEC > 1 ? 0 : shift(x + row * a.ldx))), tid, size, a.cols);
-    hy.template load<EXACT>(reinterpret_cast<const T*>(from + a.pitch + (VEC > 1 ? 0 : shift(dy + row * a.lddy))), tid, size, a.cols);
+    hx.template load<EXACT>(reinterpret_cast<const T*>(from + (VEC > 1 ? 0 : shift(x + row * a.ldx))), c0, a.cols);
+    hy.template load<EXACT>(reinterpret_cast<const T*>(from + a.pitch + (VEC > 1 ? 0 : shift(dy + row * a.lddy))), c0, a.cols);
     const float2 s = group_sum(c.add(hx, hy, mean, rstd), red[flip], size, group);
     // the reduction is behind every thread's reads of the buffer
     if (tid == 0 && fill < a.rows) copy(ring.slot);
     fill += step;
     ring.next();
     if (a.dx)
-      c.template write<EXACT>(hx, hy, static_cast<T*>(a.dx) + row * a.lddx, tid, size, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+      c.template write<EXACT>(hx, hy, static_cast<T*>(a.dx) + row * a.lddx, c0, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
   }
   if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
   grid_dependents_launch();
   __syncthreads();  // the buffers are free: they take the groups' sums
-  c.finish(a, tid, size, group, groups, reinterpret_cast<float*>(ring_smem));
+  c.finish(a, tid, size, group, groups, reinterpret_cast<float4*>(ring_smem));
 }
 
 // Long rows, first pass: a block per row, its mean, rstd and two sums to `stats`.
@@ -534,6 +561,7 @@ template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
   constexpr int N = VEC > 1 ? VEC : 2;
   __shared__ float2 red[2][32];
+  const int c0 = Held<T, VEC, N>::first(threadIdx.x);
   int flip = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -544,10 +572,10 @@ __global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
 #pragma unroll 2
     for (int c = 0; c < a.cols; c += 512 * N) {
       Held<T, VEC, N> hx, hy;
-      hx.template load<false>(x + c, threadIdx.x, 512, a.cols - c);
-      hy.template load<false>(dy + c, threadIdx.x, 512, a.cols - c);
+      hx.template load<false>(x + c, c0, a.cols - c);
+      hy.template load<false>(dy + c, c0, a.cols - c);
       uint64_t g[N / 2];
-      load_params<P, VEC, N>(a.gamma, 1.f, c + threadIdx.x * VEC, 512, a.cols, g);
+      load_params<P, VEC, N>(a.gamma, 1.f, c + c0, a.cols, g);
 #pragma unroll
       for (int p = 0; p < N / 2; ++p) {
         const uint64_t w = mul2(hy.pair(p), g[p]);
@@ -566,9 +594,9 @@ constexpr int kSlabThreads = 256, kSlabRows = 4;
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
   constexpr int N = VEC > 1 ? VEC : 2;
-  const int col0 = blockIdx.x * kSlabThreads * N, tid = threadIdx.x, cols = a.cols - col0;
+  const int c0 = blockIdx.x * kSlabThreads * N + Held<T, VEC, N>::first(threadIdx.x);
   Columns<T, P, VEC, N> c;
-  c.init(a, col0 + tid * VEC, kSlabThreads);
+  c.init(a, c0);
   for (long long row0 = (long long)blockIdx.y * kSlabRows; row0 < a.rows; row0 += (long long)gridDim.y * kSlabRows) {
     Held<T, VEC, N> x[kSlabRows], y[kSlabRows];
     float4 st[kSlabRows];
@@ -576,8 +604,9 @@ __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a)
     for (int r = 0; r < kSlabRows; ++r) {
       const long long row = row0 + r;
       const bool here = row < a.rows;
-      x[r].template load<false>(static_cast<const T*>(a.x) + row * a.ldx + col0, tid, kSlabThreads, cols, here);
-      y[r].template load<false>(static_cast<const T*>(a.dy) + row * a.lddy + col0, tid, kSlabThreads, cols, here);
+      const int cols = here ? a.cols : 0;
+      x[r].template load<false>(static_cast<const T*>(a.x) + row * a.ldx, c0, cols);
+      y[r].template load<false>(static_cast<const T*>(a.dy) + row * a.lddy, c0, cols);
       st[r] = here ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
@@ -585,16 +614,16 @@ __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a)
       if (row0 + r >= a.rows) break;
       c.add(x[r], y[r], st[r].x, st[r].y);
       if (a.dx)
-        c.template write<false>(x[r], y[r], static_cast<T*>(a.dx) + (row0 + r) * a.lddx + col0, tid, kSlabThreads, cols, st[r].x, st[r].y, st[r].z,
-                                st[r].w);
+        c.template write<false>(x[r], y[r], static_cast<T*>(a.dx) + (row0 + r) * a.lddx, c0, a.cols, st[r].x, st[r].y, st[r].z, st[r].w);
     }
   }
-  float* part = a.part + (long long)blockIdx.y * 2 * a.cols + col0;
+  float* part = a.part + (long long)blockIdx.y * 2 * a.cols;
 #pragma unroll
-  for (int v = 0; v < N; ++v) {
-    const int col = (v / VEC * kSlabThreads + tid) * VEC + v % VEC;
+  for (int v = 0; v < N; v += 2) {
     const float2 g = unpair(c.dg[v / 2]), b = unpair(c.db[v / 2]);
-    if (col < cols) part[col] = v & 1 ? g.y : g.x, part[a.cols + col] = v & 1 ? b.y : b.x;
+    const int ca = c0 + (v / VEC) * 32 * VEC + v % VEC, cb = VEC > 1 ? ca + 1 : ca + 32;
+    if (ca < a.cols) part[ca] = g.x, part[a.cols + ca] = b.x;
+    if (cb < a.cols) part[cb] = g.y, part[a.cols + cb] = b.y;
   }
 }
 
