@@ -23,6 +23,7 @@
 // workspace and a second kernel (launched with programmatic dependency) adds the
 // partial rows in a fixed order, so results do not depend on timing. All sums are fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "ops_common.h"
 #include "ops_device.cuh"
@@ -83,6 +84,7 @@ struct Held {
   // the thread's first column
   static __device__ __forceinline__ int first(int tid) { return ((tid >> 5) * K * 32 + (tid & 31)) * VEC; }
   static __device__ __forceinline__ constexpr int at(int k) { return k * 32 * VEC; }
+  static __device__ __forceinline__ bool whole(int tid, int cols) { return first(tid | 31) + at(K - 1) + VEC <= cols; }
   template <bool EXACT>
   __device__ __forceinline__ void load(const T* row, int c0, int cols) {
     row += c0;
@@ -113,6 +115,16 @@ struct Held {
     return pair_of(c0 + at(2 * p / VEC) < cols ? -mean : 0.f, c0 + at((2 * p + 1) / VEC) < cols ? -mean : 0.f);
   }
 };
+
+// Runs f(true) where all of a warp's columns are inside the row, so that they need no
+// comparisons (a third of the instructions where values go one by one), else f(false).
+template <bool EXACT, typename F>
+__device__ __forceinline__ void by_whole(bool whole, F f) {
+  if (EXACT || whole)
+    f(std::true_type{});
+  else
+    f(std::false_type{});
+}
 
 // The results of a row, rounded to its type once.
 template <typename T, int VEC, int N, bool EXACT>
@@ -246,6 +258,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
   const int c0 = Held<T, VEC, N>::first(tid);
+  const bool whole = Held<T, VEC, N>::whole(tid, a.cols);
   float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols rounded up to 4]
   const int pcols = (a.cols + 3) & ~3;
   for (int c = threadIdx.x; c < a.cols; c += kRingThreads) {
@@ -268,18 +281,21 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   const long long next_y = step * a.ldy, next_x = step * a.ldx;
   for (long long row = first; row < a.rows; row += 2 * step, y += 2 * next_y, at += 2 * next_x) {
     const bool two = row + step < a.rows;
-    Held<T, VEC, N> x0, x1;  // a missing second row is zeros
+    Held<T, VEC, N> x0, x1;  // a missing second row: the first one again, not stored
     const int slot0 = ring.slot;
+    const uint8_t* from0 = ring.buf + slot0 * ring.bytes + (VEC > 1 ? 0 : shift(at));
     ring.wait(a.status);
-    x0.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at))), c0, a.cols);
-    ring.next();
+    if (two) ring.next(), ring.wait(a.status);
     const int slot1 = ring.slot;
-    if (two) ring.wait(a.status);
-    x1.template load<EXACT>(reinterpret_cast<const T*>(ring.buf + ring.slot * ring.bytes + (VEC > 1 ? 0 : shift(at + next_x))), c0, two ? a.cols : 0);
-    if (two) ring.next();
+    const uint8_t* from1 = VEC > 1 || !two ? ring.buf + slot1 * ring.bytes + (VEC > 1 ? 0 : shift(at)) : ring.buf + slot1 * ring.bytes + shift(at + next_x);
+    ring.next();
     uint64_t s0 = 0, s1 = 0;
+    by_whole<EXACT>(whole, [&](auto w) {
+      x0.template load<decltype(w)::value>(reinterpret_cast<const T*>(from0), c0, a.cols);
+      x1.template load<decltype(w)::value>(reinterpret_cast<const T*>(from1), c0, a.cols);
 #pragma unroll
-    for (int p = 0; p < N / 2; ++p) s0 = add2(s0, x0.pair(p)), s1 = add2(s1, x1.pair(p));
+      for (int p = 0; p < N / 2; ++p) s0 = add2(s0, x0.pair(p)), s1 = add2(s1, x1.pair(p));
+    });
     const float2 sum = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[0], size, group);
     const float2 mean = make_float2(sum.x * a.inv_cols, sum.y * a.inv_cols);
     // the reduction is behind every thread's reads of the buffers
@@ -289,13 +305,15 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     }
     fill += 2 * step;
     s0 = s1 = 0;
+    by_whole<EXACT>(whole, [&](auto w) {
 #pragma unroll
-    for (int p = 0; p < N / 2; ++p) {
-      const uint64_t d0 = add2(x0.pair(p), x0.template minus<EXACT>(mean.x, p, c0, a.cols));
-      const uint64_t d1 = add2(x1.pair(p), x1.template minus<EXACT>(mean.y, p, c0, a.cols));
-      s0 = fma2(d0, d0, s0);
-      s1 = fma2(d1, d1, s1);
-    }
+      for (int p = 0; p < N / 2; ++p) {
+        const uint64_t d0 = add2(x0.pair(p), x0.template minus<decltype(w)::value>(mean.x, p, c0, a.cols));
+        const uint64_t d1 = add2(x1.pair(p), x1.template minus<decltype(w)::value>(mean.y, p, c0, a.cols));
+        s0 = fma2(d0, d0, s0);
+        s1 = fma2(d1, d1, s1);
+      }
+    });
     const float2 sq = group_sum(make_float2(sum_of(s0), sum_of(s1)), red[1], size, group);
     const float2 rstd = make_float2(1.f / sqrtf(sq.x * a.inv_cols + a.eps), 1.f / sqrtf(sq.y * a.inv_cols + a.eps));
     if (tid == 0) {
@@ -304,39 +322,41 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
     }
     const uint64_t m0 = twice(-mean.x), m1 = twice(-mean.y), r0 = twice(rstd.x), r1 = twice(rstd.y);
     constexpr int C = VEC > 1 ? VEC : 2;  // values stored together
+    by_whole<EXACT>(whole, [&](auto w) {
 #pragma unroll
-    for (int q = 0; q < N / C; ++q) {
-      const int ca = c0 + Held<T, VEC, N>::at(q * C / VEC), cb = VEC > 1 ? ca + 1 : ca + Held<T, VEC, N>::at(1);
-      if (!EXACT && ca >= a.cols) continue;
-      uint64_t g[C / 2], b[C / 2], out[C / 2];
-      if constexpr (VEC > 1) {
-#pragma unroll
-        for (int i = 0; i < C / 4; ++i) {
-          const float4 u = *reinterpret_cast<const float4*>(params + ca + 4 * i), v = *reinterpret_cast<const float4*>(params + pcols + ca + 4 * i);
-          g[2 * i] = pair_of(u.x, u.y), g[2 * i + 1] = pair_of(u.z, u.w);
-          b[2 * i] = pair_of(v.x, v.y), b[2 * i + 1] = pair_of(v.z, v.w);
-        }
-      } else {
-        const bool in = cb < a.cols;
-        g[0] = pair_of(params[ca], in ? params[cb] : 0.f);
-        b[0] = pair_of(params[pcols + ca], in ? params[pcols + cb] : 0.f);
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (r == 1 && !two) break;
-#pragma unroll
-        for (int i = 0; i < C / 2; ++i)
-          out[i] = fma2(mul2(add2((r ? x1 : x0).pair(q * C / 2 + i), r ? m1 : m0), r ? r1 : r0), g[i], b[i]);
-        T* to = y + (r ? next_y : 0);
+      for (int q = 0; q < N / C; ++q) {
+        const int ca = c0 + Held<T, VEC, N>::at(q * C / VEC), cb = VEC > 1 ? ca + 1 : ca + Held<T, VEC, N>::at(1);
+        if (!decltype(w)::value && ca >= a.cols) continue;
+        uint64_t g[C / 2], b[C / 2], out[C / 2];
         if constexpr (VEC > 1) {
-          store_pairs<T, VEC>(to + ca, out);
+#pragma unroll
+          for (int i = 0; i < C / 4; ++i) {
+            const float4 u = *reinterpret_cast<const float4*>(params + ca + 4 * i), v = *reinterpret_cast<const float4*>(params + pcols + ca + 4 * i);
+            g[2 * i] = pair_of(u.x, u.y), g[2 * i + 1] = pair_of(u.z, u.w);
+            b[2 * i] = pair_of(v.x, v.y), b[2 * i + 1] = pair_of(v.z, v.w);
+          }
         } else {
-          const float2 f = unpair(out[0]);
-          from_f32(f.x, to + ca);
-          if (cb < a.cols) from_f32(f.y, to + cb);
+          const bool in = decltype(w)::value || cb < a.cols;
+          g[0] = pair_of(params[ca], in ? params[cb] : 0.f);
+          b[0] = pair_of(params[pcols + ca], in ? params[pcols + cb] : 0.f);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (r == 1 && !two) break;
+#pragma unroll
+          for (int i = 0; i < C / 2; ++i)
+            out[i] = fma2(mul2(add2((r ? x1 : x0).pair(q * C / 2 + i), r ? m1 : m0), r ? r1 : r0), g[i], b[i]);
+          T* to = y + (r ? next_y : 0);
+          if constexpr (VEC > 1) {
+            store_pairs<T, VEC>(to + ca, out);
+          } else {
+            const float2 f = unpair(out[0]);
+            from_f32(f.x, to + ca);
+            if (decltype(w)::value || cb < a.cols) from_f32(f.y, to + cb);
+          }
         }
       }
-    }
+    });
   }
   if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
 }
@@ -508,6 +528,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
   const long long first = (long long)blockIdx.x * groups + group, step = (long long)gridDim.x * groups;
   const uint32_t bytes = uint32_t(a.cols) * sizeof(T);
   const int c0 = Held<T, VEC, N>::first(tid);
+  const bool whole = Held<T, VEC, N>::whole(tid, a.cols);
   Columns<T, P, VEC, N> c;
   c.init(a, c0);
   float mean32, rstd32, next_mean32, next_rstd32;
@@ -518,8 +539,12 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
   };
   fetch(first);
   Ring ring = make_ring(ring_smem, full, a, groups, group, 2 * a.pitch);
-  const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
   long long fill = first;
+  const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+  const long long next_dx = step * a.lddx;
+  uint32_t sx = shift(x + first * a.ldx), sy = shift(dy + first * a.lddy);  // of this row, modulo 16
+  const uint32_t next_sx = uint32_t(step * a.ldx) * uint32_t(sizeof(T)), next_sy = uint32_t(step * a.lddy) * uint32_t(sizeof(T));
+  T* dx = static_cast<T*>(a.dx) + (a.dx ? first * a.lddx : 0);
   auto copy = [&](int slot) {
     const T *fx = x + fill * a.ldx, *fy = dy + fill * a.lddy;
     const uint32_t nx = granules(fx, bytes), ny = granules(fy, bytes);
@@ -539,16 +564,22 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
     const float mean = __shfl_sync(0xffffffffu, mean32, at), rstd = __shfl_sync(0xffffffffu, rstd32, at);
     ring.wait(a.status);
     const uint8_t* from = ring.buf + ring.slot * ring.bytes;
+    const T *rx = reinterpret_cast<const T*>(from + (VEC > 1 ? 0 : sx & 15)), *ry = reinterpret_cast<const T*>(from + a.pitch + (VEC > 1 ? 0 : sy & 15));
     Held<T, VEC, N> hx, hy;
-    hx.template load<EXACT>(reinterpret_cast<const T*>(from + (VEC > 1 ? 0 : shift(x + row * a.ldx))), c0, a.cols);
-    hy.template load<EXACT>(reinterpret_cast<const T*>(from + a.pitch + (VEC > 1 ? 0 : shift(dy + row * a.lddy))), c0, a.cols);
+    by_whole<EXACT>(whole, [&](auto w) {
+      hx.template load<decltype(w)::value>(rx, c0, a.cols);
+      hy.template load<decltype(w)::value>(ry, c0, a.cols);
+    });
     const float2 s = group_sum(c.add(hx, hy, mean, rstd), red[flip], size, group);
     // the reduction is behind every thread's reads of the buffer
     if (tid == 0 && fill < a.rows) copy(ring.slot);
-    fill += step;
+    fill += step, sx += next_sx, sy += next_sy;
     ring.next();
     if (a.dx)
-      c.template write<EXACT>(hx, hy, static_cast<T*>(a.dx) + row * a.lddx, c0, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+      by_whole<EXACT>(whole, [&](auto w) {
+        c.template write<decltype(w)::value>(hx, hy, dx, c0, a.cols, mean, rstd, s.x * a.inv_cols, s.y * a.inv_cols);
+      });
+    dx += next_dx;
   }
   if (tid == 0) ring.drain((min(fill, a.rows + step - 1) - first) / step);
   grid_dependents_launch();
