@@ -27,6 +27,15 @@
 // When there are few tiles, the CTAs of a cluster split K between them and add their
 // accumulators through distributed shared memory in rank order.
 //
+// What bounds it. 8192 x 4096 x 4096 with 128 x 128 blocks of b takes 134 us (2.05
+// PFLOP/s), with a scale per column 180 us; the same pipeline without the promotion
+// takes 104 us, which is the tensor cores under the power limit. A block of K (512 MMA
+// cycles) is bounded by its turn through one of the two TMEM accumulators that fit: the
+// MMAs, the epilogue's reads, and a release and an acquire through shared memory of 150
+// to 250 cycles each while MMAs run. That is why one issuer hands over all 256 columns
+// at once: two issuers with 128 columns each took 139 us, and parts that every epilogue
+// warp shares 170 us.
+//
 // Every wait is bounded (2 s); one that runs out sets a status word that
 // pkt_ops_status reads, and the kernel drains its copies and returns.
 #include <algorithm>
@@ -58,8 +67,6 @@ struct alignas(64) Fp8Args {
 
 template <int BN, int PAIR>
 struct Shape {
-  static constexpr int kHalves = BN > 128 ? 2 : 1;   // MMA issuers, each with its part of the columns
-  static constexpr int kPart = BN / kHalves;         // columns of an issuer
   static constexpr int kSides = BN > 64 ? 2 : 1;     // epilogue warps per 32 lanes
   static constexpr int kCols = BN / kSides;          // columns of an epilogue warp
   static constexpr int kEpiWarps = 4 * kSides;
@@ -68,7 +75,7 @@ struct Shape {
   static constexpr int kColBytes = BN / PAIR * kKBytes;
   static constexpr int kStageBytes = kRowBytes + kColBytes;
   static constexpr int kStages = kStageBytes >= 32768 ? 5 : 8;
-  static constexpr int kBufs = BN > 128 ? 2 : 4;     // TMEM accumulators of each half
+  static constexpr int kBufs = BN > 128 ? 2 : 4;     // TMEM accumulators
   static constexpr int kTmemCols = kBufs * BN < 32 ? 32 : kBufs * BN;
   static constexpr int kChunk = kCols < 32 ? kCols : 32;  // columns per TMEM load, two in flight
   static constexpr bool kStore = BN >= 128;          // the result leaves by TMA stores
@@ -82,11 +89,11 @@ struct Smem {
   uint8_t stages[S::kStages][S::kStageBytes];
   uint8_t staging[S::kStore ? S::kEpiWarps : 1][S::kStore ? 4096 : 16];  // 32 rows x 128 bytes of the result
   float row_scale[S::kScales][S::kGroup][kRows];
-  float col_scale[S::kScales][S::kGroup][BN];  // of every column, or one for each half's columns
+  float col_scale[S::kScales][S::kGroup][BN];  // of every column, or of every 128
   uint64_t sfull[S::kScales], sempty[S::kScales];
   uint64_t full[S::kStages], empty[S::kStages];
-  uint64_t tfull[S::kHalves][S::kBufs], tempty[S::kHalves][S::kBufs];
-  uint64_t drain[S::kHalves];
+  uint64_t tfull[S::kBufs], tempty[S::kBufs];
+  uint64_t drain;
   uint32_t tmem;
   int abort;
 };
@@ -246,11 +253,10 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   const uint32_t half = PAIR == 2 ? rank : 0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], S::kHalves);
+    for (int i = 0; i < S::kStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
     for (int i = 0; i < S::kScales; ++i) mbar_init(&s.sfull[i], 32), mbar_init(&s.sempty[i], S::kEpiWarps);
-    for (int h = 0; h < S::kHalves; ++h)
-      for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[h][i], 1), mbar_init(&s.tempty[h][i], S::kEpiWarps / S::kHalves * PAIR);
-    for (int h = 0; h < S::kHalves; ++h) mbar_init(&s.drain[h], 1);
+    for (int i = 0; i < S::kBufs; ++i) mbar_init(&s.tfull[i], 1), mbar_init(&s.tempty[i], S::kEpiWarps * PAIR);
+    mbar_init(&s.drain, 1);
     s.abort = 0;
     fence_mbar_init();
   }
@@ -270,18 +276,18 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   const int first = int(blockIdx.x / cluster_size), step = int(gridDim.x / cluster_size);
   const int kb0 = int((long long)a.num_kb * part / split), kb1 = int((long long)a.num_kb * (part + 1) / split);
 
-  // With two column halves, 12 warps are launched with 168 registers each: the
+  // In 256-wide tiles 12 warps are launched with 168 registers each: the
   // epilogue warps, whose accumulators take 128, get 232 and the other four 40
   // (8 x 232 + 4 x 40 = 12 x 168)
   if (warp == S::kEpiWarps) {
     // ---- producer: one lane
-    if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (BN > 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     uint32_t stage = 0, phase = 0, issued = 0;
     bool ok = true;
     for (int t = first; ok && t < tiles; t += step) {
       int tr, tc;
       tile_at(t, a.tiles_r, a.tiles_c, &tr, &tc);
-      const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (S::kPart / PAIR);
+      const int r0 = (tr * PAIR + int(half)) * kRows, c0 = tc * BN + int(half) * (BN / PAIR);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = wait_phase(&s.empty[stage], phase ^ 1, a.status, &s.abort))) break;
         if (elect_one()) {
@@ -290,9 +296,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
           if (PAIR == 2) {
             const uint32_t bar = mapa_shared(smem_u32(&s.full[stage]), 0);  // both CTAs' bytes count on the leader's barrier
             tma_load_2d_pair(to, &a.map_r, bar, kb * kKBytes, r0);
-#pragma unroll
-            for (int h = 0; h < S::kHalves; ++h)  // each half's columns come from both CTAs
-              tma_load_2d_pair(to + S::kRowBytes + h * (S::kColBytes / S::kHalves), &a.map_c, bar, kb * kKBytes, c0 + h * S::kPart);
+            tma_load_2d_pair(to + S::kRowBytes, &a.map_c, bar, kb * kKBytes, c0);
           } else {
             tma_load_2d(to, &a.map_r, &s.full[stage], kb * kKBytes, r0);
             tma_load_2d(to + S::kRowBytes, &a.map_c, &s.full[stage], kb * kKBytes, c0);
@@ -311,11 +315,9 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       try_phase(&s.full[fill % S::kStages], (fill / S::kStages) & 1);
     }
     __syncwarp();
-  } else if (warp == S::kEpiWarps + 1 || (S::kHalves == 2 && warp == S::kEpiWarps + 3)) {
-    // ---- MMA issuers, in the leader CTA: a warp per half, as issuing a block's MMAs
-    // and commits takes about as long as running them; one lane issues
-    if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    const int h = warp == S::kEpiWarps + 1 ? 0 : 1;
+  } else if (warp == S::kEpiWarps + 1) {
+    // ---- MMA issuer, in the leader CTA; one lane issues
+    if (BN > 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (half == 0) {
       uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
       uint32_t loaded = 0, drained = 0;  // the next block's barriers were found complete
@@ -324,24 +326,24 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       for (int t = first; ok && t < tiles; t += step) {
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!__all_sync(0xffffffffu, loaded)) ok = wait_phase(&s.full[stage], phase, a.status, &s.abort);
-          if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[h][buf], bphase ^ 1, a.status, &s.abort);
+          if (ok && !__all_sync(0xffffffffu, drained)) ok = wait_phase(&s.tempty[buf], bphase ^ 1, a.status, &s.abort);
           if (!ok) break;
-          const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes + h * (S::kColBytes / S::kHalves);
-          const uint32_t to = tmem + (buf * S::kHalves + h) * S::kPart;
+          const uint32_t sr = smem_u32(s.stages[stage]), sc = sr + S::kRowBytes;
+          const uint32_t to = tmem + buf * BN;
           const uint32_t now = stage, nbuf = buf;
           if (++stage == S::kStages) stage = 0, phase ^= 1;
           if (++buf == S::kBufs) buf = 0, bphase ^= 1;
           loaded = peek_phase(&s.full[stage], phase);
-          drained = peek_phase(&s.tempty[h][buf], bphase ^ 1);
+          drained = peek_phase(&s.tempty[buf], bphase ^ 1);
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mma_fp8<PAIR>(to, hi | uint64_t((sr + 32 * k) >> 4), hi | uint64_t((sc + 32 * k) >> 4), a.idesc, k > 0);
             if (PAIR == 2)
-              mma_commit_pair_both(&s.tfull[h][nbuf]), mma_commit_pair_both(&s.empty[now]);
+              mma_commit_pair_both(&s.tfull[nbuf]), mma_commit_pair_both(&s.empty[now]);
             else
-              mma_commit(&s.tfull[h][nbuf]), mma_commit(&s.empty[now]);
+              mma_commit(&s.tfull[nbuf]), mma_commit(&s.empty[now]);
           }
           __syncwarp();
           any = true;
@@ -350,19 +352,19 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
       if (any) {  // no MMA is in flight when TMEM is released
         if (elect_one()) {
           if (PAIR == 2)
-            mma_commit_pair_local(&s.drain[h]);
+            mma_commit_pair_local(&s.drain);
           else
-            mma_commit(&s.drain[h]);
+            mma_commit(&s.drain);
         }
         __syncwarp();
-        try_phase(&s.drain[h], 0);
+        try_phase(&s.drain, 0);
       }
     }
     __syncwarp();
   } else if (warp < S::kEpiWarps) {
     // ---- epilogue
-    if (S::kHalves == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    const int quad = warp & 3, side = warp >> 2, part_h = side * S::kCols / S::kPart;
+    if (BN > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int quad = warp & 3, side = warp >> 2;
     // where this lane's values lie in the warp's 32 rows: value v of chunk j
     auto row_of = [&](int v) { return COLV ? v / (S::kChunk / 2) * 16 + (v >> 1 & 1) * 8 + (lane >> 2) : lane; };
     auto col_of = [&](int j, int v) {
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
         if (in == 0 && !wait_phase(&s.sfull[at], ph, a.status, &s.abort)) return false;
 #pragma unroll
         for (int i = 0; i < R; ++i) next_r[i] = s.row_scale[at][in][quad * 32 + (COLV ? 8 * i + (lane >> 2) : lane)];
-        if (!COLV) next_c = s.col_scale[at][in][part_h];
+        if (!COLV) next_c = s.col_scale[at][in][side * S::kCols / kScaleBlock];
         return true;
       };
       uint32_t ready = 0;
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
 #pragma unroll
         for (int i = 0; i < R; ++i) scale[i] = next_r[i] * next_c;
         const float* cs = &s.col_scale[slot][in][side * S::kCols + 2 * (lane & 3)];
-        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[part_h][buf], bphase, a.status, &s.abort);
+        if (!__all_sync(0xffffffffu, ready)) ok = wait_phase(&s.tfull[buf], bphase, a.status, &s.abort);
         if (!ok) break;
         tc_fence_after();
         const uint32_t from = tmem + buf * BN + side * S::kCols + (uint32_t(quad * 32) << 16);
@@ -427,14 +429,14 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
 #pragma unroll
           for (int h = 0; h < kSplit; ++h) tmem_wait(v[j & 1][h]);
           if (j + 1 == kLoads) {  // all of the buffer is in registers
-            ready = peek_phase(&s.tfull[part_h][buf + 1 == S::kBufs ? 0 : buf + 1], buf + 1 == S::kBufs ? bphase ^ 1 : bphase);
+            ready = peek_phase(&s.tfull[buf + 1 == S::kBufs ? 0 : buf + 1], buf + 1 == S::kBufs ? bphase ^ 1 : bphase);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
               if (PAIR == 2 && half != 0)
-                arrive_peer(mapa_shared(smem_u32(&s.tempty[part_h][buf]), 0));
+                arrive_peer(mapa_shared(smem_u32(&s.tempty[buf]), 0));
               else
-                mbar_arrive(&s.tempty[part_h][buf]);
+                mbar_arrive(&s.tempty[buf]);
             }
           } else {
             load(j + 1);
@@ -477,14 +479,16 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
             *reinterpret_cast<float2*>(sums + r * (BN + 4) + c) = f;
           }
         }
-      } else if (S::kStore && a.tma_out) {
-        // 32 rows x 128 bytes at a time through swizzled shared memory
+      } else if constexpr (S::kStore) {
+        // 32 rows x 128 bytes at a time through swizzled shared memory, then a TMA store, or
+        // (rows that do not start on 16 bytes) row by row, 32 neighbouring values at once: a
+        // lane's own values of a row, stored one by one, made 1500x1500x2048 take 34 us instead of 14.5 us
         uint8_t* to = s.staging[S::kStore ? warp : 0];
         const int per = a.out_bf16 ? 64 : 32;
 #pragma unroll
         for (int j = 0; j < S::kCols / 32; ++j) {
           if (!a.out_bf16 || (j & 1) == 0) {
-            if (lane == 0) bulk_wait_read_all();  // the last store has left the staging
+            if (lane == 0) bulk_wait_read_all();  // the last TMA store has left the staging
             __syncwarp();
           }
           if constexpr (COLV) {
@@ -514,12 +518,30 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
             }
           }
           if (!a.out_bf16 || (j & 1) == 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
             const int col = col0 + j * 32 + 32 - per;
-            if (lane == 0 && row0 < a.rows && col < a.cols) {
-              tma_store_2d(&a.map_out, to, col, row0);
-              bulk_commit();
+            if (a.tma_out) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0 && row0 < a.rows && col < a.cols) {
+                tma_store_2d(&a.map_out, to, col, row0);
+                bulk_commit();
+              }
+            } else {
+              __syncwarp();
+              const int rows = min(32, a.rows - row0);
+#pragma unroll 4
+              for (int r = 0; r < rows; ++r) {
+                const uint8_t* from = to + r * 128;
+                const long long off = (long long)(row0 + r) * a.ldo + col;
+                if (a.out_bf16) {
+#pragma unroll
+                  for (int i = lane; i < 64; i += 32)
+                    if (col + i < a.cols)
+                      static_cast<uint16_t*>(a.out)[off + i] = *reinterpret_cast<const uint16_t*>(from + (((i >> 3) ^ (r & 7)) << 4) + (i & 7) * 2);
+                } else if (col + lane < a.cols) {
+                  static_cast<float*>(a.out)[off + lane] = *reinterpret_cast<const float*>(from + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                }
+              }
             }
           }
         }
@@ -536,7 +558,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
     if (S::kStore && a.tma_out && lane == 0) bulk_wait_all();
   } else {
     // ---- scales: a warp copies those of the tile's rows and columns, blocks ahead
-    if (S::kHalves == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (BN > 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == S::kEpiWarps + 2) {
       uint32_t slot = 0, phase = 0;
       bool ok = true;
@@ -562,8 +584,8 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
               const int col = col0 + lane + i;
               if (BN >= 32 || lane < BN) copy_word_async(&s.col_scale[slot][in][lane + i], pc + min(col, a.cols - 1), col < a.cols);
             }
-          } else if (lane < S::kHalves) {
-            const int col = col0 + lane * S::kPart;
+          } else if (lane < (BN + 127) / 128) {
+            const int col = col0 + lane * kScaleBlock;
             copy_word_async(&s.col_scale[slot][in][lane], pc + (min(col, a.cols - 1) >> 7), col < a.cols);
           }
           if (in == S::kGroup - 1 || kb == kb1 - 1) {
@@ -729,7 +751,7 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
     while (split < 8 && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
   const void *pr = swap ? d->b : d->a, *pc = swap ? d->a : d->b;
   if ((rc = operand_map(&a.map_r, pr, d->K, a.rows, swap ? d->ldb : d->lda, kRows)) ||
-      (rc = operand_map(&a.map_c, pc, d->K, a.cols, swap ? d->lda : d->ldb, (bn > 128 ? 128 : bn) / pair)))
+      (rc = operand_map(&a.map_c, pc, d->K, a.cols, swap ? d->lda : d->ldb, bn / pair)))
     return rc;
   a.scale_r = swap ? d->scale_b : d->scale_a, a.ld_r = swap ? d->ld_scale_b : d->ld_scale_a;
   a.scale_c = swap ? d->scale_a : d->scale_b, a.ld_c = swap ? d->ld_scale_a : d->ld_scale_b;
@@ -743,7 +765,7 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
     a.tma_out = 1;
   }
   const uint32_t fr = (swap ? d->b_dtype : d->a_dtype) == PKT_DTYPE_E5M2, fc = (swap ? d->a_dtype : d->b_dtype) == PKT_DTYPE_E5M2;
-  a.idesc = (1u << 4) | (fr << 7) | (fc << 10) | (uint32_t((bn > 128 ? 128 : bn) >> 3) << 17) | (uint32_t((kRows * pair) >> 4) << 24);
+  a.idesc = (1u << 4) | (fr << 7) | (fc << 10) | (uint32_t(bn >> 3) << 17) | (uint32_t((kRows * pair) >> 4) << 24);
   // a cluster per tile when K is split, else a persistent grid
   const int clusters = split > 1 ? int(tiles) : int(std::min<long long>(tiles, sms / pair));
   const int cs = pair == 2 ? 2 : split;
