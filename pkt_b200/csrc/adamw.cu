@@ -71,6 +71,7 @@ __device__ __forceinline__ void adam_advance(AdamState* s, double beta1, double 
 }
 
 __global__ void adam_set_state(AdamState* s, double pow1, double pow2, long long step, double beta1, double beta2) {
+  grid_dependency_wait();
   s->pow1 = pow1;
   s->pow2 = pow2;
   s->step = step;
@@ -219,6 +220,7 @@ __device__ __forceinline__ void adam_blocks(const AdamArgs& a, const AdamTensor&
 
 template <typename P, typename G, bool EIGHT>
 __global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 2) adam_step(const AdamArgs a) {
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float lr = a.scales ? a.lr * a.scales[0] : a.lr;
   AdamStep u;
@@ -291,7 +293,7 @@ struct AdamW {
     return op_check_memory(g, "grad", device);
   }
   int set_step(long long step, cudaStream_t st) {
-    const cudaError_t e = op_launch(adam_set_state, dim3(1), dim3(1), 0, st, false, d_state, std::pow(beta1, double(step)),
+    const cudaError_t e = op_launch(adam_set_state, dim3(1), dim3(1), 0, st, d_state, std::pow(beta1, double(step)),
                                     std::pow(beta2, double(step)), step, beta1, beta2);
     return e == cudaSuccess ? PKT_OK : cuda_fail(e, "set the AdamW step");
   }
@@ -353,8 +355,8 @@ int AdamW::setup(const pkt_adamw_config& c) {
 
 template <typename P, typename G>
 cudaError_t adam_launch(const AdamArgs& a, bool eight, int blocks, cudaStream_t st) {
-  return eight ? op_launch(adam_step<P, G, true>, dim3(blocks), dim3(kAdamThreads), 0, st, false, a)
-               : op_launch(adam_step<P, G, false>, dim3(blocks), dim3(kAdamThreads), 0, st, false, a);
+  return eight ? op_launch(adam_step<P, G, true>, dim3(blocks), dim3(kAdamThreads), 0, st, a)
+               : op_launch(adam_step<P, G, false>, dim3(blocks), dim3(kAdamThreads), 0, st, a);
 }
 
 int AdamW::run(float lr, float grad_scale, const float* scales, cudaStream_t st) {

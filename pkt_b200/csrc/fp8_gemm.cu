@@ -271,6 +271,8 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
   if (cluster_size > 1) cluster_sync();  // the barriers of the whole cluster exist
   tc_fence_after();
   const uint32_t tmem = s.tmem;
+  grid_dependents_launch();  // a product behind this one may set up as far as here on the SMs left over
+  grid_dependency_wait();    // nothing of global memory has been touched yet
 
   const int tiles = a.tiles_r * a.tiles_c;
   const int first = int(blockIdx.x / cluster_size), step = int(gridDim.x / cluster_size);
@@ -670,7 +672,9 @@ int fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaSt
   static std::atomic<uint64_t> done;
   const int rc = op_shared_memory(reinterpret_cast<const void*>(fp8_gemm_kernel<BN, PAIR, COLV>), &done, dev, smem);
   if (rc) return rc;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // as in op_launch
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(cluster_size);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -680,7 +684,7 @@ int fp8_launch(const Fp8Args& a, int dev, int clusters, int cluster_size, cudaSt
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, PAIR, COLV>, a);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch fp8 gemm");
 }

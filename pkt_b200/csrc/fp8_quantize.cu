@@ -156,6 +156,7 @@ __device__ __forceinline__ void quantize_each_row(const QuantArgs& a, long long 
 // 17.2 us with 8 blocks and 17.7 us with 6; fp32 32.6 us with 8 and 26.4 us with 6.
 template <typename T, bool WIDE, bool E5M2, int N>
 __global__ void __launch_bounds__(128, N < 16 ? 1 : sizeof(T) == 2 ? 8 : 6) quantize_rows(const QuantArgs a) {
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, kb = blockIdx.x, col = kb * kScaleBlock + 4 * lane;
   const long long groups = ((long long)a.rows + N - 1) / N;
   for (long long g = (long long)blockIdx.y * 4 + (threadIdx.x >> 5); g < groups; g += (long long)gridDim.y * 4) {
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(128, N < 16 ? 1 : sizeof(T) == 2 ? 8 : 6) quan
 // 4096x1024 in 128 x 128 blocks 6.6 us with 2 and 6.9 us with 3, which spill.
 template <typename T, bool WIDE, bool E5M2>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile(const QuantArgs a) {
+  grid_dependency_wait();
   __shared__ __align__(16) uint32_t col_big[8][128];
   __shared__ __align__(16) float col_factor[128];
   __shared__ uint32_t tile_big[8];
@@ -264,11 +266,11 @@ cudaError_t quantize_run(const QuantArgs& a, int sms, cudaStream_t st) {
     const int rows = many ? 64 : 16;
     const dim3 grid(kbs, unsigned(std::min((a.rows - 1) / rows + 1, 65535)));
     if constexpr (WIDE)
-      if (many) return op_launch(quantize_rows<T, true, E5M2, 16>, grid, dim3(128), 0, st, false, a);
-    return op_launch(quantize_rows<T, WIDE, E5M2, 4>, grid, dim3(128), 0, st, false, a);
+      if (many) return op_launch(quantize_rows<T, true, E5M2, 16>, grid, dim3(128), 0, st, a);
+    return op_launch(quantize_rows<T, WIDE, E5M2, 4>, grid, dim3(128), 0, st, a);
   }
   const int tiles = (a.rows - 1) / 128 + 1;
-  return op_launch(quantize_tile<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(tiles, 65535))), dim3(256), 0, st, false, a);
+  return op_launch(quantize_tile<T, WIDE, E5M2>, dim3(kbs, unsigned(std::min(tiles, 65535))), dim3(256), 0, st, a);
 }
 
 template <typename T>

@@ -218,6 +218,7 @@ __device__ __forceinline__ void put_stats(const LnArgs& a, long long row, float 
 
 template <typename T, typename P, int VEC, int N>
 __global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
+  grid_dependency_wait();
   __shared__ float2 red[2][32];
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
   for (long long row = (long long)blockIdx.x * groups + group; row < a.rows; row += (long long)gridDim.x * groups) {
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(1024) ln_forward(const LnArgs a) {
 // thirds of that), 19 with 16, 12 like this (8192 x 4096 bf16: 43, 33 and 26 us).
 template <typename T, typename P, int VEC, int N, bool EXACT>
 __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) {
+  grid_dependency_wait();
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
   __shared__ float2 red[2][32];
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
 // (the second and third time from L2).
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(1024) ln_forward_long(const LnArgs a) {
+  grid_dependency_wait();
   constexpr int N = VEC > 1 ? VEC : 2;
   __shared__ float2 red[2][32];
   const int c0 = Held<T, VEC, N>::first(threadIdx.x);
@@ -488,6 +491,7 @@ struct Columns {
 // Few rows: direct loads, the next row's issued before this row's reduction.
 template <typename T, typename P, int VEC, int N>
 __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
+  grid_dependency_wait();
   __shared__ float2 red[2][32];
   extern __shared__ __align__(128) uint8_t ring_smem[];
   const int size = a.size, groups = blockDim.x / size, group = threadIdx.x / size, tid = threadIdx.x - group * size;
@@ -521,6 +525,7 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
 // rstd are loaded 32 rows at a time, one row per lane, 32 rows ahead.
 template <typename T, typename P, int VEC, int N, bool EXACT>
 __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a) {
+  grid_dependency_wait();
   extern __shared__ __align__(128) uint8_t ring_smem[];
   __shared__ uint64_t full[kRingThreads / 32][kMaxSlots];
   __shared__ float2 red[2][32];
@@ -590,6 +595,7 @@ __global__ void __launch_bounds__(kRingThreads) ln_backward_ring(const LnArgs a)
 // Long rows, first pass: a block per row, its mean, rstd and two sums to `stats`.
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
+  grid_dependency_wait();
   constexpr int N = VEC > 1 ? VEC : 2;
   __shared__ float2 red[2][32];
   const int c0 = Held<T, VEC, N>::first(threadIdx.x);
@@ -624,6 +630,7 @@ __global__ void __launch_bounds__(512) ln_row_sums(const LnArgs a) {
 constexpr int kSlabThreads = 256, kSlabRows = 4;
 template <typename T, typename P, int VEC>
 __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a) {
+  grid_dependency_wait();
   constexpr int N = VEC > 1 ? VEC : 2;
   const int c0 = blockIdx.x * kSlabThreads * N + Held<T, VEC, N>::first(threadIdx.x);
   Columns<T, P, VEC, N> c;
@@ -661,8 +668,8 @@ __global__ void __launch_bounds__(kSlabThreads) ln_backward_slab(const LnArgs a)
 // dgamma / dbeta = the partial rows added in order: 32 columns per block, the
 // partial rows dealt to 32 warps, their sums added in warp order.
 __global__ void __launch_bounds__(1024) ln_column_sums(const float* part, int parts, int cols, float* dgamma, float* dbeta) {
-  __shared__ float2 sums[32][33];
   grid_dependency_wait();
+  __shared__ float2 sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float2 s = make_float2(0.f, 0.f);
   if (col < cols) {
@@ -765,7 +772,7 @@ template <typename... KArgs>
 int ln_launch(void (*kernel)(KArgs...), std::atomic<uint64_t>* done, int dev, const LnArgs& a, const LnPlan& p, unsigned blocks, cudaStream_t st) {
   const int rc = done ? op_shared_memory(reinterpret_cast<const void*>(kernel), done, dev, kSharedMax) : PKT_OK;
   if (rc) return rc;
-  const cudaError_t e = op_launch(kernel, dim3(blocks), dim3(p.threads), p.smem, st, false, a);
+  const cudaError_t e = op_launch(kernel, dim3(blocks), dim3(p.threads), p.smem, st, a);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
 }
 
@@ -800,14 +807,14 @@ template <typename T, typename P, int VEC>
 int ln_pick(const LnArgs& a, const LnPlan& p, bool backward, int dev, int sms, cudaStream_t st) {
   if (p.n == 0) {
     if (!backward) {
-      const cudaError_t e = op_launch(ln_forward_long<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(1024), 0, st, false, a);
+      const cudaError_t e = op_launch(ln_forward_long<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(1024), 0, st, a);
       return e == cudaSuccess ? PKT_OK : cuda_fail(e, "launch layer norm");
     }
     const int slabs = (a.cols - 1) / (kSlabThreads * (VEC > 1 ? VEC : 2)) + 1;
     const long long want = std::max(1LL, 8LL * sms / slabs);  // about 8 blocks of 256 threads per SM
     const int rows = int(std::min<long long>({want, a.parts, (a.rows - 1) / kSlabRows + 1}));
-    cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(512), 0, st, false, a);
-    if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(slabs, rows), dim3(kSlabThreads), 0, st, false, a);
+    cudaError_t e = op_launch(ln_row_sums<T, P, VEC>, dim3(ln_blocks(a.rows)), dim3(512), 0, st, a);
+    if (e == cudaSuccess) e = op_launch(ln_backward_slab<T, P, VEC>, dim3(slabs, rows), dim3(kSlabThreads), 0, st, a);
     return e == cudaSuccess ? rows : cuda_fail(e, "launch layer norm");
   }
   switch (p.n) {
@@ -936,7 +943,7 @@ int pkt_layernorm_backward(const pkt_layernorm_desc* d, void* stream) {
                                   : ln_dispatch<float>(a, p, d->param_dtype, true, dev, sms, st);
   if (rc < 0) return rc;
   if (d->dgamma || d->dbeta) {
-    const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, true, static_cast<const float*>(a.part), rc,
+    const cudaError_t e = op_launch(ln_column_sums, dim3((d->cols - 1) / 32 + 1), dim3(1024), 0, st, static_cast<const float*>(a.part), rc,
                                     a.cols, d->dgamma, d->dbeta);
     if (e != cudaSuccess) return cuda_fail(e, "launch layer norm column sums");
   }

@@ -36,23 +36,21 @@ struct RelaxedCapture {
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// One launch; `dependent`: programmatic dependent launch (the kernel starts its
-// preamble early and waits for the grid before it itself, griddepcontrol.wait).
+// One launch, with programmatic stream serialization: it is made while the kernel before
+// it still drains, and each kernel here begins with griddepcontrol.wait, which waits for
+// all of that kernel and its memory (0.2 to 0.5 us of a call in a graph).
 template <typename... KArgs, typename... Args>
-cudaError_t op_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool dependent,
-                      Args... args) {
+cudaError_t op_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  if (dependent) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 

@@ -246,6 +246,46 @@ def test_layer_step_with_update_in_a_graph(pk):
         assert torch.equal(p, q)
 
 
+def test_captured_behind_copies_and_joins(pk):
+    """Operators as the first node of a graph, behind a copy and behind two kernels at once."""
+    rows, cols = 2000, 1024
+    x, y, z, w = (torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16) for _ in range(4))
+    host = torch.randn(rows, cols, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).pin_memory()
+
+    def norm(a, b, stream):
+        pk.layernorm_forward(pk.LayerNormDesc(rows=rows, cols=cols, dtype=pk.DTYPE_BF16, param_dtype=pk.DTYPE_F32, eps=1e-5,
+                                              x=a.data_ptr(), ldx=cols, y=b.data_ptr(), ldy=cols), stream.cuda_stream)
+
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    forked, joined = torch.cuda.Event(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        norm(x, y, s)
+        x.copy_(host, non_blocking=True)
+        norm(x, y, s)
+        forked.record(s)
+        t.wait_event(forked)
+        with torch.cuda.stream(t):
+            torch.mul(x, 2, out=w)
+            joined.record(t)
+        y.mul_(1.5)
+        s.wait_event(joined)
+        norm(y, z, s)
+        y.zero_()  # after the reads of the call before
+    for _ in range(50):
+        g.replay()
+    torch.cuda.synchronize()
+    def want(v):
+        c = v.double() - v.double().mean(1, keepdim=True)
+        return c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5)
+    first = (want(host.cuda()).to(torch.bfloat16) * 1.5)
+    # y is one rounding of its type from the formula, 1.5 y another; z one more: 3 half steps of values below 8,
+    # each through the second norm at most once (its scale is 1 / 1.5)
+    assert torch.all((z.double() - want(first)).abs() <= 3 * 2.0 ** -8 * (1 + want(first).abs()))
+    assert torch.all(y == 0)
+
+
 def test_first_calls_inside_a_capture():
     """A process whose first call of each operator is captured into a graph."""
     import subprocess
