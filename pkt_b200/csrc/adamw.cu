@@ -2,9 +2,6 @@
 //
 // Bound by memory: 28 bytes per parameter with fp32 states (parameter, m and v read
 // and written, gradient read), 16 1/8 with 8-bit states, 2 more for a bf16 copy.
-// Measured (6.55 TB/s: a plain copy): 41.9 million parameters, fp32 states and a bf16
-// copy 199 us, 6.32 TB/s; 268 million, 8-bit states and a copy 810 us, 6.0 TB/s; 5.3
-// million in 6 tensors, 8-bit states 20.8 us, 4.2 TB/s (launch and the loads' latency).
 // The tensors are cut into chunks of 4096 values, listed once in device memory; a
 // block takes every gridDim-th chunk, and within it a warp owns blocks of 128 values,
 // 4 per lane, so that a block of 8-bit states is quantised with one warp reduction.
@@ -35,7 +32,6 @@ namespace {
 
 constexpr int kChunk = 4096;
 constexpr int kAdamThreads = 256;
-constexpr int kListed = 16;  // chunks whose records a block fetches together
 constexpr int kBlocksPerWarp = kChunk / kScaleBlock / (kAdamThreads / 32);
 
 struct AdamTensor {
@@ -231,34 +227,16 @@ __global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 2) adam_step(const A
   u.gs = a.scales ? a.grad_scale * a.scales[1] : a.grad_scale;
   u.step_size = lr * a.state->inv_bc1;
   u.inv_root = a.state->inv_root_bc2;
-  // The records of the block's next 16 chunks at once: a chunk's own two loads after one
-  // another (its tensor, then the record) would come before its first data.
-  __shared__ AdamTensor record[kListed];
-  __shared__ int chunk_of[kListed];
-  constexpr int kWords = sizeof(AdamTensor) / 8;
-  static_assert(sizeof(AdamTensor) % 8 == 0 && kWords <= kAdamThreads / kListed, "a thread copies 8 bytes of a record");
-  for (long long c0 = blockIdx.x; c0 < a.num_chunks; c0 += (long long)kListed * gridDim.x) {
-    {
-      const int i = threadIdx.x / (kAdamThreads / kListed), word = threadIdx.x % (kAdamThreads / kListed);
-      const long long c = c0 + (long long)i * gridDim.x;
-      if (c < a.num_chunks) {
-        const int2 where = a.chunks[c];
-        if (word < kWords) reinterpret_cast<uint64_t*>(&record[i])[word] = reinterpret_cast<const uint64_t*>(&a.tensors[where.x])[word];
-        if (word == 0) chunk_of[i] = where.y;
-      }
-    }
-    __syncthreads();
-    for (int i = 0; i < kListed && c0 + (long long)i * gridDim.x < a.num_chunks; ++i) {
-      const AdamTensor& t = record[i];
-      if (t.grad == nullptr) continue;
-      u.keep = 1.f - lr * t.decay;
-      const long long base = (long long)chunk_of[i] * kChunk + warp * (kBlocksPerWarp * kScaleBlock);
-      if (t.wide && base + kBlocksPerWarp * kScaleBlock <= t.n)
-        adam_blocks<P, G, EIGHT, true>(a, t, u, base, lane);
-      else if (base < t.n)
-        adam_blocks<P, G, EIGHT, false>(a, t, u, base, lane);
-    }
-    __syncthreads();
+  for (int c = blockIdx.x; c < a.num_chunks; c += gridDim.x) {
+    const int2 where = a.chunks[c];
+    const AdamTensor t = a.tensors[where.x];
+    if (t.grad == nullptr) continue;
+    u.keep = 1.f - lr * t.decay;
+    const long long base = (long long)where.y * kChunk + warp * (kBlocksPerWarp * kScaleBlock);
+    if (t.wide && base + kBlocksPerWarp * kScaleBlock <= t.n)
+      adam_blocks<P, G, EIGHT, true>(a, t, u, base, lane);
+    else if (base < t.n)
+      adam_blocks<P, G, EIGHT, false>(a, t, u, base, lane);
   }
   __syncthreads();  // every thread of the block has read the state
   if (threadIdx.x == 0 && atomicAdd(&a.state->ticket, 1u) == gridDim.x - 1) {
