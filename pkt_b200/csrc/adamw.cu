@@ -2,6 +2,10 @@
 //
 // Bound by memory: 28 bytes per parameter with fp32 states (parameter, m and v read
 // and written, gradient read), 16 1/8 with 8-bit states, 2 more for a bf16 copy.
+// Measured (6.55 TB/s: a plain copy): 41.9 million parameters, fp32 states and a bf16
+// copy 198 us, 6.35 TB/s; 268 million, 8-bit states and a copy 789 us, 6.17 TB/s; 5.3
+// million in 6 tensors, 8-bit states 21 us, 4.1 TB/s (launch and the loads' latency; a
+// block that fetches the records of 16 chunks ahead takes 21 and, on 268 million, 810 us).
 // The tensors are cut into chunks of 4096 values, listed once in device memory; a
 // block takes every gridDim-th chunk, and within it a warp owns blocks of 128 values,
 // 4 per lane, so that a block of 8-bit states is quantised with one warp reduction.
