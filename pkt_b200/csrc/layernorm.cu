@@ -724,9 +724,11 @@ LnPlan ln_plan(const pkt_layernorm_desc& d, bool backward, int sms) {
     return (long long)p.size * n >= d.cols;
   };
   // The ring pays from a few rows per group on: up to 32 values per thread in the
-  // forward pass (16 one by one), 16 in the backward pass (three more registers each; 8
-  // one by one while they hold the row), in as few threads as hold the row.
-  const int most = wide && !backward ? 32 : backward && !wide && d.cols <= 8 * kRingThreads ? 8 : 16, least = 8;
+  // forward pass (16 one by one), 16 in the backward pass (three more registers each), in
+  // as few threads as hold the row. One by one in the backward pass bf16 takes 16 (8192 x
+  // 4095: 52 us, 65 us with 8) and fp32, whose two rows and sums then fill the registers,
+  // 8 while they hold the row (65 us, 75 us with 16).
+  const int most = wide && !backward ? 32 : backward && !wide && es == 4 && d.cols <= 8 * kRingThreads ? 8 : 16, least = 8;
   for (int n = most; n >= least; n /= 2) {
     if (!fit(n, kRingThreads)) break;
     if (p.size == 32 && 32 * (n / 2) >= d.cols && n / 2 >= least) continue;
