@@ -263,11 +263,19 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   const bool whole = Held<T, VEC, N>::whole(tid, a.cols);
   float* params = reinterpret_cast<float*>(ring_smem);  // [2][cols rounded up to 4]
   const int pcols = (a.cols + 3) & ~3;
-  for (int c = threadIdx.x; c < a.cols; c += kRingThreads) {
-    params[c] = a.gamma ? to_f32(static_cast<const P*>(a.gamma)[c]) : 1.f;
-    params[pcols + c] = a.beta ? to_f32(static_cast<const P*>(a.beta)[c]) : 0.f;
-  }
+  auto gamma_at = [&](int c) { return a.gamma ? to_f32(static_cast<const P*>(a.gamma)[c]) : 1.f; };
+  auto beta_at = [&](int c) { return a.beta ? to_f32(static_cast<const P*>(a.beta)[c]) : 0.f; };
+  // the loads of the parameters go out before the copies, which would hold them up, and
+  // are waited for behind them
+  constexpr int kFirst = 8;
+  for (int c = threadIdx.x + kFirst * kRingThreads; c < a.cols; c += kRingThreads) params[c] = gamma_at(c), params[pcols + c] = beta_at(c);
   Ring ring = make_ring(ring_smem + 8 * (size_t)pcols, full, a, groups, group, a.pitch);
+  float gammas[kFirst], betas[kFirst];
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int c = threadIdx.x + i * kRingThreads;
+    if (c < a.cols) gammas[i] = gamma_at(c), betas[i] = beta_at(c);
+  }
   const T* x = static_cast<const T*>(a.x);
   long long fill = first;  // the next row to copy
   auto copy = [&](int slot, long long row) {
@@ -278,6 +286,12 @@ __global__ void __launch_bounds__(kRingThreads) ln_forward_ring(const LnArgs a) 
   };
   for (int i = 0; i < a.slots && fill < a.rows; ++i, fill += step)
     if (tid == 0) copy(i, fill);
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) {
+    const int c = threadIdx.x + i * kRingThreads;
+    if (c < a.cols) params[c] = gammas[i], params[pcols + c] = betas[i];
+  }
+  __syncthreads();
   T* y = static_cast<T*>(a.y) + first * a.ldy;
   const T* at = x + first * a.ldx;
   const long long next_y = step * a.ldy, next_x = step * a.ldx;
