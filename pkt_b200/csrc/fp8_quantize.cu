@@ -72,8 +72,19 @@ __device__ __forceinline__ void cols_big(const Row4<float> (&r)[N], uint32_t (&b
   }
 }
 
+// 4 consecutive values that start s values into two neighbouring groups of 4.
+__device__ __forceinline__ Row4<bf16_t> shifted(const Row4<bf16_t>& lo, const Row4<bf16_t>& hi, uint32_t s) {
+  const uint32_t x0 = s & 2 ? lo.w[1] : lo.w[0], x1 = s & 2 ? hi.w[0] : lo.w[1], x2 = s & 2 ? hi.w[1] : hi.w[0], bits = 16 * (s & 1);
+  Row4<bf16_t> r;
+  r.w[0] = __funnelshift_r(x0, x1, bits), r.w[1] = __funnelshift_r(x1, x2, bits);
+  return r;
+}
+
 // N rows of 4 columns: all loads before the first use. `whole`: every value is inside
-// the matrix and the accesses are aligned.
+// the matrix. bf16 rows that do not start on a boundary of 4 values (!WIDE) are read as
+// the two aligned groups of 4 that hold a lane's values, a few rows at a time: a group
+// with one value of the matrix in it is memory that may be read, and what else it holds
+// goes (8192x4097 both ways 36 us, value by value 57 us; fp32 55 and 42 us).
 template <typename T, bool WIDE, int N>
 __device__ __forceinline__ void load_rows(const QuantArgs& a, long long row0, int col, bool whole, Row4<T> (&r)[N]) {
   const T* p = static_cast<const T*>(a.x) + row0 * a.ldx + col;
@@ -82,18 +93,45 @@ __device__ __forceinline__ void load_rows(const QuantArgs& a, long long row0, in
     for (int i = 0; i < N; ++i, p += a.ldx) r[i].load(p, true);
     return;
   }
-  const bool four = WIDE && col + 4 <= a.cols;
+  const int left = a.cols - col;
+  if constexpr (WIDE || sizeof(T) == 4) {
+    const bool four = WIDE && left >= 4;
 #pragma unroll
-  for (int i = 0; i < N; ++i, p += a.ldx) {
+    for (int i = 0; i < N; ++i, p += a.ldx) {
 #pragma unroll
-    for (int k = 0; k < Row4<T>::kWords; ++k) r[i].w[k] = 0;
-    if (row0 + i >= a.rows) continue;
-    if (four) {
-      r[i].load(p, true);
-    } else {
+      for (int k = 0; k < Row4<T>::kWords; ++k) r[i].w[k] = 0;
+      if (row0 + i >= a.rows) continue;
+      if (four) {
+        r[i].load(p, true);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (col + k < a.cols) r[i].set(k, p[k]);
+        for (int k = 0; k < 4; ++k)
+          if (k < left) r[i].set(k, p[k]);
+      }
+    }
+  } else {
+    uint32_t keep[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) keep[k] = 2 * k + 1 < left ? ~0u : 2 * k < left ? 0xffffu : 0u;
+    constexpr int B = 4;
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += B) {
+      Row4<T> lo[B], hi[B];
+      uint32_t s[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i, p += a.ldx) {
+        const bool in = row0 + i0 + i < a.rows;
+        s[i] = uint32_t(reinterpret_cast<uintptr_t>(p) / sizeof(T)) & 3;
+        const T* from = p - s[i];
+        lo[i].load(from, in && left > 0);
+        hi[i].load(from + 4, in && s[i] > 0 && left > 4 - int(s[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        r[i0 + i] = shifted(lo[i], hi[i], s[i]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) r[i0 + i].w[k] &= keep[k];
+      }
     }
   }
 }
@@ -260,13 +298,14 @@ cudaError_t quantize_run(const QuantArgs& a, int sms, cudaStream_t st) {
   if (a.block_rows == 1 && !a.qt) {
     // 16 rows per warp keep more bytes in flight, 4 start more warps: bf16 256x4096 (54
     // row blocks per SM) takes 2.4 us with 16 and 2.2 us with 4, 512x4096 2.8 and 3.1 us,
-    // 8192x4096 17.5 and 34 us. With one value per access 4 rows are the better:
-    // 4099x777 takes 7.3 us instead of 11.9 us.
-    const bool many = WIDE && (long long)kbs * a.rows >= 110LL * sms;
+    // 8192x4096 17.5 and 34 us. Off the boundary of 4 values: bf16 4099x777 (194 row
+    // blocks per SM) 8.8 us with 16 and 5.4 us with 4, 8192x4097 34 and 40 us; fp32, value
+    // by value, takes 4.
+    const bool many = (WIDE || sizeof(T) == 2) && (long long)kbs * a.rows >= (WIDE ? 110LL : 440LL) * sms;
     const int rows = many ? 64 : 16;
     const dim3 grid(kbs, unsigned(std::min((a.rows - 1) / rows + 1, 65535)));
-    if constexpr (WIDE)
-      if (many) return op_launch(quantize_rows<T, true, E5M2, 16>, grid, dim3(128), 0, st, a);
+    if constexpr (WIDE || sizeof(T) == 2)
+      if (many) return op_launch(quantize_rows<T, WIDE, E5M2, 16>, grid, dim3(128), 0, st, a);
     return op_launch(quantize_rows<T, WIDE, E5M2, 4>, grid, dim3(128), 0, st, a);
   }
   const int tiles = (a.rows - 1) / 128 + 1;

@@ -313,3 +313,37 @@ def test_refuses_what_it_cannot_reach(pk):
         setattr(bad, field, host.data_ptr())
         with pytest.raises(pk.PktError, match=f"{field} is not device memory"):
             pk.fp8_gemm(bad)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (130, 5), (300, 131), (700, 778), (20000, 643)])
+def test_quantise_between_nans(pk, rows, cols, dtype, block_rows):
+    """Rows that start anywhere, in memory that holds NaN elsewhere: the bytes and scales of a contiguous copy."""
+    x = torch.randn(rows, cols, generator=torch.Generator(device="cuda").manual_seed(cols), device="cuda").to(TYPES[dtype])
+
+    def run(t):
+        q = torch.zeros(rows, up(cols), dtype=torch.uint8, device="cuda")
+        s = torch.zeros(-(-cols // 128), -(-rows // block_rows), device="cuda")
+        qt = torch.zeros(cols, up(rows), dtype=torch.uint8, device="cuda")
+        st = torch.zeros(-(-rows // 128), -(-cols // block_rows), device="cuda")
+        out = []
+        for both in (False, True):  # rows alone, then both ways
+            d = pk.Fp8QuantizeDesc(rows=rows, cols=cols, dtype=kind(pk, dtype), q_dtype=pk.DTYPE_E4M3, block_rows=block_rows, x=t.data_ptr(),
+                                   ldx=t.stride(0), q=q.data_ptr(), ldq=q.stride(0), scale=s.data_ptr(), ld_scale=s.stride(0))
+            if both:
+                d.qt, d.ldqt, d.scale_t, d.ld_scale_t = qt.data_ptr(), qt.stride(0), st.data_ptr(), st.stride(0)
+            pk.fp8_quantize(d)
+            out += [q.clone(), s.clone(), qt.clone(), st.clone()]
+        return out
+
+    aligned = torch.zeros(rows, -(-cols // 8) * 8, dtype=x.dtype, device="cuda")[:, :cols]
+    aligned.copy_(x)
+    want = run(aligned)
+    assert all(torch.all(torch.isfinite(t)) for t in want if t.dtype == torch.float32)
+    for offset, pad in ((0, 1), (1, 0), (2, 3), (3, 2), (5, 4)):
+        flat = torch.full((rows * (cols + pad) + offset + 8,), float("nan"), dtype=x.dtype, device="cuda")
+        t = flat[offset:offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        t.copy_(x)
+        for a, b in zip(run(t), want):
+            assert torch.equal(a, b)
