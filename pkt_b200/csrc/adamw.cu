@@ -290,7 +290,7 @@ struct AdamW {
   int check_grad(const void* g, size_t i) const {
     const size_t bytes = grad_dtype == PKT_DTYPE_F32 ? 4 : 2;
     if (!aligned_to(g, bytes)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
-    if (!g) return PKT_OK;
+    if (!g || tensors[i].n == 0) return PKT_OK;
     const uintptr_t at = reinterpret_cast<uintptr_t>(g), end = at + size_t(tensors[i].n) * bytes;
     const auto next = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const std::pair<uintptr_t, uintptr_t>& w) { return v < w.second; });
     if (next != written.end() && next->first < end) return fail(PKT_ERR_ARGS, "grad of tensor %zu overlaps an array that the step writes", i);

@@ -65,9 +65,7 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
     if (!in) return;
-    if constexpr (VEC == 1) {
-      set(0, *p);
-    } else if constexpr (kBytes >= 16) {
+    if constexpr (kBytes >= 16) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
         const uint4 v = reinterpret_cast<const uint4*>(p)[i];
@@ -89,25 +87,19 @@ struct Raw {
   }
 };
 
-// Stores VEC values to p, as one aligned access per 16 bytes.
+// Stores VEC values to p, as one aligned access.
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   constexpr int kBytes = VEC * int(sizeof(T));
-  if constexpr (VEC == 1) {
-    from_f32(v[0], p);
-  } else {
-    uint32_t w[kBytes / 4];
+  static_assert(kBytes == 8 || kBytes == 16, "one access");
+  uint32_t w[kBytes / 4];
 #pragma unroll
-    for (int i = 0; i < kBytes / 4; ++i)
-      w[i] = sizeof(T) == 4 ? __float_as_uint(v[i % VEC]) : pack_bf16x2(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
-    if constexpr (kBytes >= 16) {
-#pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i)
-        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    }
-  }
+  for (int i = 0; i < kBytes / 4; ++i)
+    w[i] = sizeof(T) == 4 ? __float_as_uint(v[i % VEC]) : pack_bf16x2(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
+  if constexpr (kBytes == 16)
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
 template <typename T, int VEC>

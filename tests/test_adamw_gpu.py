@@ -293,7 +293,7 @@ def test_refuses_overlapping_arrays(pk):
     t[7] = 1.0
     plan.step(1e-2)
     assert torch.all(t[2] != 0) and torch.all(t[5] == 0)
-    pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**ok, "n": 0})])  # nothing is written twice
+    pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**ok, "n": 0, "grad": at[0] + 8})])  # nothing is written twice
 
 
 def test_gradients_stay_as_they_were_inside_a_capture(pk):
