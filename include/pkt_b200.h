@@ -410,7 +410,7 @@ typedef struct pkt_adamw_tensor {
   float* m_scale;        /* 8-bit states: [ceil(n/128)] */
   float* v_scale;
   void* copy_bf16;       /* optional [n]: the new parameters rounded to bf16 */
-  long long n;
+  long long n;           /* 0: no pointer of the tensor is looked at */
   float weight_decay;
   int pad;
 } pkt_adamw_tensor;

@@ -279,7 +279,7 @@ struct AdamW {
   // with one of them; gradients may be shared.
   void writes(const void* p, long long n, size_t bytes) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    if (p && n > 0) written.push_back({at, at + size_t(n) * bytes});
+    if (p) written.push_back({at, at + size_t(n) * bytes});
   }
   int sort_written() {
     std::sort(written.begin(), written.end());
@@ -289,8 +289,8 @@ struct AdamW {
   }
   int check_grad(const void* g, size_t i) const {
     const size_t bytes = grad_dtype == PKT_DTYPE_F32 ? 4 : 2;
-    if (!aligned_to(g, bytes)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
     if (!g || tensors[i].n == 0) return PKT_OK;
+    if (!aligned_to(g, bytes)) return fail(PKT_ERR_ARGS, "grad of tensor %zu is not aligned to its type", i);
     const uintptr_t at = reinterpret_cast<uintptr_t>(g), end = at + size_t(tensors[i].n) * bytes;
     const auto next = std::upper_bound(written.begin(), written.end(), at, [](uintptr_t v, const std::pair<uintptr_t, uintptr_t>& w) { return v < w.second; });
     if (next != written.end() && next->first < end) return fail(PKT_ERR_ARGS, "grad of tensor %zu overlaps an array that the step writes", i);
@@ -322,8 +322,12 @@ int AdamW::setup(const pkt_adamw_config& c) {
   for (int i = 0; i < c.num_tensors; ++i) {
     const pkt_adamw_tensor& s = c.tensors[i];
     if (s.n < 0) return fail(PKT_ERR_ARGS, "tensor %d has %lld values", i, s.n);
-    if (s.n > 0 && (!s.param || !s.m || !s.v)) return fail(PKT_ERR_ARGS, "tensor %d needs param, m and v", i);
-    if (s.n > 0 && eight && (!s.m_scale || !s.v_scale)) return fail(PKT_ERR_ARGS, "tensor %d needs m_scale and v_scale (8-bit states)", i);
+    if (s.n == 0) {  // it has no chunk: its pointers may be the next tensor's, or any
+      tensors.push_back(AdamTensor{});
+      continue;
+    }
+    if (!s.param || !s.m || !s.v) return fail(PKT_ERR_ARGS, "tensor %d needs param, m and v", i);
+    if (eight && (!s.m_scale || !s.v_scale)) return fail(PKT_ERR_ARGS, "tensor %d needs m_scale and v_scale (8-bit states)", i);
     if (!aligned_to(s.param, ps) || !aligned_to(s.m, ss) || !aligned_to(s.v, ss) || !aligned_to(s.m_scale, 4) || !aligned_to(s.v_scale, 4) ||
         !aligned_to(s.copy_bf16, 2))
       return fail(PKT_ERR_ARGS, "an array of tensor %d is not aligned to its type", i);
@@ -336,7 +340,7 @@ int AdamW::setup(const pkt_adamw_config& c) {
     tensors.push_back(t);
     writes(s.param, s.n, ps), writes(s.m, s.n, ss), writes(s.v, s.n, ss), writes(s.copy_bf16, s.n, 2);
     if (eight) writes(s.m_scale, (s.n - 1) / kScaleBlock + 1, 4), writes(s.v_scale, (s.n - 1) / kScaleBlock + 1, 4);
-    const long long count = s.n > 0 ? (s.n - 1) / kChunk + 1 : 0;
+    const long long count = (s.n - 1) / kChunk + 1;
     if (count + (long long)chunks.size() > 0x7fffffffLL) return fail(PKT_ERR_ARGS, "too many parameters for one AdamW plan");
     for (long long k = 0; k < count; ++k) chunks.push_back(make_int2(i, int(k)));
   }

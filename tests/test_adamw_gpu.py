@@ -335,3 +335,38 @@ def test_two_plans_on_two_streams(pk):
     torch.cuda.synchronize()
     a.check(want[0], 1, 1e-2)
     b.check(want[1], 1, 1e-2)
+
+
+@pytest.mark.parametrize("state", ["f32", "e4m3"])
+def test_tensors_without_values_claim_nothing(pk, state):
+    """Scales packed at ceil(n / 128) each: an empty tensor's arrays begin where the next one's do."""
+    sizes, eight = [256, 0, 300, 0, 5], state == "e4m3"
+    at = [sum(sizes[:i]) for i in range(5)]
+    blocks = [-(-n // 128) for n in sizes]
+    sat = [sum(blocks[:i]) for i in range(5)]
+    p, m, v = torch.full((561,), 0.5, device="cuda"), torch.zeros(561, device="cuda"), torch.zeros(561, device="cuda")
+    if eight:
+        m, v = m.to(torch.float8_e4m3fn), v.to(torch.float8_e4m3fn)
+    g, ms, vs = torch.full((561,), 0.25, device="cuda"), torch.zeros(6, device="cuda"), torch.zeros(6, device="cuda")
+    rec = [pk.AdamWTensor(param=p[a:].data_ptr(), grad=g[a:].data_ptr(), m=m[a:].data_ptr(), v=v[a:].data_ptr(), n=n,
+                          m_scale=ms[b:].data_ptr() if eight else None, v_scale=vs[b:].data_ptr() if eight else None)
+           for a, b, n in zip(at, sat, sizes)]
+    plan = pk.AdamW(rec, state_dtype=state, eps=1e-8)
+    plan.step(0.125)
+    # a first step from empty states moves by lr m / (1 - b1) / (|g| + eps) = lr, 16 u of the step and 3 u of the value off
+    assert torch.all((p.double() - 0.375).abs() <= 16 * U * 0.125 + 3 * U * 0.5 + 0.125 * 1e-8 / 0.25)
+    if eight:
+        assert torch.all(ms > 0) and torch.all(vs > 0)
+
+
+def test_a_tensor_without_values_may_name_anything(pk):
+    """No pointer of it is looked at: host memory, an odd address, one that another tensor writes."""
+    t = torch.zeros(4, 256, device="cuda")
+    host = torch.zeros(256)
+    ok = dict(param=t[0].data_ptr(), grad=t[1].data_ptr(), m=t[2].data_ptr(), v=t[3].data_ptr(), n=256)
+    for kw in (dict(param=host.data_ptr()), dict(m=t[2].data_ptr() + 1), dict(v=t[0].data_ptr()), dict(grad=t[1].data_ptr() + 3), dict(copy_bf16=host.data_ptr())):
+        plan = pk.AdamW([pk.AdamWTensor(**ok), pk.AdamWTensor(**{**ok, "n": 0, **kw})])
+        plan.set_grads([t[1].data_ptr(), t[1].data_ptr() + 1])
+        plan.step(1e-3)
+    torch.cuda.synchronize()
+    assert torch.all(t == 0)
