@@ -433,7 +433,8 @@ int pkt_adamw_step(pkt_adamw* h, float lr, float grad_scale, const float* scales
 /* New gradient pointers (num_tensors of them), for steps enqueued from now on. Not
  * inside a stream capture: steps captured before then read the new pointers too. */
 int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream);
-/* Steps taken: set (stream-ordered), and read (synchronises the stream). */
+/* Steps taken: set (stream-ordered), and read (synchronises the stream; not inside a
+ * stream capture). */
 int pkt_adamw_set_step(pkt_adamw* h, long long step, void* stream);
 int pkt_adamw_get_step(pkt_adamw* h, long long* step, void* stream);
 

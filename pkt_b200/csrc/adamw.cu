@@ -399,6 +399,14 @@ struct OnDevice {
   }
 };
 
+// What a captured stream would refuse after it had spoilt the capture is refused before.
+int outside_capture(cudaStream_t st, const char* what) {
+  cudaStreamCaptureStatus capturing;
+  const cudaError_t e = cudaStreamIsCapturing(st, &capturing);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  return capturing == cudaStreamCaptureStatusNone ? PKT_OK : fail(PKT_ERR_ARGS, "%s inside a stream capture", what);
+}
+
 }  // namespace
 }  // namespace pkb
 
@@ -451,11 +459,8 @@ int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream) {
   AdamW& p = h->plan;
   OnDevice on(p.device);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaStreamCaptureStatus capturing;
-  cudaError_t e = cudaStreamIsCapturing(st, &capturing);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-  if (capturing != cudaStreamCaptureStatusNone) return fail(PKT_ERR_ARGS, "AdamW gradients cannot be set inside a stream capture");
-  int rc;
+  int rc = outside_capture(st, "AdamW gradients cannot be set");
+  if (rc) return rc;
   for (size_t i = 0; i < p.tensors.size(); ++i)
     if ((rc = p.check_grad(grads[i], i))) return rc;
   for (size_t i = 0; i < p.tensors.size(); ++i) {
@@ -463,7 +468,7 @@ int pkt_adamw_set_grads(pkt_adamw* h, const void* const* grads, void* stream) {
     p.set_wide(&p.tensors[i]);
   }
   if (p.tensors.empty()) return PKT_OK;
-  e = cudaMemcpyAsync(p.d_tensors, p.tensors.data(), sizeof(AdamTensor) * p.tensors.size(), cudaMemcpyHostToDevice, st);
+  const cudaError_t e = cudaMemcpyAsync(p.d_tensors, p.tensors.data(), sizeof(AdamTensor) * p.tensors.size(), cudaMemcpyHostToDevice, st);
   return e == cudaSuccess ? PKT_OK : cuda_fail(e, "copy AdamW gradients");
 }
 
@@ -479,6 +484,8 @@ int pkt_adamw_get_step(pkt_adamw* h, long long* step, void* stream) {
   OnDevice on(h->plan.device);
   AdamState s;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = outside_capture(st, "the AdamW step cannot be read");
+  if (rc) return rc;
   cudaError_t e = cudaMemcpyAsync(&s, h->plan.d_state, sizeof(s), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return cuda_fail(e, "read the AdamW step");

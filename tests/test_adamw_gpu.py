@@ -370,3 +370,20 @@ def test_a_tensor_without_values_may_name_anything(pk):
         plan.step(1e-3)
     torch.cuda.synchronize()
     assert torch.all(t == 0)
+
+
+def test_the_step_is_not_read_inside_a_capture(pk):
+    """Refused before anything is enqueued, so the capture goes on."""
+    c = Case(pk, [3000])
+    before = c.snapshot()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        with pytest.raises(pk.PktError, match="stream capture"):
+            c.plan.get_step(st.cuda_stream)
+        c.plan.step(1e-2, stream=st.cuda_stream)
+    g.replay()
+    torch.cuda.synchronize()
+    c.check(before, 1, 1e-2)
+    assert c.plan.get_step() == 1
