@@ -372,3 +372,18 @@ def test_two_calls_at_once(pk):
     for d, s in (a, b):
         check_forward(s)
         check_backward(s)
+
+
+@pytest.mark.parametrize("dtype,pad", [("f32", 0), ("f32", 1), ("bf16", 0), ("bf16", 1)])
+@pytest.mark.parametrize("rows,cols", [(6, 1000), (6, 777), (3000, 1000), (3000, 777), (5000, 40), (5000, 41), (700, 6000), (700, 6007), (3, 20000), (3, 24999), (3, 25001)])
+def test_rows_without_spread(pk, rows, cols, dtype, pad):
+    """Every partial sum of these values is exact in any order, so the mean is the value and y is beta
+    (directly loaded rows, rows through the rings, long rows; whole and one by one)."""
+    d, s = make(pk, rows, cols, dtype, pad=pad, seed=cols)
+    values = [3.0, 100.0, -7.0, 0.75, 113.0, 1.0]
+    for i, v in enumerate(values):
+        s["x"][i::len(values), :cols] = v
+    pk.layernorm_forward(d)
+    assert torch.equal(s["mean"], s["x"][:, 0].float())
+    assert torch.equal(s["y"][:, :cols], s["beta"].to(TYPES[dtype]).expand(rows, cols))
+    check_guards(s, "y")
