@@ -61,6 +61,7 @@ struct alignas(64) Fp8Args {
   long long ldo;
   int out_bf16, swap;  // swap: out[col * ldo + row]
   int wide, tma_out;   // 4 values of out in one store; map_out is valid
+  int tma_cols;        // columns that map_out covers
   uint32_t idesc;
   int* status;
 };
@@ -525,9 +526,20 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1) fp8_gemm_kernel(
             if (a.tma_out) {
               fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0 && row0 < a.rows && col < a.cols) {
+              if (lane == 0 && row0 < a.rows && col < a.tma_cols) {
                 tma_store_2d(&a.map_out, to, col, row0);
                 bulk_commit();
+              }
+              if (a.tma_cols < col + per && row0 + lane < a.rows) {  // the columns left behind it, a row per lane
+                for (int c = max(a.tma_cols, col); c < a.cols; ++c) {
+                  const long long at = (long long)(row0 + lane) * a.ldo + c;
+                  const int in = (c - col) * (a.out_bf16 ? 2 : 4);
+                  const uint8_t* from = to + lane * 128 + (((in >> 4) ^ (lane & 7)) << 4) + (in & 15);
+                  if (a.out_bf16)
+                    static_cast<uint16_t*>(a.out)[at] = *reinterpret_cast<const uint16_t*>(from);
+                  else
+                    static_cast<float*>(a.out)[at] = *reinterpret_cast<const float*>(from);
+                }
               }
             } else {
               __syncwarp();
@@ -788,9 +800,13 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream) {
   a.c_shift = (swap ? d->a_block_rows : d->b_block_rows) == 1 ? 0 : 7;
   a.out = d->out, a.ldo = d->ldo, a.out_bf16 = es == 2, a.swap = swap;
   a.wide = aligned_to(d->out, 4 * es) && d->ldo % 4 == 0;
-  // TMA stores need 16-byte aligned rows; else value by value
-  if (!swap && aligned_to(d->out, 16) && d->ldo * es % 16 == 0) {
-    if ((rc = result_map(&a.map_out, d->out, d->out_dtype, d->N, d->M, d->ldo))) return rc;
+  // TMA stores need 16-byte aligned rows; else value by value. They write 16 bytes whole,
+  // zeros past a map's last column, and behind column N there may be the next columns of a
+  // wider matrix: the map ends at the last whole 16 bytes, what is left of a row is stored
+  // value by value (8192x777x4096 into rows of 784 bf16 39.0 us, all value by value 42.3 us).
+  a.tma_cols = d->N & -(16 / es);
+  if (!swap && a.tma_cols > 0 && aligned_to(d->out, 16) && d->ldo * es % 16 == 0) {
+    if ((rc = result_map(&a.map_out, d->out, d->out_dtype, a.tma_cols, d->M, d->ldo))) return rc;
     a.tma_out = 1;
   }
   const uint32_t fr = (swap ? d->b_dtype : d->a_dtype) == PKT_DTYPE_E5M2, fc = (swap ? d->a_dtype : d->b_dtype) == PKT_DTYPE_E5M2;

@@ -347,3 +347,14 @@ def test_quantise_between_nans(pk, rows, cols, dtype, block_rows):
         t.copy_(x)
         for a, b in zip(run(t), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bb", [1, 128])
+@pytest.mark.parametrize("M,N,K,out,pad", [(100, 11, 103, "f32", 1), (658, 9, 103, "f32", 3), (658, 11, 1000, "f32", 5), (3799, 1, 29, "f32", 3),
+                                           (300, 65, 128, "bf16", 7), (4261, 222, 103, "bf16", 2), (4261, 223, 300, "bf16", 9),
+                                           (4261, 777, 1000, "bf16", 7), (2100, 1111, 600, "f32", 1), (2100, 1100, 600, "bf16", 4),
+                                           (40, 11, 200, "f32", 1)])
+def test_product_beside_other_columns(pk, M, N, K, out, pad, bb):
+    """Rows of out on 16-byte boundaries that end inside 16 bytes: the columns behind them keep their values (`product` looks)."""
+    got, want, mag, _ = product(pk, M, N, K, out=out, bb=bb, seed=N, pad=pad)
+    close(got, want, mag, K, out)
