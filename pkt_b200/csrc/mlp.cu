@@ -544,7 +544,7 @@ int Mlp::build(int p, int q) {
     g.push_back(d);
   }
   int first = 0;
-  int rc = rt->register_gemms(g.data(), int(g.size()), &first);
+  int rc = rt->register_gemms(g.data(), int(g.size()), true, &first);
   if (rc) return rc;
   auto G = [&](int idx) -> const DevGemm& { return rt->host_gemms[first + idx]; };
   if (grad_mode == 2) {

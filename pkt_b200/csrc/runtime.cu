@@ -135,7 +135,7 @@ int gemm_tiles(const pkt_gemm_desc& d, int* tm, int* tn) {
   return PKT_OK;
 }
 
-int build_dev_gemm(const pkt_gemm_desc& d, DevGemm* g) {
+int build_dev_gemm(const pkt_gemm_desc& d, bool own_rows, DevGemm* g) {
   std::memset(g, 0, sizeof(*g));
   g->d = d;
   int rc = gemm_tiles(d, &g->tiles_m, &g->tiles_n);
@@ -220,14 +220,16 @@ int build_dev_gemm(const pkt_gemm_desc& d, DevGemm* g) {
     return fail(PKT_ERR_ARGS, "WGRAD_SGD / WGRAD_PEER epilogues need w_in / w_out");
   if (d.epilogue < 0 || d.epilogue > PKT_EPI_WGRAD_PEER) return fail(PKT_ERR_ARGS, "bad epilogue");
   // TMA tile stores need whole 32-column chunks inside a tile (a box must not
-  // spill into the neighbouring tile's columns).
+  // spill into the neighbouring tile's columns). They write 16 bytes whole, zeros past
+  // the last column.
+  auto ends = [&](int es) { return own_rows || (long long)d.N * es % 16 == 0; };
   if (d.bn % 32 == 0) {
     if (d.epilogue == PKT_EPI_WGRAD_SGD || d.epilogue == PKT_EPI_WGRAD_PEER) {
-      g->tma_w = make_store_map(&g->map_w, d.w_out, PKT_DTYPE_F32, d.N, d.M, d.ldw) &&
+      g->tma_w = ends(d.w_shadow ? 2 : 4) && make_store_map(&g->map_w, d.w_out, PKT_DTYPE_F32, d.N, d.M, d.ldw) &&
                  (d.w_shadow == nullptr ||
                   make_store_map(&g->map_shadow, d.w_shadow, PKT_DTYPE_BF16, d.N, d.M, d.ldw));
     } else {
-      g->tma_out = make_store_map(&g->map_out, d.out, d.out_dtype, d.N, d.M, d.ldo);
+      g->tma_out = ends(d.out_dtype == PKT_DTYPE_BF16 ? 2 : 4) && make_store_map(&g->map_out, d.out, d.out_dtype, d.N, d.M, d.ldo);
     }
   }
   if (d.epilogue == PKT_EPI_MSE || d.epilogue == PKT_EPI_DGRAD_RELU)
@@ -448,11 +450,11 @@ int Runtime::status(int* code, int* task, int* detail) {
   return PKT_OK;
 }
 
-int Runtime::register_gemms(const pkt_gemm_desc* descs, int n, int* first) {
+int Runtime::register_gemms(const pkt_gemm_desc* descs, int n, bool own_rows, int* first) {
   cudaSetDevice(device);
   std::vector<DevGemm> add(n);
   for (int i = 0; i < n; ++i) {
-    int rc = build_dev_gemm(descs[i], &add[i]);
+    int rc = build_dev_gemm(descs[i], own_rows, &add[i]);
     if (rc) return rc;
   }
   if (num_gemms + n > gemm_cap) {
@@ -587,7 +589,7 @@ int pkt_runtime_status(pkt_runtime* rt, int* code, int* task_index, int* detail)
 
 int pkt_runtime_register_gemms(pkt_runtime* rt, const pkt_gemm_desc* descs, int n, int* first_id) {
   if (!rt || n <= 0 || !descs) return pkb::fail(PKT_ERR_ARGS, "bad gemm registration");
-  return rt->rt->register_gemms(descs, n, first_id);
+  return rt->rt->register_gemms(descs, n, false, first_id);
 }
 
 int pkt_runtime_clear_gemms(pkt_runtime* rt) {

@@ -12,7 +12,9 @@ namespace pkb {
 int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
 int gemm_tiles(const pkt_gemm_desc& d, int* tm, int* tn);
-int build_dev_gemm(const pkt_gemm_desc& d, DevGemm* g);
+// own_rows: what lies behind column N of the results up to a 16-byte boundary is the
+// caller's padding, which TMA stores fill with zeros; else only columns below N are written.
+int build_dev_gemm(const pkt_gemm_desc& d, bool own_rows, DevGemm* g);
 bool make_store_map(CUtensorMap* map, const void* base, int dtype, long long cols, long long rows,
                     long long ld);
 
@@ -58,7 +60,7 @@ struct Runtime {
   // counters and the kernel parameters of the submitted list.
   int prepare(int blocks, cudaStream_t stream, KParams* out, int* out_blocks);
   int status(int* code, int* task, int* detail);
-  int register_gemms(const pkt_gemm_desc* descs, int n, int* first);
+  int register_gemms(const pkt_gemm_desc* descs, int n, bool own_rows, int* first);
   // Clamps a persistent grid to the CTAs that fit on the device at once (and to
   // whole clusters of `pair`); 0 or a negative count asks for the largest grid.
   int clamp_blocks(int blocks, int pair, int* out);

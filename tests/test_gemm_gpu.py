@@ -185,3 +185,44 @@ def test_gemm_wgrad_sgd_epilogue(pk):
     from pkt_b200.mlp import from_bf16_bits, to_bf16_bits
     sh = from_bf16_bits(host(shadow).view(np.uint16).ravel()).reshape(n_out, -1)[:, :n_in]
     assert np.array_equal(sh, from_bf16_bits(to_bf16_bits(got)).reshape(sh.shape))
+
+
+@pytest.mark.parametrize("pair", [1, 2])
+@pytest.mark.parametrize("out_dtype,M,N,K,ldo", [(3, 200, 81, 100, 84), (3, 300, 130, 77, 132), (1, 300, 130, 77, 136), (1, 256, 250, 128, 256)])
+def test_gemm_beside_other_columns(pk, out_dtype, M, N, K, ldo, pair):
+    """Rows of out on 16-byte boundaries that end inside 16 bytes: the columns behind them keep their values."""
+    rng = np.random.default_rng(N)
+    A, Bm = rng.standard_normal((M, K)).astype(np.float32), rng.standard_normal((N, K)).astype(np.float32)
+    a_t, b_t = stored(A, "bf16", pad(K)), stored(Bm, "bf16", pad(K))
+    out = torch.full((M, ldo), 5.0, dtype=torch.float32 if out_dtype == 3 else torch.bfloat16, device="cuda")
+    d = pk.GemmDesc()
+    d.M, d.N, d.K, d.bn, d.in_dtype = M, N, K, 64, 1
+    d.a, d.lda, d.a_major, d.b, d.ldb, d.b_major = a_t.data_ptr(), a_t.shape[1], 0, b_t.data_ptr(), b_t.shape[1], 0
+    d.epilogue, d.out, d.ldo, d.out_dtype, d.cta_pair = 0, out.data_ptr(), ldo, out_dtype, pair
+    run_gemm(pk, d)
+    got = out.float().cpu().numpy()
+    # bf16 out: half a step, 2^-8 of the value
+    assert rel_err(got[:, :N], bf16r(A).astype(np.float64) @ bf16r(Bm).astype(np.float64).T) < TOL + (2.0 ** -8 if out_dtype == 1 else 0)
+    assert np.all(got[:, N:] == 5.0)
+
+
+@pytest.mark.parametrize("shadow", [False, True])
+def test_gemm_update_beside_other_columns(pk, shadow):
+    B, n_out, n_in, ldw, lr = 256, 192, 250, 256, 0.05
+    rng = np.random.default_rng(4)
+    dY, H = rng.standard_normal((B, n_out)).astype(np.float32), rng.standard_normal((B, n_in)).astype(np.float32)
+    W0 = np.full((n_out, ldw), 5.0, np.float32)
+    W0[:, :n_in] = rng.standard_normal((n_out, n_in))
+    dy_t, h_t, w = stored(dY, "bf16", pad(n_out)), stored(H, "bf16", pad(n_in)), dev(W0)
+    copy = torch.full((n_out, ldw), 5.0, dtype=torch.bfloat16, device="cuda")
+    d = pk.GemmDesc()
+    d.M, d.N, d.K, d.bn, d.in_dtype = n_out, n_in, B, 128, 1
+    d.a, d.lda, d.a_major, d.b, d.ldb, d.b_major = dy_t.data_ptr(), dy_t.shape[1], 1, h_t.data_ptr(), h_t.shape[1], 1
+    d.epilogue = 4
+    d.w_in, d.w_out, d.w_shadow, d.ldw, d.lr = w.data_ptr(), w.data_ptr(), copy.data_ptr() if shadow else None, ldw, lr
+    run_gemm(pk, d)
+    ref = W0[:, :n_in] - lr * (bf16r(dY).astype(np.float64).T @ bf16r(H).astype(np.float64))
+    assert rel_err(host(w)[:, :n_in], ref) < TOL
+    assert np.all(host(w)[:, n_in:] == 5.0) and torch.all(copy[:, n_in:] == 5.0)
+    if shadow:
+        assert rel_err(copy[:, :n_in].float().cpu().numpy(), ref) < TOL + 2.0 ** -8
