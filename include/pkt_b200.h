@@ -172,7 +172,7 @@ typedef struct pkt_gemm_desc {
   int b_major;
   int epilogue;      /* pkt_epilogue */
   void* out;         /* D / dY / dH / dW output */
-  int ldo;
+  int ldo;           /* columns N.. of a row are not written (ldw too) */
   int out_dtype;     /* PKT_DTYPE_BF16 or PKT_DTYPE_F32 */
   int relu;          /* PKT_EPI_BIAS_ACT: apply ReLU */
   const float* bias; /* [N] or null */
@@ -280,9 +280,12 @@ int pkt_axpy_noalloc_status(int* code, int* task_index, int* detail);
 /* ---- stand-alone operators ---------------------------------------------- */
 /* These run on the current device and in the order of `stream`; every pointer is
  * memory of that device (checked: a host pointer or another device's memory is
- * PKT_ERR_ARGS). They allocate nothing and may be captured into a CUDA graph.
+ * PKT_ERR_ARGS). They allocate nothing and may be captured into a CUDA graph
+ * (pkt_adamw_create and pkt_ops_status, which allocate or synchronise, may not).
  * A descriptor is read during the call only. Outputs must not overlap inputs
- * unless an operator says so. No counterpart in pkt. */
+ * unless an operator says so. Only a result's own rows and columns are written. Of
+ * an input, bytes beside a row may be read, within the 16-byte granules that hold
+ * the row's first and last value; they never change a result. No counterpart in pkt. */
 
 /* Every wait inside their kernels is bounded (about 2 s). code: PKT_DEV_TIMEOUT_PIPE
  * when one has run out on the current device since the last call (results since then
@@ -295,9 +298,10 @@ int pkt_ops_status(int* code);
  *             y = (x - mean) rstd gamma + beta
  *   backward  dx, and the sums over all rows dgamma = sum dy (x-mean) rstd,
  *             dbeta = sum dy, from x, dy and the forward pass's mean and rstd
- * Any cols >= 1 and row strides >= cols (16-byte aligned rows are fastest).
- * y may be x, dx may be dy or x, with the same row stride. The columns of a
- * padded row past cols are neither read nor written. rows = 0 is allowed (dgamma
+ * Any cols >= 1 and row strides >= cols. Fastest where every row and gamma and beta
+ * start on 16 bytes and a row is a multiple of 16 bytes; else the call goes value by
+ * value. y may be x, dx may be dy or x, with the same row stride. The columns of a
+ * padded row past cols do not count and are not written. rows = 0 is allowed (dgamma
  * and dbeta are then zero). */
 typedef struct pkt_layernorm_desc {
   long long rows;
@@ -365,7 +369,9 @@ int pkt_fp8_quantize(const pkt_fp8_quantize_desc* d, void* stream);
  *             scale_a[kb, m / a_block_rows] * scale_b[kb, n / b_block_rows]
  *             * sum over k in kb of a[m, k] * b[n, k]
  * on the tensor cores (tcgen05, fp32 accumulators); the scales are applied to each
- * block's fp32 sum and the blocks are added in fp32. Any M, N, K >= 0 (K = 0:
+ * block's fp32 sum and the blocks are added in fp32; the two scales may be multiplied
+ * with one another first, so their product should not leave fp32's normal range
+ * (below 2^-126 it loses bits). Any M, N, K >= 0 (K = 0:
  * zeros); a and b are 16-byte aligned with row strides that are multiples of 16.
  * The result of a call does not depend on timing. */
 typedef struct pkt_fp8_gemm_desc {
@@ -394,8 +400,11 @@ int pkt_fp8_gemm(const pkt_fp8_gemm_desc* d, void* stream);
  * in fp32. state_dtype PKT_DTYPE_F32 keeps m and v as fp32. PKT_DTYPE_E4M3 keeps m
  * and sqrt(v) as block-scaled 8-bit floats (blocks of 128 consecutive values from
  * the tensor's start, scales m_scale / v_scale): 2 1/16 bytes per parameter instead
- * of 8; a positive sqrt(v) is held as at least the smallest 8-bit value, so that it
- * never divides by eps alone. States start as zeros (scales too).
+ * of 8; beside larger ones of its block a positive sqrt(v) is held as at least the
+ * smallest 8-bit value, so that it does not turn into a division by eps alone (in a
+ * block that is held as zeros it does). States start as zeros (scales too). Fastest
+ * where all arrays of a tensor start on boundaries of 4 of their values; a tensor with
+ * one that does not goes value by value.
  * The plan keeps the pointers and, on the device, the step count: replaying a
  * captured step advances it. Calls on a plan are ordered by the caller (one
  * stream, or events), also against replays of a captured step, and a plan outlives the

@@ -3,8 +3,9 @@
 // Bound by memory: 28 bytes per parameter with fp32 states (parameter, m and v read
 // and written, gradient read), 16 1/8 with 8-bit states, 2 more for a bf16 copy.
 // Measured (6.55 TB/s: a plain copy): 41.9 million parameters, fp32 states and a bf16
-// copy 198 us, 6.35 TB/s; 268 million, 8-bit states and a copy 789 us, 6.17 TB/s; 5.3
-// million in 6 tensors, 8-bit states 21 us, 4.1 TB/s (launch and the loads' latency; a
+// copy 200 us, 6.29 TB/s; 268 million, 8-bit states and a copy 790 us alone and 827 us
+// among others, 5.9 TB/s; 5.3 million in 6 tensors, 8-bit states 21 us, 4.1 TB/s (a block
+// has one or two chunks, each behind a chain of chunk record, tensor record and data; a
 // block that fetches the records of 16 chunks ahead takes 21 and, on 268 million, 810 us).
 // The tensors are cut into chunks of 4096 values, listed once in device memory; a
 // block takes every gridDim-th chunk, and within it a warp owns blocks of 128 values,
@@ -185,7 +186,8 @@ __device__ __forceinline__ void adam_blocks(const AdamArgs& a, const AdamTensor&
       m[b][i] = __fadd_rn(__fmul_rn(m[b][i], a.b1), __fmul_rn(g, a.c1));
       v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(g, g), a.c2));
       r[b][i] = __fsqrt_rn(v[i]);
-      // the quotient's own error (2 ulp of the step) is far below p's last bit
+      // the quotient's own error is 2 ulp of the step, like the rest of its arithmetic
+      // (where p is near zero, of p too)
       p[i] = rp[b].get(i) * u.keep - __fdividef(u.step_size * m[b][i], fmaf(r[b][i], u.inv_root, a.eps));
       mbig = max(mbig, abs_bits(m[b][i]));
       rbig = max(rbig, abs_bits(r[b][i]));
@@ -222,6 +224,9 @@ __device__ __forceinline__ void adam_blocks(const AdamArgs& a, const AdamTensor&
   }
 }
 
+// Three blocks per SM with 8-bit states leave 80 registers, and the form with fp32 gradients
+// spills 84 bytes; it is faster all the same (5.3 million values: 25.6 us with two blocks and
+// 22.5 us with three).
 template <typename P, typename G, bool EIGHT>
 __global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 2) adam_step(const AdamArgs a) {
   grid_dependency_wait();
@@ -376,7 +381,12 @@ int AdamW::run(float lr, float grad_scale, const float* scales, cudaStream_t st)
   a.lr = lr, a.grad_scale = grad_scale;
   a.b1 = float(beta1), a.c1 = float(1.0 - beta1), a.b2 = float(beta2), a.c2 = float(1.0 - beta2), a.eps = float(eps);
   a.beta1 = beta1, a.beta2 = beta2;
-  // one block per chunk up to what the SMs hold; a plan without values still counts the step
+  // One block per chunk up to 8 per SM, more than the 3 (8-bit states, 80 registers) or 2
+  // that an SM holds at once: a block that starts late fills the place of one that is done.
+  // With 2, 3, 4, 8 and 16 per SM: 5.3 million values, 8-bit states 18.3, 17.2, 17.1, 16.9 and
+  // 18.5 us in a graph, fp32 states 21, 24, 22, 24 and 25 us; 268 million 8-bit 867, 834, 929,
+  // 811 and 789 us; 41.9 million fp32 208, 202, 206, 198 and 193 us. A plan without values
+  // still counts the step.
   const int blocks = std::max(1, std::min(num_chunks, sms * 8));
   const bool eight = state_dtype == PKT_DTYPE_E4M3, pf = param_dtype == PKT_DTYPE_F32, gf = grad_dtype == PKT_DTYPE_F32;
   const cudaError_t e = pf ? (gf ? adam_launch<float, float>(a, eight, blocks, st) : adam_launch<float, bf16_t>(a, eight, blocks, st))

@@ -13,7 +13,7 @@
 // they do not, it holds 4 rows and a quarter of the columns (TMEM loads of 16 lanes x
 // 256 bits): each lane then needs a quarter of the columns' scales, and it is their
 // delivery from shared memory, 128 bytes a cycle for all warps, that bounds this case
-// (8192 x 4096 x 4096: 215 us with a row per lane).
+// (8192 x 4096 x 4096: 180 us where a row per lane took 215 us, at the same clock).
 //
 // Roles of a CTA: warps 0..3 (0..7) epilogue, one per 32 TMEM lanes (and half of the
 // columns); then one TMA producer warp, one MMA issuer warp and one that copies the
@@ -27,14 +27,18 @@
 // When there are few tiles, the CTAs of a cluster split K between them and add their
 // accumulators through distributed shared memory in rank order.
 //
-// What bounds it. 8192 x 4096 x 4096 with 128 x 128 blocks of b takes 134 us (2.05
-// PFLOP/s), with a scale per column 180 us; the same pipeline without the promotion
-// takes 104 us, which is the tensor cores under the power limit. A block of K (512 MMA
-// cycles) is bounded by its turn through one of the two TMEM accumulators that fit: the
-// MMAs, the epilogue's reads, and a release and an acquire through shared memory of 150
-// to 250 cycles each while MMAs run. That is why one issuer hands over all 256 columns
-// at once: two issuers with 128 columns each took 139 us, parts that every epilogue warp
-// shares 170 us, and 256 x 128 tiles with four accumulators 186 us.
+// What bounds it. 8192 x 4096 x 4096 with 128 x 128 blocks of b takes 154 us call after
+// call (1.78 PFLOP/s; the power limit lowers the clock) and 131 to 149 us in short runs, with
+// a scale per column 195 to 208 us; the tensor pipe is busy 48 % of the time. A block of K
+// (512 MMA cycles) is bounded by its turn through one of the two TMEM accumulators that
+// fit: the MMAs, the epilogue's reads, and a release and an acquire through shared memory
+// of 150 to 250 cycles each while MMAs run. That is why one issuer hands over all 256
+// columns at once. In runs at the clock of 134 us two issuers with 128 columns each took
+// 139 us, parts that every epilogue warp shares 170 us, 256 x 128 tiles with four
+// accumulators 186 us, and the same pipeline without the promotion 104 us.
+//
+// Only M asks for narrow tiles: 65536 x 16 x 4096 runs in 256-wide pair tiles and takes 77
+// us, 1.8 times the reading of its operands.
 //
 // Every wait is bounded (2 s); one that runs out sets a status word that
 // pkt_ops_status reads, and the kernel drains its copies and returns.

@@ -190,8 +190,10 @@ __device__ __forceinline__ void quantize_each_row(const QuantArgs& a, long long 
   store_rows<T, E5M2>(a, row0, col, whole, r, [&](int i) { return __shfl_sync(0xffffffffu, f, i); });
 }
 
-// Registers follow the blocks per SM that hide the most latency. 16 rows, 8192x4096: bf16
-// 17.2 us with 8 blocks and 17.7 us with 6; fp32 32.6 us with 8 and 26.4 us with 6.
+// Registers follow the blocks per SM that hide the most latency. 16 rows, 8192x4096 again
+// and again: bf16 15.7 us with 8 blocks, 17.2 us with 6 and 18.2 us with 5; fp32 36.7 us with
+// 8, 26.9 us with 6 (it spills 104 bytes) and 26.7 us with 5. bf16 rows off the boundary of 4
+// values spill 188 bytes with 8 blocks (8192x4097 34.5 us; 31.2 us with 6).
 template <typename T, bool WIDE, bool E5M2, int N>
 __global__ void __launch_bounds__(128, N < 16 ? 1 : sizeof(T) == 2 ? 8 : 6) quantize_rows(const QuantArgs a) {
   grid_dependency_wait();
@@ -206,9 +208,9 @@ __global__ void __launch_bounds__(128, N < 16 ? 1 : sizeof(T) == 2 ? 8 : 6) quan
   }
 }
 
-// Blocks per SM with both results, 8192x4096: bf16 31.4 us with 2, 26.7 us with 3 and
-// 25.5 us with 4; fp32 34.2, 33.8 and 48.5 us (4 blocks leave too few registers), but
-// 4096x1024 in 128 x 128 blocks 6.6 us with 2 and 6.9 us with 3, which spill.
+// Blocks per SM with both results, 8192x4096: bf16 31.5 us with 2, 26.7 us with 3 and
+// 23.9 us with 4 (16 bytes spilled); fp32 49.0 us with 1, 33.6 us with 2 and with 3, but
+// 4096x1024 in 128 x 128 blocks 4.6 us with 2 and 5.0 us with 3.
 template <typename T, bool WIDE, bool E5M2>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) quantize_tile(const QuantArgs a) {
   grid_dependency_wait();

@@ -7,9 +7,10 @@
 //             dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
 //
 // Both are bound by memory: 2 and 3 passes over the rows. Measured (6.55 TB/s: a plain
-// copy): forward 8192x4096 bf16 25.3 us, 5.30 TB/s, fp32 49.1 us, 5.47 TB/s; backward 37.9
-// us, 5.31 TB/s, and 72 us, 5.59 TB/s; rows off 16 bytes, which go value by value, are
-// bound by instructions (4099x777 fp32: forward 9.4 us, backward 12.9 us). A row is read once and stays
+// copy): forward 8192x4096 bf16 25.4 us, 5.28 TB/s, fp32 49.4 us, 5.43 TB/s; backward 38.0
+// us, 5.30 TB/s, and 72 us, 5.58 TB/s, with 42 and 52 % of the issue slots used. Rows off 16
+// bytes go value by value, and that, not memory, sets their time (4099x777 fp32: forward 8.9
+// us, backward 13.0 us; 8192x4095 bf16 40 and 52 us). A row is read once and stays
 // in registers between the statistics and the result (the variance is the mean square
 // of the centred values, not E x^2 - mean^2, which cancels). Rows belong to groups of
 // 32..512 threads, several groups to a block where rows are short; a thread computes on
@@ -548,7 +549,8 @@ __global__ void __launch_bounds__(512) ln_backward(const LnArgs a) {
   c.finish(a, tid, size, group, groups, reinterpret_cast<float4*>(ring_smem));
 }
 
-// x and dy through the ring. The copies queued ahead of it make any other load slow
+// x and dy through the ring, a row per turn. Narrow rows pay for a warp, a wait, two copies
+// and a reduction each (65536x64 bf16 32 us, 4 us of reading and writing). The copies queued ahead of it make any other load slow
 // (a mean loaded one row ahead measured 3400 cycles of waiting per row), so mean and
 // rstd are loaded 32 rows at a time, one row per lane, 32 rows ahead.
 template <typename T, typename P, int VEC, int N, bool EXACT>
