@@ -280,7 +280,8 @@ int pkt_axpy_noalloc_status(int* code, int* task_index, int* detail);
 /* ---- stand-alone operators ---------------------------------------------- */
 /* These run on the current device and in the order of `stream`; every pointer is
  * memory of that device (checked: a host pointer or another device's memory is
- * PKT_ERR_ARGS). They allocate nothing and may be captured into a CUDA graph
+ * PKT_ERR_ARGS, and so is what the captured graph will allocate itself, by an
+ * allocation node of the same capture: it is not memory yet). They allocate nothing and may be captured into a CUDA graph
  * (pkt_adamw_create and pkt_ops_status, which allocate or synchronise, may not).
  * A descriptor is read during the call only. Outputs must not overlap inputs
  * unless an operator says so. Only a result's own rows and columns are written. Of
@@ -508,7 +509,8 @@ int pkt_mlp_set_grad_scale(pkt_mlp* m, float scale);
  * pkt_mlp_apply_update then update the fp32 masters (and their bf16 copies) with it,
  * with the engine's lr and gradient scale; weight decay is for the weights, not the
  * biases. Starts with empty states and step 0; cfg = NULL goes back to SGD. A call that
- * fails leaves what was set before. pkt_mlp_set_params keeps the states. Synchronises
+ * fails leaves what was set before. pkt_mlp_set_params keeps the states, which (with
+ * their step count) are the engine's own and cannot be read or set. Synchronises
  * the device. */
 typedef struct pkt_mlp_adamw {
   double beta1, beta2, eps;

@@ -18,7 +18,9 @@ int op_device(int* dev, int* sms, int** status = nullptr);
 // Raises a kernel's shared-memory limit, once per kernel and device.
 int op_shared_memory(const void* kernel, std::atomic<uint64_t>* done, int dev, int bytes);
 // `p` is memory of device `dev` (or managed memory), so that a host pointer or
-// another GPU's buffer is an error here and not a fault in the kernel. Null passes.
+// another GPU's buffer is an error here and not a fault in the kernel. Null passes. Until
+// a graph has run, memory of its own allocation nodes looks like any unknown address and
+// is refused with them.
 int op_check_memory(const void* p, const char* what, int dev);
 // cuTensorMapEncodeTiled, looked up once; null when the driver has none.
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

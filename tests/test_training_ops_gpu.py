@@ -314,3 +314,37 @@ print("ok")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_memory_that_a_graph_will_allocate_is_refused():
+    """The address of an allocation node is no memory yet: refused, and the capture goes on."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, pkt_b200 as pk
+x = torch.randn(64, 256, device="cuda"); y = torch.zeros_like(x)
+def norm(a, b, s):
+    pk.layernorm_forward(pk.LayerNormDesc(rows=64, cols=256, dtype=pk.DTYPE_F32, param_dtype=pk.DTYPE_F32, eps=1e-5, x=a.data_ptr(), ldx=256,
+                                          y=b.data_ptr(), ldy=256), s)
+st = torch.cuda.Stream(); torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+refused = ""
+with torch.cuda.graph(g, stream=st):
+    t = x * 1.0
+    try:
+        norm(t, y, st.cuda_stream)
+    except pk.PktError as e:
+        refused = str(e)
+    norm(x, y, st.cuda_stream)
+assert "x is not device memory" in refused, refused
+g.replay(); torch.cuda.synchronize()
+c = x.double() - x.double().mean(1, keepdim=True)
+want = c / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5)
+# 96 u rstd max|x| (1 + |h|) with |x| and |h| below 5.5 and rstd below 1.3: 2.7e-4
+assert x.abs().max() < 5 and (y.double() - want).abs().max() <= 2.7e-4
+print("ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTORCH_CUDA_ALLOC_CONF": "backend:cudaMallocAsync"})
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
